@@ -1,0 +1,42 @@
+// out[x] = sum over s of in[s][x]: fp32 summed in 64 bits and rounded once, in a fixed order.  Used for gradients of what
+// several workgroups share: heads that share keys (few slices, many columns), norm weights, a decay that all tokens share
+// (many slices, few columns).  A workgroup takes `cw` columns and deals the slices to its 256 / cw rows of threads; with
+// more than one part each part sums a range of slices into its own row of `out` (fp32), and a second launch joins them.
+#include <hip/hip_runtime.h>
+
+typedef long long i64;
+
+struct Args {
+  const float* in;
+  char* out;
+  i64 S, X, type, cw, parts;       // type: 0 bfloat16, 1 float16, 2 float32; cw: a power of two from 1 to 256
+};
+
+extern "C" __global__ void __launch_bounds__(256) slice_sum(Args a) {
+  __shared__ double part[256];
+  const int tid = threadIdx.x, cw = (int)a.cw, col = tid % cw, row = tid / cw, nr = 256 / cw;
+  const i64 groups = (a.X + cw - 1) / cw, x = (i64)(blockIdx.x % groups) * cw + col, pt = blockIdx.x / groups;
+  const i64 per = (a.S + a.parts - 1) / a.parts, s0 = pt * per, s1 = s0 + per < a.S ? s0 + per : a.S;
+  double s = 0.0;
+  if (x < a.X) {
+    i64 i = s0 + row;
+    for (; i + 3 * nr < s1; i += 4 * nr) {
+      const float v0 = a.in[i * a.X + x], v1 = a.in[(i + nr) * a.X + x], v2 = a.in[(i + 2 * nr) * a.X + x], v3 = a.in[(i + 3 * nr) * a.X + x];
+      s += (double)v0 + (double)v1 + ((double)v2 + (double)v3);
+    }
+    for (; i < s1; i += nr) s += (double)a.in[i * a.X + x];
+  }
+  part[tid] = s;
+  __syncthreads();
+  for (int n = nr / 2; n > 0; n /= 2) {
+    if (row < n) part[tid] += part[tid + n * cw];
+    __syncthreads();
+  }
+  if (row == 0 && x < a.X) {
+    const float v = (float)part[col];
+    const i64 at = pt * a.X + x;
+    if (a.type == 2) ((float*)a.out)[at] = v;
+    else if (a.type == 1) ((_Float16*)a.out)[at] = (_Float16)v;
+    else ((__bf16*)a.out)[at] = (__bf16)v;
+  }
+}

@@ -1,0 +1,402 @@
+"""Linear attention with a decay for each head, as block products on the matrix cores.
+
+    S_t = exp(g_t) S_(t-1) + v_t k_t^T,    y_t = scale * S_t q_t
+
+The recurrence of `ops.retention` and `ops.mamba2` (and of `ops.gla` with one gate per head), whose decay is a number per
+token and head: a block of tokens is then a handful of matrix products, where `jit` walks the sequence a token at a time.
+Recurrences whose decay differs along the state's columns, or that read the state to update it (delta rules), are `jit`'s.
+
+    y, state = linear_attention(q, k, v, g, state)              # a prompt, or training (differentiable)
+    y = linear_attention_step(q, k, v, g, state)                # one token; `state` is updated in place
+
+The kernels are in csrc/linear_attention.hip.  Like the compiled operators they run on the GPU only, on the current stream of
+the tensors' device, without synchronising, and can be captured into a HIP graph after a first call with the same types
+and head sizes; `linear_attention.naive` and `linear_attention.naive_fp64` are the per-token loop in plain PyTorch.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch as th
+
+from . import handwritten as hw
+from .handwritten import DTYPES, require
+
+SOURCE = 'linear_attention.hip'
+MAX_HEAD = 256                  # largest M and N
+WIDTHS = (64, 128, 256)         # what M and N are padded to
+WORKGROUPS = 512                # two per compute unit: below this a sequence is split into segments
+MAX_SEGMENTS = 16
+
+# argument blocks (see the structs in the source): Tensor 6 fields, Gate 5, States 6
+_FW = '6q6q6q5q6q6qqqqq8qd'
+_JOB = '6q6q6q6qqqq4qq'
+_WALK = _JOB + _JOB + '5qq7qd'
+_GRAD = '6q6q6q6q5qqqqqqqq8qd'
+_STEP = '6q6q6q5q6qq8qd'
+
+
+def _width(n: int) -> int:
+    return next(w for w in WIDTHS if n <= w)
+
+
+def _block(dtype: th.dtype, width: int) -> int:
+    """Tokens per block: 64, and 32 where the operands' parts (or 256 columns) would leave LDS for less than two
+    workgroups per compute unit."""
+    return 64 if dtype == th.bfloat16 and width <= 128 else 32
+
+
+def _grad_block(dtype: th.dtype) -> int:
+    """The same for the gradient kernel, which holds two operand tiles only."""
+    return 64 if dtype == th.bfloat16 else 32
+
+
+def _fw_defines(dtype, N):
+    w = _width(N)
+    return (('KERNEL_FW', 1), ('IN', DTYPES[dtype]), ('WA', w), ('L', _block(dtype, w)))
+
+
+def _walk_defines(dtype, width, block):
+    return (('KERNEL_WALK', 1), ('IN', DTYPES[dtype]), ('WA', _width(width)), ('L', block))
+
+
+def _grad_waves(M, N):
+    return 8 if max(_width(M), _width(N)) >= 128 else 4
+
+
+def _grad_defines(dtype, M, N):
+    return (('KERNEL_GRAD', 1), ('IN', DTYPES[dtype]), ('WA', _width(M)), ('WB', _width(N)), ('L', _grad_block(dtype)), ('NW', _grad_waves(M, N)))
+
+
+def _step_defines(dtype):
+    return (('KERNEL_STEP', 1), ('IN', DTYPES[dtype]))
+
+
+def builds():
+    """Every code object of this module: (source, kernel, defines)."""
+    out = []
+    for dt in DTYPES:
+        for w in WIDTHS:
+            out.append((SOURCE, 'la_fw', _fw_defines(dt, w)))
+            for block in {_block(dt, w), _grad_block(dt)}:
+                out.append((SOURCE, 'la_walk', _walk_defines(dt, w, block)))
+            out += [(SOURCE, 'la_grad', _grad_defines(dt, m, w)) for m in WIDTHS]
+        out.append((SOURCE, 'la_step', _step_defines(dt)))
+    return out
+
+
+# ------------------------------------------------------------------ argument blocks
+def _tensor(t: th.Tensor, batch: int, time: Optional[int], head: int):
+    sb, sh, sn = t.stride(batch), t.stride(head), t.stride(-1)
+    st = 0 if time is None else t.stride(time)
+    size = t.element_size()
+    wide = sn == 1 and t.shape[-1] % 8 == 0 and t.data_ptr() % 16 == 0 and sb * size % 16 == 0 and st * size % 16 == 0 and sh * size % 16 == 0
+    return t.data_ptr(), sb, st, sh, sn, int(wide)
+
+
+def _btH(t):
+    return _tensor(t, 0, 1, 2)
+
+
+def _gate(g: th.Tensor):
+    code = DTYPES[g.dtype]
+    if g.ndim == 1:
+        return g.data_ptr(), 0, 0, g.stride(0), code
+    if g.ndim == 2:
+        return g.data_ptr(), g.stride(0), 0, g.stride(1), code
+    return g.data_ptr(), g.stride(0), g.stride(1), g.stride(2), code
+
+
+def _states(s: Optional[th.Tensor]):
+    return (0, 0, 0, 0, 0, 2) if s is None else (s.data_ptr(), *s.stride(), DTYPES[s.dtype])
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _segments(groups: int, blocks: int) -> Tuple[int, int]:
+    """(segments, blocks per segment) of a walk over `blocks` blocks by `groups` workgroups side by side."""
+    n = min(-(-WORKGROUPS // max(groups, 1)), blocks // 4, MAX_SEGMENTS)
+    if n <= 1:
+        return 1, blocks
+    per = -(-blocks // n)
+    return -(-blocks // per), per
+
+
+# ------------------------------------------------------------------ launches
+def _forward(q, k, v, g, state, lengths, scale):
+    B, T, Hk, N = k.shape
+    H, M = v.shape[2], v.shape[3]
+    dev = q.device
+    y = th.empty((B, T, H, M), dtype=v.dtype, device=dev)
+    out = th.empty((B, H, M, N), dtype=th.float32, device=dev) if state is None else th.empty_like(state)
+    defines = _fw_defines(q.dtype, N)
+    width, L = defines[2][1], defines[3][1]
+    blocks, tiles = -(-T // L), -(-M // 64)
+    nseg, per = _segments(B * H * tiles, blocks)
+    local = totals = None
+    gate, s0 = _gate(g), _states(state)
+    if nseg > 1:
+        local = th.empty(B * H * (nseg - 1) * tiles * 64 * width, dtype=th.float32, device=dev)
+        totals = th.empty(B * H * (nseg - 1), dtype=th.float64, device=dev)
+        job = (*_btH(k), *_btH(v), *_states(None), *_states(None), 0, local.data_ptr(), totals.data_ptr(), N, M, Hk, H, 0)
+        _walk(dev, q.dtype, N, L, [job], gate, lengths, B, T, H, nseg, per, True, tiles, scale)
+    groups = B * H * nseg
+    hw.launch(hw.kernel(dev, SOURCE, 'la_fw', defines), dev, -(-groups // 8) * 8 * tiles, 256, _FW,
+              *_btH(q), *_btH(k), *_btH(v), *gate, *s0, *_states(out), y.data_ptr(), _ptr(lengths), _ptr(local), _ptr(totals),
+              B, T, H, Hk, M, N, nseg, per, scale)
+    return y, out
+
+
+_NO_JOB = (0,) * 32
+
+
+def _walk(dev, dtype, width, L, jobs, gate, lengths, B, T, H, nseg, per, only_local, tiles, scale):
+    groups = B * H * (nseg - 1 if only_local else nseg)
+    flat = [*jobs[0], *(jobs[1] if len(jobs) > 1 else _NO_JOB)]
+    hw.launch(hw.kernel(dev, SOURCE, 'la_walk', _walk_defines(dtype, width, L)), dev, -(-groups // 8) * 8 * tiles, 256, _WALK,
+              *flat, *gate, _ptr(lengths), B, T, H, nseg, per, int(only_local), tiles, scale, grid_y=len(jobs))
+
+
+def _backward(q, k, v, g, state, lengths, dy, dstate, scale, need_g, need_state):
+    B, T, Hk, N = k.shape
+    H, M = v.shape[2], v.shape[3]
+    dev, dt = q.device, q.dtype
+    defines = _grad_defines(dt, M, N)
+    wm, L = defines[2][1], defines[4][1]
+    blocks, tiles = -(-T // L), -(-N // 64)
+    gate = _gate(g)
+    dq, dk, dv = (th.empty(x.shape, dtype=dt, device=dev) for x in (q, k, v))
+    ds = None
+    if need_state:
+        ds = th.empty_like(state)
+    # the state in front of every block and the gradient of the one behind it
+    marks = th.empty((2, B * H * blocks * -(-N // 16) * 16 * wm), dtype=th.float32, device=dev)
+    nseg, per = _segments(2 * B * H * tiles, blocks)
+    local = totals = None
+    if nseg > 1:
+        local = th.empty((2, B * H * (nseg - 1) * tiles * 64 * wm), dtype=th.float32, device=dev)
+        totals = th.empty((2, B * H * (nseg - 1)), dtype=th.float64, device=dev)
+
+    def jobs(only_local):
+        def one(i, a, b, init, fin):
+            scratch = (0, 0) if local is None else (local[i].data_ptr(), totals[i].data_ptr())
+            return (*_btH(a), *_btH(b), *_states(init), *_states(fin), 0 if only_local else marks[i].data_ptr(), *scratch, M, N, H, Hk, i)
+        return [one(0, v, k, state, None), one(1, dy, q, dstate, ds)]
+
+    for only_local in ((True, False) if nseg > 1 else (False,)):
+        _walk(dev, dt, M, L, jobs(only_local), gate, lengths, B, T, H, nseg, per, only_local, tiles, scale)
+    # heads that share a query and key: one workgroup sums what it can of them, as long as the chip stays full
+    share = H // Hk
+    slices = 1
+    while slices < share and B * blocks * Hk * slices < WORKGROUPS:
+        slices *= 2
+    slices = min(slices, share)
+    slices = -(-share // -(-share // slices))
+    if slices > 1:
+        part = th.empty((2, slices, B, T, Hk, N), dtype=th.float32, device=dev)
+        pq, pk = part[0], part[1]
+    else:
+        pq, pk = dq, dk
+    per_head = g.ndim == 1
+    dg = dg_out = None
+    if need_g:
+        dg_out = dg = th.empty(g.shape, dtype=g.dtype, device=dev)
+        if per_head:
+            dg_out = th.empty((B, T, H), dtype=th.float32, device=dev)
+    hw.launch(hw.kernel(dev, SOURCE, 'la_grad', defines), dev, blocks * slices * B * Hk, 64 * defines[5][1], _GRAD,
+              *_btH(q), *_btH(k), *_btH(v), *_btH(dy), *gate, marks[0].data_ptr(), marks[1].data_ptr(), pq.data_ptr(), pk.data_ptr(),
+              dv.data_ptr(), _ptr(dg_out), _ptr(lengths), B, T, H, Hk, M, N, slices, 2 if dg_out is None else DTYPES[dg_out.dtype], scale)
+    if slices > 1:
+        hw.slice_sum(pq, slices, dq)
+        hw.slice_sum(pk, slices, dk)
+    if need_g and per_head:
+        hw.slice_sum(dg_out, B * T, dg)
+    return dq, dk, dv, dg, ds
+
+
+def _step(q, k, v, g, state, scale):
+    B, Hk, N = k.shape
+    H, M = v.shape[1], v.shape[2]
+    dev = q.device
+    y = th.empty((B, H, M), dtype=v.dtype, device=dev)
+    size = state.element_size()
+    ve = 16 // size
+    wide = state.stride(3) == 1 and N % ve == 0 and state.data_ptr() % 16 == 0 and all(state.stride(i) * size % 16 == 0 for i in range(3))
+    lanes = 1
+    while lanes < 64 and lanes * (ve if wide else 1) < N:
+        lanes *= 2
+    rows = min(M, 256 // lanes * 4)
+    hw.launch(hw.kernel(dev, SOURCE, 'la_step', _step_defines(q.dtype)), dev, B * H * -(-M // rows), 256, _STEP,
+              *_tensor(q, 0, None, 1), *_tensor(k, 0, None, 1), *_tensor(v, 0, None, 1), *_gate(g), *_states(state), y.data_ptr(),
+              B, H, Hk, M, N, int(wide), lanes, rows, scale)
+    return y
+
+
+# ------------------------------------------------------------------ operators
+_lib = th.library.Library('flex_rnn', 'FRAGMENT')
+_lib.define('linear_attention(Tensor q, Tensor k, Tensor v, Tensor g, Tensor? state, Tensor? lengths, float scale) -> (Tensor, Tensor)')
+_lib.define('linear_attention_backward(Tensor q, Tensor k, Tensor v, Tensor g, Tensor? state, Tensor? lengths, Tensor dy, Tensor? dstate, '
+            'float scale, bool need_g, bool need_state) -> (Tensor, Tensor, Tensor, Tensor, Tensor)')
+_lib.define('linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor g, Tensor(a!) state, float scale) -> Tensor')
+
+
+def _backward_op(q, k, v, g, state, lengths, dy, dstate, scale, need_g, need_state):
+    out = _backward(q, k, v, g, state, lengths, dy, dstate, scale, need_g, need_state)
+    return tuple(q.new_empty(0) if x is None else x for x in out)       # (an operator returns tensors)
+
+
+_lib.impl('linear_attention', _forward, 'CUDA')
+_lib.impl('linear_attention_backward', _backward_op, 'CUDA')
+_lib.impl('linear_attention_step', _step, 'CUDA')
+
+
+@th.library.register_fake('flex_rnn::linear_attention', lib=_lib)
+def _(q, k, v, g, state, lengths, scale):
+    B, T, H, M = v.shape
+    return (v.new_empty((B, T, H, M)), v.new_empty((B, H, M, k.shape[3]), dtype=th.float32) if state is None else th.empty_like(state))
+
+
+@th.library.register_fake('flex_rnn::linear_attention_backward', lib=_lib)
+def _(q, k, v, g, state, lengths, dy, dstate, scale, need_g, need_state):
+    return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), g.new_empty(g.shape) if need_g else q.new_empty(0),
+            th.empty_like(state) if need_state else q.new_empty(0))
+
+
+@th.library.register_fake('flex_rnn::linear_attention_step', lib=_lib)
+def _(q, k, v, g, state, scale):
+    return v.new_empty(v.shape)
+
+
+_fw_op = th.ops.flex_rnn.linear_attention.default
+_bw_op = th.ops.flex_rnn.linear_attention_backward.default
+_step_op = th.ops.flex_rnn.linear_attention_step.default
+
+
+class _LinearAttention(th.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, state, lengths, scale):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, g, state, lengths)
+        ctx.scale = scale
+        return _fw_op(q, k, v, g, state, lengths, scale)
+
+    @staticmethod
+    @th.autograd.function.once_differentiable
+    def backward(ctx, dy, dstate):
+        q, k, v, g, state, lengths = ctx.saved_tensors
+        if dy is None and dstate is None:
+            return (None,) * 7
+        if dy is None:
+            dy = th.zeros_like(v)
+        need = ctx.needs_input_grad
+        dq, dk, dv, dg, ds = _bw_op(q, k, v, g, state, lengths, dy, dstate, ctx.scale, need[3], need[4])
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dg if need[3] else None, ds if need[4] else None, None, None
+
+
+def _check(q, k, v, g, state, lead, what):
+    """Argument checks shared by the prompt and the single-token form; `lead`: the dimensions in front of the heads."""
+    n = len(lead)
+    names = '[' + ', '.join(lead) + (', ' if lead else '')
+    require(q.ndim == n + 2 and k.ndim == n + 2 and v.ndim == n + 2, f'{what}: q and k are {names}Hk, N] and v is {names}H, M]')
+    require(q.shape == k.shape, f'{what}: q {list(q.shape)} and k {list(k.shape)} differ')
+    require(q.shape[:n] == v.shape[:n], f'{what}: q {list(q.shape)} and v {list(v.shape)} differ in {names[1:-2]}')
+    B, Hk, N = q.shape[0], q.shape[-2], q.shape[-1]
+    H, M = v.shape[-2], v.shape[-1]
+    require(Hk >= 1 and H >= 1 and H % Hk == 0, f'{what}: {H} heads of v do not divide into {Hk} heads of q and k')
+    require(1 <= N <= MAX_HEAD and 1 <= M <= MAX_HEAD, f'{what}: head sizes from 1 to {MAX_HEAD} (q and k have {N}, v has {M})')
+    require(q.dtype in DTYPES and q.dtype == k.dtype == v.dtype, f'{what}: q, k and v are of one type, bfloat16, float16 or float32 '
+            f'(got {q.dtype}, {k.dtype}, {v.dtype})')
+    require(g.dtype in (q.dtype, th.float32), f'{what}: g is float32 or of the type of q (got {g.dtype})')
+    require(tuple(g.shape) in ((H,), (*v.shape[:n], H)), f'{what}: g is [H] or {names}H] with H = {H} (got {list(g.shape)})')
+    if state is not None:
+        require(tuple(state.shape) == (B, H, M, N), f'{what}: the state is [B, H, M, N] = {[B, H, M, N]} (got {list(state.shape)})')
+        require(state.dtype in (q.dtype, th.float32), f'{what}: the state is float32 or of the type of q (got {state.dtype})')
+
+
+def _check_device(tensors, what):
+    dev = tensors[0].device
+    require(dev.type in ('cuda', 'meta'), f'{what} runs on the GPU only (got a {dev} tensor); `.naive` is the plain PyTorch loop')
+    for t in tensors[1:]:
+        require(t is None or t.device == dev, f'{what}: all tensors must live on the same device ({t.device if t is not None else ""} and {dev})')
+
+
+def linear_attention(q: th.Tensor, k: th.Tensor, v: th.Tensor, g: th.Tensor, state: Optional[th.Tensor] = None, *,
+                     lengths: Optional[th.Tensor] = None, scale: float = 1.0) -> Tuple[th.Tensor, th.Tensor]:
+    """`S_t = exp(g_t) S_(t-1) + v_t k_t^T`, `y_t = scale * S_t q_t` over whole sequences; returns `(y, final state)`.
+
+    q, k    [B,T,Hk,N]; Hk divides H (heads h * Hk // H share a query and key)
+    v       [B,T,H,M], of the same type (bfloat16, float16, float32); M and N from 1 to 256, T from 0
+    g       the decay's logarithm, [B,T,H] or [H], float32 or the type of q; -inf forgets everything before the token
+    state   [B,H,M,N], float32 or the type of q; None: zero, and the final state is float32
+    lengths [B], int64 or int32: sequence b ends after `lengths[b]` tokens (clamped to 0..T); what is behind is not
+            looked at, its `y` and gradients are zero, and the final state is the one after the last real token
+
+    Any strides.  Sums and the state are fp32.  Differentiable once in q, k, v, g and state; gradients are deterministic.
+    """
+    _check(q, k, v, g, state, ('B', 'T'), 'linear_attention')
+    _check_device((q, k, v, g, state, lengths), 'linear_attention')
+    if lengths is not None:
+        require(tuple(lengths.shape) == (q.shape[0],) and lengths.dtype in (th.int64, th.int32),
+                f'linear_attention: lengths is int64 or int32 [B] = [{q.shape[0]}] (got {lengths.dtype} {list(lengths.shape)})')
+        lengths = lengths.to(th.int64).contiguous()
+    if th.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or (state is not None and state.requires_grad)):
+        return _LinearAttention.apply(q, k, v, g, state, lengths, float(scale))
+    return _fw_op(q, k, v, g, state, lengths, float(scale))
+
+
+def linear_attention_step(q: th.Tensor, k: th.Tensor, v: th.Tensor, g: th.Tensor, state: th.Tensor, *, scale: float = 1.0) -> th.Tensor:
+    """One token of `linear_attention` for decoding: `state` [B,H,M,N] is updated in place, y [B,H,M] is returned.
+
+    q, k [B,Hk,N], v [B,H,M], g [B,H] or [H]; types as there.  Any strides, except that no two elements of the state may
+    share memory.  Not differentiable: with T = 1, `linear_attention` is.
+    """
+    _check(q, k, v, g, state, ('B',), 'linear_attention_step')
+    _check_device((q, k, v, g, state), 'linear_attention_step')
+    require(not th.is_grad_enabled() or not any(t.requires_grad for t in (q, k, v, g, state)),
+            'linear_attention_step updates the state in place and cannot be differentiated: use linear_attention, or th.no_grad()')
+    require(not _overlaps(state), 'linear_attention_step: elements of the state share memory')
+    return _step_op(q, k, v, g, state, float(scale))
+
+
+def _overlaps(t: th.Tensor) -> bool:
+    """Whether two indices of `t` may name the same element (the dimensions do not nest)."""
+    if t.is_contiguous():
+        return False
+    end = 0
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if stride <= end:
+            return True
+        end += stride * (size - 1)
+    return False
+
+
+def _naive(q, k, v, g, state=None, *, lengths=None, scale=1.0, dtype=th.float32):
+    """The same operator as a loop over tokens in plain PyTorch (any device, differentiable), computed in `dtype`."""
+    _check(q, k, v, g, state, ('B', 'T'), 'linear_attention')
+    B, T, Hk, N = q.shape
+    H, M = v.shape[2:]
+    s_dtype = th.float32 if state is None else state.dtype
+    S = th.zeros(B, H, M, N, dtype=dtype, device=q.device) if state is None else state.to(dtype)
+    ys = []
+    for t in range(T):
+        qt, kt = (x[:, t].to(dtype).repeat_interleave(H // Hk, 1)[..., None, :] for x in (q, k))
+        gt = g.to(dtype).expand(B, H) if g.ndim == 1 else g[:, t].to(dtype)
+        new = gt.exp()[..., None, None] * S + v[:, t].to(dtype)[..., None] * kt
+        yt = (new * qt).sum(-1) * scale
+        if lengths is not None:
+            real = (t < lengths)[:, None, None]
+            new, yt = th.where(real[..., None], new, S), th.where(real, yt, 0.0)
+        S = new
+        ys.append(yt)
+    y = th.stack(ys, 1) if ys else v.new_empty(B, 0, H, M, dtype=dtype)
+    return y.to(v.dtype), S.to(s_dtype)
+
+
+def _naive_fp64(*args, **kwargs):
+    return _naive(*args, **kwargs, dtype=th.double)
+
+
+linear_attention.naive = _naive
+linear_attention.naive_fp64 = _naive_fp64
