@@ -9,27 +9,40 @@
 //
 // so a block costs matrix products only, and the state is read and written once per L tokens.
 //
-// Compiled once per (IN, RP_, L, W..) by flex_rnn_amd/linear.py, which passes
-//   IN    element type of q, k, v, dy: 0 bfloat16, 1 float16, 2 float32
-//   WA    padded width (32, 64, 128 or 256) of the operand that every wave reads whole
-//   WB    the same of the other operand (gradient kernel only)
-//   L     tokens per block (32 or 64)
-//   KERNEL_FW / KERNEL_WALK / KERNEL_GRAD / KERNEL_STEP: which kernel this code object holds
+// The gradients are the same walk in other roles (dy already scaled; X the gradient of the state):
+//
+//     dq_i = sum_{j<=i} exp(G_i - G_j) (dy_i.v_j) k_j + exp(G_i) S^T dy_i              forwards,  (q, k, v) <- (dy, v, k)
+//     dk_j = sum_{i>=j} exp(G_i - G_j) (v_j.dy_i) q_i + exp(G_L - G_j) X^T v_j         backwards, (q, k, v) <- (v, dy, q)
+//     dv_j = sum_{i>=j} exp(G_i - G_j) (k_j.q_i) dy_i + exp(G_L - G_j) X k_j           backwards, (q, k, v) <- (k, q, dy)
+//
+// so one kernel, la_block, computes y and all three; backwards, a sequence is read from its end and the decay of a position
+// is the one of the token behind it.
+//
+// Compiled per set of constants by flex_rnn_amd/linear.py, which passes
+//   KERNEL_BLOCK / KERNEL_GATE / KERNEL_STEP   which kernel this code object holds
+//   IN     element type of q, k, v, dy: 0 bfloat16, 1 float16, 2 float32
+//   W      padded width (64, 128 or 256) of q and k
+//   OUT    0: the state alone (what a segment of a sequence leaves behind)
+//   DOTS   1: also what the gradient of g is made of
+//   NBUF   operand tiles in LDS: 2 lets a block's operands arrive while the one before is read, 1 saves LDS
+//   OCC    waves per SIMD to compile for
 //
 // Numbers on the matrix cores.  All products are v_mfma_f32_16x16x32_bf16: fp32 sums of bfloat16 factors.  A factor with
 // more bits is a sum of RP bfloat16 parts (float16: 2, float32: 3; the parts hold every bit, because each takes the leading
 // 8 bits of what is left), and a product of two such factors is the sum of the products of their parts, less those below the
 // last bit that counts.  The bfloat16 exponent is that of float32, so nothing overflows on the way that would not in float32.
 //   - factors read from memory are exact;
-//   - the decayed products P = exp(G_i - G_j) q_i.k_j are rounded to RP parts (one rounding to the inputs' own precision,
-//     2^-9 of the value on average below half a step, where y is rounded to the same type anyway);
-//   - the decayed v (or k) that enters a state has three parts: the state is an fp32 result even where the inputs are not.
+//   - the decayed products P = exp(G_i - G_j) q_i.k_j are rounded to RP parts: one rounding to the inputs' own precision,
+//     as large as the one of the result that they are summed into;
+//   - the state, where it is a factor, is rounded to RP parts too; to three where the product is part of g's gradient, whose
+//     type may be float32 with 16-bit inputs;
+//   - the decayed v that enters the state has three parts: the state is an fp32 result even where the inputs are not.
 // The state itself stays in fp32 accumulators for the whole sequence.
 //
 // Layout.  Operand tiles sit in LDS as [token][column], one plane per part.  The matrix instruction's reduction index may be
 // permuted as long as both factors use the same order; everything here uses the order of its own results - in a block of 32,
 // lane group g = lane/16 holds {4g..4g+3, 16+4g..16+4g+3} - so an accumulator tile becomes an operand without leaving
-// its registers (the state in y, checkpoints in the gradients), and ds_read_b64_tr_b16 delivers the same order for
+// its registers, and ds_read_b64_tr_b16 delivers the same order for
 // operands whose reduction index runs down a tile's rows.  Row strides: 4 (tiles read along rows) or 8 (tiles read
 // down columns) dwords modulo 64, which spreads the 16 rows that a half wave touches over all 64 banks.
 #include <hip/hip_runtime.h>
@@ -48,6 +61,7 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 
 #define DEV static __device__ __forceinline__
 #define DEV_MEMBER __device__ __forceinline__
+#define FENCE __builtin_amdgcn_sched_barrier(0)
 
 #ifndef IN
 #error "IN is not defined"
@@ -55,6 +69,7 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 
 constexpr int ESZ = IN == 2 ? 4 : 2;          // bytes per element of q, k, v, dy
 constexpr int RP = IN + 1;                    // bfloat16 parts of such an element
+constexpr int L = 32;                         // tokens per block
 constexpr double LOG2E = 1.4426950408889634;
 constexpr double NO_DECAY = -200.0;           // exp of less is zero in fp32; keeps the sums of logarithms finite
 
@@ -65,9 +80,9 @@ struct Tensor {      // strides in elements; `vec`: 16-byte loads of 8 (4 of fp3
   i64 sb, st, sh, sn, vec;
 };
 
-struct States {      // [B,H,M,N] of a type, or p = null
+struct States {      // element (row, column) of a head's state, of a type; or p = null
   char* p;
-  i64 sb, sh, sm, sn, type;
+  i64 sb, sh, sr, sc, type;
 };
 
 DEV float as_f(u32 x) { return __uint_as_float(x); }
@@ -136,6 +151,20 @@ DEV f4 mul(const Frag<PA>& a, const Frag<PB>& b, f4 c) {
     }
   return c;
 }
+// the same for N left factors, one after the other within a pair of parts: no product waits for the one before it
+template <int N, int LIM, int PA, int PB>
+DEV void mul_each(const Frag<PA>* a, const Frag<PB>& b, f4* c) {
+#pragma unroll
+  for (int s = LIM; s >= 0; s--)
+#pragma unroll
+    for (int i = 0; i < PA; i++) {
+      const int j = s - i;
+      if (j >= 0 && j < PB)
+#pragma unroll
+        for (int n = 0; n < N; n++)
+          c[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bh8, a[n].d[i]), __builtin_bit_cast(bh8, b.d[j]), c[n], 0, 0, 0);
+    }
+}
 constexpr int RAW = RP == 1 ? 0 : 2;           // both factors exact
 constexpr int CALC = RP - 1;                   // one factor rounded to RP parts
 
@@ -149,39 +178,39 @@ DEV v4s tr_read(const u16* p) {
 }
 
 // lane (p = lane % 16, g = lane / 16) gets column c0 + p, rows r0 + {4g..4g+3, 16+4g..16+4g+3}
-template <int STR, int ROWS>
+template <int STR>
 DEV Frag<RP> down(const u16* tile, int r0, int c0, int lane) {
   const int p = lane & 15, g = lane >> 4;
   const u16* at = tile + (r0 + 4 * g + (p >> 2)) * STR + c0 + 4 * (p & 3);
   Frag<RP> f;
 #pragma unroll
   for (int i = 0; i < RP; i++) {
-    const v2u a = __builtin_bit_cast(v2u, tr_read(at + i * ROWS * STR));
-    const v2u b = __builtin_bit_cast(v2u, tr_read(at + i * ROWS * STR + 16 * STR));
+    const v2u a = __builtin_bit_cast(v2u, tr_read(at + i * L * STR));
+    const v2u b = __builtin_bit_cast(v2u, tr_read(at + i * L * STR + 16 * STR));
     f.d[i] = v4u{a[0], a[1], b[0], b[1]};
   }
   return f;
 }
 
 // lane (p, g) gets row r, columns c0 + {4g..4g+3, 16+4g..16+4g+3}
-template <int STR, int ROWS>
+template <int STR>
 DEV Frag<RP> along(const u16* tile, int r, int c0, int g) {
   const u16* at = tile + r * STR + c0 + 4 * g;
   Frag<RP> f;
 #pragma unroll
   for (int i = 0; i < RP; i++) {
-    const v2u a = *(const v2u*)(at + i * ROWS * STR), b = *(const v2u*)(at + i * ROWS * STR + 16);
+    const v2u a = *(const v2u*)(at + i * L * STR), b = *(const v2u*)(at + i * L * STR + 16);
     f.d[i] = v4u{a[0], a[1], b[0], b[1]};
   }
   return f;
 }
 
 // lane (p, g) gets row r, columns c0 + 8g..8g+7: where the order is free on both sides
-template <int STR, int ROWS>
+template <int STR>
 DEV Frag<RP> along8(const u16* tile, int r, int c0, int g) {
   Frag<RP> f;
 #pragma unroll
-  for (int i = 0; i < RP; i++) f.d[i] = *(const v4u*)(tile + i * ROWS * STR + r * STR + c0 + 8 * g);
+  for (int i = 0; i < RP; i++) f.d[i] = *(const v4u*)(tile + i * L * STR + r * STR + c0 + 8 * g);
   return f;
 }
 
@@ -190,28 +219,27 @@ struct Raw {         // 8 elements as they are in memory
   v4u d[ESZ / 2];
 };
 
-// `base`: the first token of the block (wave uniform); tokens from `rows` on and columns from `cols` on are zero.  Whether
-// memory is read is decided before the address is formed: nothing outside the tensor is touched.
-DEV Raw load8(const char* base, i64 st, i64 sn, bool vec, int row, int col, int rows, int cols) {
+// A tensor's block of tokens as a buffer: what is not to be read gets an offset behind its end and comes back as zero, so
+// nothing outside the tensor is touched and no branch waits.  Offsets are 32 bits within a block; the block's address is 64.
+constexpr u32 NOTHING = 0x80000000u;
+typedef __amdgpu_buffer_rsrc_t Buffer;
+DEV Buffer buffer_at(const char* base) { return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00027000); }
+
+// 8 elements from byte offset `at` on, `step` apart; those from `n` on are zero
+DEV Raw load_apart(Buffer base, u32 at, u32 step, int n) {
   Raw r;
-  if (vec) {
-    const bool ok = row < rows && col < cols;               // (cols is a multiple of 8 here)
-    const v4u* at = (const v4u*)(base + (row * st + col) * ESZ);
-    for (int i = 0; i < ESZ / 2; i++) r.d[i] = ok ? at[i] : v4u{0, 0, 0, 0};
+  u32 w[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const u32 off = e < n ? at + e * step : NOTHING;
+    if constexpr (ESZ == 4) w[e] = __builtin_amdgcn_raw_buffer_load_b32(base, off, 0, 0);
+    else w[e] = (u16)__builtin_amdgcn_raw_buffer_load_b16(base, off, 0, 0);
+  }
+  if constexpr (ESZ == 4) {
+    r.d[0] = v4u{w[0], w[1], w[2], w[3]};
+    r.d[ESZ / 2 - 1] = v4u{w[4], w[5], w[6], w[7]};
   } else {
-    u32 w[8];
-    for (int e = 0; e < 8; e++) {
-      const bool ok = row < rows && col + e < cols;
-      const char* at = base + (row * st + (col + e) * sn) * ESZ;
-      if constexpr (ESZ == 4) w[e] = ok ? *(const u32*)at : 0u;
-      else w[e] = ok ? *(const u16*)at : 0u;
-    }
-    if constexpr (ESZ == 4) {
-      r.d[0] = v4u{w[0], w[1], w[2], w[3]};
-      r.d[ESZ / 2 - 1] = v4u{w[4], w[5], w[6], w[7]};
-    } else {
-      r.d[0] = v4u{w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16};
-    }
+    r.d[0] = v4u{w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16};
   }
   return r;
 }
@@ -231,26 +259,52 @@ DEV void store_parts(u16* at, const Raw& r) {
   }
 }
 
-// a tile of ROWS tokens x W columns, staged by THREADS threads
-template <int W, int STR, int ROWS, int THREADS>
+// A tile of L tokens x W_ columns, staged by 256 threads, block after block; row r of the tile is token r, or L - 1 - r
+// backwards.  A thread's offsets within a block stay the same, only the block's address moves.
+template <int W_, int STR>
 struct Staging {
-  static constexpr int UNITS = ROWS * (W / 8);
-  static constexpr int N = (UNITS + THREADS - 1) / THREADS;
+  static constexpr int N = L * (W_ / 8) / 256, ROWS = 256 / (W_ / 8);       // pieces of a thread, and the rows between them
   Raw r[N];
+  u32 off[N], sn;
+  const char* at;           // the next block's first token
+  i64 step;
+  int token, dir;           // of the thread's first piece
+  bool vec;
+  int left;                 // columns from the thread's own on
 
-  DEV_MEMBER void load(const char* base, const Tensor& t, int rows, int cols, int tid) {
+  DEV_MEMBER void init(const Tensor& t, const char* first, int cols, bool back, int tid) {
+    const int row = tid / (W_ / 8), col = tid % (W_ / 8) * 8;
+    const u32 st = (u32)t.st * ESZ;
+    sn = (u32)t.sn * ESZ;
+    vec = t.vec != 0;
+    token = back ? L - 1 - row : row;
+    dir = back ? -ROWS : ROWS;
+    left = cols - col;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const int u = tid + i * THREADS;
-      if (UNITS % THREADS == 0 || u < UNITS) r[i] = load8(base, t.st, t.sn, t.vec != 0, u / (W / 8), u % (W / 8) * 8, rows, cols);
+    for (int i = 0; i < N; i++) off[i] = left > 0 ? (token + i * dir) * st + col * sn : NOTHING;
+    at = first;
+    step = (back ? -L : L) * t.st * ESZ;
+  }
+  // (with vec, columns come in eights: all of a piece's are inside, or none)
+  DEV_MEMBER void load(int tokens) {
+    const Buffer from = buffer_at(at);
+    at += step;
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const u32 o = token + i * dir < tokens ? off[i] : NOTHING;
+#pragma unroll
+        for (int e = 0; e < ESZ / 2; e++) r[i].d[e] = __builtin_amdgcn_raw_buffer_load_b128(from, o + 16 * e, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) r[i] = load_apart(from, off[i], sn, token + i * dir < tokens ? left : 0);
     }
   }
   DEV_MEMBER void store(u16* tile, int tid) {
+    const int row = tid / (W_ / 8), col = tid % (W_ / 8) * 8;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const int u = tid + i * THREADS;
-      if (UNITS % THREADS == 0 || u < UNITS) store_parts<ROWS * STR>(tile + u / (W / 8) * STR + u % (W / 8) * 8, r[i]);
-    }
+    for (int i = 0; i < N; i++) store_parts<L * STR>(tile + (row + i * ROWS) * STR + col, r[i]);
   }
 };
 
@@ -273,18 +327,20 @@ DEV double dpp_or_zero(double x) {
   const int hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROW_MASK, 0xf, false);
   return __builtin_bit_cast(double, (u64)(u32)hi << 32 | (u32)lo);
 }
-DEV double scan64(double x) {                  // inclusive sums over the 64 lanes
+DEV double scan32(double x) {                  // inclusive sums over either half of the 64 lanes
   x += dpp_or_zero<0x111, 0xf>(x);             // row_shr 1, 2, 4, 8: within rows of 16
   x += dpp_or_zero<0x112, 0xf>(x);
   x += dpp_or_zero<0x114, 0xf>(x);
   x += dpp_or_zero<0x118, 0xf>(x);
-  x += dpp_or_zero<0x142, 0xa>(x);             // a row's last lane into the next row
-  x += dpp_or_zero<0x143, 0xc>(x);             // lane 31 into the upper half
-  return x;
+  return x + dpp_or_zero<0x142, 0xa>(x);       // an even row's last lane into the odd row behind it
 }
-DEV double last_lane(double x) {
+DEV double scan64(double x) {                  // over all of them
+  x = scan32(x);
+  return x + dpp_or_zero<0x143, 0xc>(x);       // lane 31 into the upper half
+}
+DEV double read_lane(double x, int lane) {
   const u64 b = __builtin_bit_cast(u64, x);
-  const u32 lo = __builtin_amdgcn_readlane((int)b, 63), hi = __builtin_amdgcn_readlane((int)(b >> 32), 63);
+  const u32 lo = __builtin_amdgcn_readlane((int)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
   return __builtin_bit_cast(double, (u64)hi << 32 | lo);
 }
 
@@ -293,38 +349,50 @@ struct Gate {        // g: [B,T,H] (or [H]: strides 0)
   i64 sb, st, sh, type;
 };
 
-DEV double gate_of(const Gate& g, i64 b, i64 h, i64 t) {
-  const double x = load_type(g.p, b * g.sb + t * g.st + h * g.sh, (int)g.type);
+// as it is in memory: what it means is asked for later, so that nothing waits for it here
+DEV u32 raw_gate(const Gate& g, i64 b, i64 h, i64 t) {
+  const i64 i = b * g.sb + t * g.st + h * g.sh;
+  return g.type == FP32 ? ((const u32*)g.p)[i] : (u32)((const u16*)g.p)[i];
+}
+DEV double gate_value(const Gate& g, u32 raw) {
+  const double x = g.type == FP32 ? as_f(raw) : g.type == FP16 ? half_to_f((u16)raw) : as_f(raw << 16);
   return x < NO_DECAY ? NO_DECAY : x;
 }
+DEV double gate_of(const Gate& g, i64 b, i64 h, i64 t) { return gate_value(g, raw_gate(g, b, h, t)); }
 
-template <int L_>
 struct Decays {
   // G * log2(e) as a sum of two floats: differences of far sums keep the precision of near ones
-  float hi[L_], lo[L_];
-  float from_start[L_], to_end[L_];            // exp(G_i), exp(G_L - G_i)
-  float all;                                   // exp(G_L)
+  alignas(16) float hi[L];
+  alignas(16) float lo[L];
+  alignas(16) float from_start[L];             // exp(G_i); the last one is the whole block's
+  alignas(16) float to_end[L];                 // exp(G_L - G_i)
 };
 
-// one wave; lane i holds token i's g (0 behind the last token)
-template <int L_>
-DEV double fill_decays(Decays<L_>& d, double g, int lane) {
-  const double G = scan64(g), end = last_lane(G);
-  if (lane < L_) {
-    const double G2 = G * LOG2E;
-    const float hi = (float)G2;
-    d.hi[lane] = hi;
-    d.lo[lane] = (float)(G2 - (double)hi);
-    d.from_start[lane] = expf((float)G);
-    d.to_end[lane] = expf((float)(end - G));
-    if (lane == 0) d.all = expf((float)end);
-  }
-  return end;
+DEV float exp2_sum(float hi, float lo) {       // 2^(hi + lo), |lo| far below 1
+  const float e = __builtin_amdgcn_exp2f(hi);
+  return e + e * (lo * 0.693147181f);
 }
 
-template <int L_>
-DEV float decay_between(const Decays<L_>& d, float hi_i, float lo_i, int j) {
-  return __builtin_amdgcn_exp2f((hi_i - d.hi[j]) + (lo_i - d.lo[j]));
+// one wave prepares two blocks: lane i of either half holds token i's g (0 behind the last token); returns the sum of g
+DEV double fill_decays(Decays* first, Decays* second, double g, int lane) {
+  const double G = scan32(g);
+  const double end0 = read_lane(G, 31), end1 = read_lane(G, 63);
+  const double G2 = G * LOG2E, E2 = (lane < L ? end0 : end1) * LOG2E;
+  Decays* d = lane < L ? first : second;
+  const int i = lane & (L - 1);
+  const float hi = (float)G2, lo = (float)(G2 - (double)hi);
+  const double to = E2 - G2;
+  d->hi[i] = hi;
+  d->lo[i] = lo;
+  d->from_start[i] = exp2_sum(hi, lo);
+  const float th = (float)to;
+  d->to_end[i] = exp2_sum(th, (float)(to - (double)th));
+  return end0 + end1;
+}
+
+DEV f4 decay_between(const Decays& d, int i, int j) {     // tokens j..j+3 to token i
+  const f4 x = (d.hi[i] - *(const f4*)(d.hi + j)) + (d.lo[i] - *(const f4*)(d.lo + j));
+  return f4{__builtin_amdgcn_exp2f(x[0]), __builtin_amdgcn_exp2f(x[1]), __builtin_amdgcn_exp2f(x[2]), __builtin_amdgcn_exp2f(x[3])};
 }
 
 // Workgroups go to the 8 XCDs in turn; the `n` workgroups of one group (which read the same operands) get numbers 8 apart
@@ -342,12 +410,6 @@ DEV i64 length_of(const i64* lengths, i64 b, i64 T) {
   return n < 0 ? 0 : n > T ? T : n;
 }
 
-DEV void tile_of(int idx, int* it, int* jt) {   // the idx-th tile on or below the diagonal, row by row
-  const int i = (idx >= 1) + (idx >= 3) + (idx >= 6);
-  *it = i;
-  *jt = idx - i * (i + 1) / 2;
-}
-
 DEV float sum16(float x) {                     // over the 16 lanes of a row
   for (int m = 1; m < 16; m <<= 1) x += __shfl_xor(x, m, 64);
   return x;
@@ -357,592 +419,488 @@ DEV float sum_groups(float x) {                // over the 4 lanes with the same
   return x + __shfl_xor(x, 32, 64);
 }
 
-// ================================================================== forward pass
-#ifdef KERNEL_FW
-// One workgroup walks the blocks of one (batch, head, segment) for 64 of the M columns of v; wave w owns 16 of them: its
-// share of the state, S^T [WA x 16], stays in accumulators.  q and k are read by every workgroup of a head (up to four,
-// on one XCD).  The next block's operands are loaded into registers while the current one is computed.
-struct FwArgs {
-  Tensor q, k, v;
-  Gate g;
-  States s0, sT;
-  char* y;                  // [B,T,H,M], contiguous
-  const i64* lengths;
-  const float* local;       // states that the segments in front leave behind, each from zero; null: one segment
-  const double* totals;     // their sums of g
-  i64 B, T, H, Hk, M, N, nseg, blocks_per_seg;
-  double scale;
-};
-
-constexpr int SQ = stride_along(WA), SK = stride_down(WA), SV = stride_down(64), SP = stride_along(L);
-constexpr int LT = L / 16, NT = WA / 16;
-
-extern "C" __global__ void __launch_bounds__(256, 2) la_fw(FwArgs a) {
-  __shared__ __attribute__((aligned(16))) u16 Q[RP * L * SQ], K[RP * L * SK], V[RP * L * SV], P[RP * L * SP];
-  __shared__ Decays<L> D;
-  const int tid = threadIdx.x, lane = tid & 63, p = lane & 15, g = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int nmt = (int)((a.M + 63) / 64);
-  i64 group;
-  int mt;
-  if (!spread(blockIdx.x, nmt, a.B * a.H * a.nseg, &group, &mt)) return;
-  const i64 bh = group / a.nseg, seg = group % a.nseg, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
-  const int m0 = mt * 64, mw = m0 + 16 * w;
-  const i64 len = length_of(a.lengths, b, a.T);
-  const i64 first = seg * a.blocks_per_seg, nblocks = (a.T + L - 1) / L;
-  const i64 last = first + a.blocks_per_seg < nblocks ? first + a.blocks_per_seg : nblocks;
-
-  f4 S[NT];                 // S^T: column m = mw + p, rows n = 16 nt + 4 g + r
-  for (int nt = 0; nt < NT; nt++)
-    for (int r = 0; r < 4; r++) {
-      const int n = 16 * nt + 4 * g + r, m = mw + p;
-      S[nt][r] = a.s0.p && m < a.M && n < a.N ? load_type(a.s0.p, b * a.s0.sb + h * a.s0.sh + m * a.s0.sm + n * a.s0.sn, (int)a.s0.type) : 0.f;
-    }
-  for (i64 s = 0; s < seg; s++) {                // the state at this segment's start
-    const i64 at = bh * (a.nseg - 1) + s;
-    const float e = expf((float)a.totals[at]);
-    const f4* from = (const f4*)a.local + (at * nmt * 4 + mt * 4 + w) * (NT * 64) + lane;
-    for (int nt = 0; nt < NT; nt++) S[nt] = S[nt] * e + from[nt * 64];
-  }
-  // (tiles above the diagonal stay zero)
-  for (int i = tid; i < RP * L * SP / 8; i += 256) *(v4u*)(P + 8 * i) = v4u{0, 0, 0, 0};
-
-  const char* qb = a.q.p + (b * a.q.sb + hk * a.q.sh) * ESZ;
-  const char* kb = a.k.p + (b * a.k.sb + hk * a.k.sh) * ESZ;
-  const char* vb = a.v.p + (b * a.v.sb + h * a.v.sh + m0 * a.v.sn) * ESZ;
-  const int vcols = a.M - m0 < 64 ? (int)(a.M - m0) : 64;
-  Staging<WA, SQ, L, 256> rq;
-  Staging<WA, SK, L, 256> rk;
-  Staging<64, SV, L, 256> rv;
-  double rg = 0.0;
-  const auto fetch = [&](i64 c) {
-    const i64 t0 = c * L;
-    const int rows = len - t0 < L ? (int)(len - t0) : L;       // (may be negative)
-    rq.load(qb + t0 * a.q.st * ESZ, a.q, rows, (int)a.N, tid);
-    rk.load(kb + t0 * a.k.st * ESZ, a.k, rows, (int)a.N, tid);
-    rv.load(vb + t0 * a.v.st * ESZ, a.v, rows, vcols, tid);
-    rg = tid < L && tid < rows ? gate_of(a.g, b, h, t0 + tid) : 0.0;
-  };
-  if (first < last) fetch(first);
-  for (i64 c = first; c < last; c++) {
-    const i64 t0 = c * L;
-    __syncthreads();
-    rq.store(Q, tid);
-    rk.store(K, tid);
-    rv.store(V, tid);
-    if (w == 0) fill_decays<L>(D, rg, lane);
-    if (c + 1 < last) fetch(c + 1);
-    __syncthreads();
-    for (int idx = w; idx < LT * (LT + 1) / 2; idx += 4) {
-      int it, jt;
-      tile_of(idx, &it, &jt);
-      f4 x = {0.f, 0.f, 0.f, 0.f};               // column i = 16 it + p, rows j = 16 jt + 4 g + r
-#pragma unroll
-      for (int ks = 0; ks < WA / 32; ks++)
-        x = mul<RAW>(along8<SK, L>(K, 16 * jt + p, 32 * ks, g), along8<SQ, L>(Q, 16 * it + p, 32 * ks, g), x);
-      const int i = 16 * it + p;
-      const float hi = D.hi[i], lo = D.lo[i];
-      for (int r = 0; r < 4; r++) {
-        const int j = 16 * jt + 4 * g + r;
-        x[r] = j <= i ? x[r] * decay_between(D, hi, lo, j) : 0.f;
-      }
-      u32 d[RP * 2];
-      split2<RP>(x[0], x[1], d, 2);
-      split2<RP>(x[2], x[3], d + 1, 2);
-      for (int q = 0; q < RP; q++) *(v2u*)(P + (q * L + i) * SP + 16 * jt + 4 * g) = v2u{d[2 * q], d[2 * q + 1]};
-    }
-    __syncthreads();
-    f4 y[LT];                                    // y^T: column i = 16 it + p, rows m = mw + 4 g + r
-    for (int it = 0; it < LT; it++) y[it] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ks = 0; ks < WA / 32; ks++) {
-      float x[8];
-      for (int r = 0; r < 4; r++) {
-        x[r] = S[2 * ks][r];
-        x[4 + r] = S[2 * ks + 1][r];
-      }
-      const Frag<RP> s = make_frag<RP>(x);
-#pragma unroll
-      for (int it = 0; it < LT; it++) y[it] = mul<CALC>(s, along<SQ, L>(Q, 16 * it + p, 32 * ks, g), y[it]);
-    }
-    for (int it = 0; it < LT; it++) y[it] *= D.from_start[16 * it + p];
-    const float all = D.all;
-    for (int nt = 0; nt < NT; nt++) S[nt] *= all;
-#pragma unroll
-    for (int jb = 0; jb < L / 32; jb++) {
-      const Frag<RP> vf = down<SV, L>(V, 32 * jb, 16 * w, lane);
-#pragma unroll
-      for (int it = 2 * jb; it < LT; it++) y[it] = mul<CALC>(vf, along<SP, L>(P, 16 * it + p, 32 * jb, g), y[it]);
-      float x[8];
-      frag_values(vf, x);
-      const f4 e0 = *(const f4*)(D.to_end + 32 * jb + 4 * g), e1 = *(const f4*)(D.to_end + 32 * jb + 16 + 4 * g);
-      for (int r = 0; r < 4; r++) {
-        x[r] *= e0[r];
-        x[4 + r] *= e1[r];
-      }
-      const Frag<3> vd = make_frag<3>(x);
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) S[nt] = mul<2>(down<SK, L>(K, 32 * jb, 16 * nt, lane), vd, S[nt]);
-    }
-    const float scale = (float)a.scale;
-    for (int it = 0; it < LT; it++) {
-      const i64 t = t0 + 16 * it + p;
-      const int m = mw + 4 * g;
-      if (t >= a.T || m >= a.M) continue;
-      f4 o = y[it] * scale;
-      if (t >= len) o = f4{0.f, 0.f, 0.f, 0.f};
-      char* at = a.y + (((b * a.T + t) * a.H + h) * a.M + m) * ESZ;
-      if (a.M % 4 == 0) {
-        if constexpr (IN == FP32) *(f4*)at = o;
-        else if constexpr (IN == BF16) *(v2u*)at = v2u{pack_rne(o[0], o[1]), pack_rne(o[2], o[3])};
-        else {
-          typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-          *(h4*)at = __builtin_convertvector(o, h4);
-        }
-      } else {
-        for (int r = 0; r < 4; r++)
-          if (m + r < a.M) store_type(at, r, IN, o[r]);
-      }
-    }
-  }
-  if (seg == a.nseg - 1)
-    for (int nt = 0; nt < NT; nt++)
-      for (int r = 0; r < 4; r++) {
-        const int n = 16 * nt + 4 * g + r, m = mw + p;
-        if (m < a.M && n < a.N) store_type(a.sT.p, b * a.sT.sb + h * a.sT.sh + m * a.sT.sm + n * a.sT.sn, (int)a.sT.type, S[nt][r]);
-      }
+// Four neighbours of a block's result, the first n of them inside; in one piece where `whole` says that rows are a multiple
+// of four long.  Nothing is written at NOTHING.
+DEV void store_wide(Buffer to, u32 off, f4 x, int n, bool whole) {
+  if (whole) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, x), to, n > 0 ? off : NOTHING, 0, 0);
+  else
+    for (int r = 0; r < 4; r++) __builtin_amdgcn_raw_buffer_store_b32(as_u(x[r]), to, r < n ? off + 4 * r : NOTHING, 0, 0);
 }
+DEV void store_in(Buffer to, u32 off, f4 x, int n, bool whole) {
+  if constexpr (IN == FP32) {
+    store_wide(to, off, x, n, whole);
+  } else {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    v2u d;
+    if constexpr (IN == BF16) d = v2u{pack_rne(x[0], x[1]), pack_rne(x[2], x[3])};
+    else d = __builtin_bit_cast(v2u, __builtin_convertvector(x, h4));
+    if (whole) __builtin_amdgcn_raw_buffer_store_b64(d, to, n > 0 ? off : NOTHING, 0, 0);
+    else
+      for (int r = 0; r < 4; r++) __builtin_amdgcn_raw_buffer_store_b16((u16)(d[r / 2] >> (r % 2 * 16)), to, r < n ? off + 2 * r : NOTHING, 0, 0);
+  }
+}
+
+// ================================================================== the walk over a sequence's blocks
+#ifdef KERNEL_BLOCK
+// One workgroup walks the blocks of one (batch, head, segment) for 64 of v's columns; wave w owns 16 of them: its share of
+// the state, S^T [W x 16], stays in accumulators.  q and k are read by every workgroup of a head (up to four, on one XCD).
+// A block: waves 0..2 form the three 16 x 16 tiles of P on and below the diagonal while wave 3 prepares the next block's
+// decays; every wave then adds the state's share of its columns of y, updates its state, and, once P is complete, adds the
+// block's own share.  The next block's operands are on their way into registers meanwhile.
+//
+// With DOTS the walk also leaves, per token, what the gradient of g is made of (see la_gate): forwards (dq) the products
+// q_i.dq_i with the block's own share taken from unrounded numbers, less the share of each j; backwards (dk) the products
+// k_j.dk_j of the state's share.  x is the operand of these products (q, k), in the 64 columns that the workgroup owns;
+// sums over column tiles are left to la_gate.  At every MARK-th block's border the state is written down too.
+#ifndef DOTS
+#define DOTS 0
 #endif
 
-// ================================================================== states only
-#ifdef KERNEL_WALK
-// X' = exp(G_L) X + sum_t e_t a_t b_t^T over the blocks of a sequence, forwards (e_t = exp(G_L - G_t): the state itself)
-// or backwards (e_t = scale exp(G_t): the state's gradient, from a = dy, b = q).  One workgroup holds 64 of b's columns,
-// wave w 16 of them times all WA of a's.  Two uses: what a segment leaves behind (`local`, from zero), and the
-// value in front of every block (`marks`) for the gradient kernel; both as accumulator tiles, fp32, in lane order.
 struct Job {
-  Tensor a, b;              // [B,T,heads,width]
-  States init, fin;         // sm: stride of a's index, sn: of b's
-  float* marks;
-  float* local;
-  double* totals;
-  i64 Wa, Wb, Ha, Hb;       // widths and heads of a and b
-  i64 back;
+  Tensor q, k, v, x;
+  States init, fin;
+  char* out;                // element (b, t, h, column): b * ob + t * ot + h / share * og + h % share * os + column
+  i64 ob, ot, og, os, share, out_type;
+  float* dots;              // [column tiles][B*H][T]
+  float* marks;             // [B*H][spans][ceil(C/16)][W/16][64][4]
+  float* local;             // [B*H][nseg-1][column tiles][4][W/16][64][4]: states that segments leave behind, from zero
+  double* totals;           // [B*H][nseg-1]: their sums of g
+  i64 Hq, Hk, Hv, Hx;       // heads of the operands
+  i64 width, C, back, pairs;      // q's and k's columns, v's columns, direction, whether dots take in P's share
+  double in_scale, out_scale;     // of what enters the state (and P), of y
 };
-struct WalkArgs {
+struct BlockArgs {
   Job job[2];
   Gate g;
   const i64* lengths;
-  i64 B, T, H, nseg, blocks_per_seg, only_local, cols_tiles;
-  double scale;
+  i64 B, T, H, nseg, per, tiles, span;    // per: blocks per segment; tiles: most column tiles of a job; span: blocks per mark
 };
 
-constexpr int SA = stride_down(WA), SB = stride_down(64);
-constexpr int AT = WA / 16;
+constexpr int NT = W / 16, LT = 2;
+constexpr int QB = RP == 1 ? (W < 128 ? W / 32 : 4) : RP == 2 ? 2 : 1;       // operands read ahead: what 32 registers hold
+constexpr int KB = RP == 1 ? 4 : RP == 2 ? 2 : 2;
+constexpr int SQ = stride_along(W), SK = stride_down(W), SV = stride_down(64), SX = stride_along(64), SP = stride_along(L);
+constexpr int SPARTS = DOTS ? 3 : RP, SLIM = DOTS ? 2 : CALC;
+constexpr int AT_K = OUT ? RP * L * SQ : 0, AT_V = AT_K + RP * L * SK, AT_X = AT_V + RP * L * SV, STAGE = AT_X + (DOTS ? RP * L * SX : 0);
 
-extern "C" __global__ void __launch_bounds__(256, 2) la_walk(WalkArgs args) {
-  __shared__ __attribute__((aligned(16))) u16 A[RP * L * SA], Bt[RP * L * SB];
-  __shared__ Decays<L> D;
-  const Job& j = args.job[blockIdx.y];
+template <int TYPE>
+DEV void load_state(f4* S, const char* from, i64 at, i64 step, int rows, int g) {
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int row = 16 * nt + 4 * g + r;
+      if (row < rows) S[nt][r] = load_type(from, at + row * step, TYPE);
+    }
+}
+template <int TYPE>
+DEV void store_state(const f4* S, float e, char* to, i64 at, i64 step, int rows, int g) {
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int row = 16 * nt + 4 * g + r;
+      if (row < rows) store_type(to, at + row * step, TYPE, S[nt][r] * e);
+    }
+}
+
+extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) {
+  __shared__ __attribute__((aligned(16))) u16 stage[NBUF][STAGE];
+  __shared__ Decays decays[4];
+#if OUT
+  __shared__ __attribute__((aligned(16))) u16 P[RP * L * SP];
+#endif
+#if DOTS
+  __shared__ float of_rows[LT][L], of_cols[LT][L], of_state[4][L];
+#endif
+  const Job& job = args.job[blockIdx.y];
   const int tid = threadIdx.x, lane = tid & 63, p = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const i64 nseg = args.only_local ? args.nseg - 1 : args.nseg;
-  const int nct = (int)((j.Wb + 63) / 64);
+  const int C = (int)job.C, ntiles = (C + 63) / 64;
+  const i64 nseg = OUT ? args.nseg : args.nseg - 1;
   i64 group;
-  int ct;
-  if (!spread(blockIdx.x, (int)args.cols_tiles, args.B * args.H * nseg, &group, &ct) || ct >= nct) return;
+  int tile;
+  if (!spread(blockIdx.x, (int)args.tiles, args.B * args.H * nseg, &group, &tile) || tile >= ntiles) return;
   const i64 bh = group / nseg, seg = group % nseg, b = bh / args.H, h = bh % args.H;
-  const i64 len = length_of(args.lengths, b, args.T);
-  const i64 nblocks = (args.T + L - 1) / L;
-  const i64 first = seg * args.blocks_per_seg;
-  const i64 last = first + args.blocks_per_seg < nblocks ? first + args.blocks_per_seg : nblocks;
-  const int c0 = ct * 64, cw = c0 + 16 * w;
+  const int c0 = tile * 64, cw = c0 + 16 * w, cols = C - c0 < 64 ? C - c0 : 64;
+  const bool back = job.back != 0;
+  const i64 T = args.T, len = length_of(args.lengths, b, T);
+  const i64 nall = (T + L - 1) / L, nreal = (len + L - 1) / L;       // blocks; blocks with a token
+  // this segment's steps: step o is block o, or nall - 1 - o backwards; those without a token only clear y
+  const i64 s0 = seg * args.per, s1 = s0 + args.per < nall ? s0 + args.per : nall;
+  const i64 first = back && s0 < nall - nreal ? (nall - nreal < s1 ? nall - nreal : s1) : s0;
+  const i64 last = back || s1 < nreal ? s1 : (nreal > s0 ? nreal : s0);
 
-  f4 X[AT];                 // column cw + p of b, rows 16 at + 4 g + r of a
-  for (int at = 0; at < AT; at++)
-    for (int r = 0; r < 4; r++) {
-      const int row = 16 * at + 4 * g + r, col = cw + p;
-      X[at][r] = !args.only_local && j.init.p && row < j.Wa && col < j.Wb
-                     ? load_type(j.init.p, b * j.init.sb + h * j.init.sh + row * j.init.sm + col * j.init.sn, (int)j.init.type) : 0.f;
-    }
-  if (!args.only_local)
-    for (i64 s = 0; s < seg; s++) {
-      const i64 at0 = bh * (args.nseg - 1) + s;
-      const float e = expf((float)j.totals[at0]);
-      const f4* from = (const f4*)j.local + (at0 * nct * 4 + ct * 4 + w) * (AT * 64) + lane;
-      for (int at = 0; at < AT; at++) X[at] = X[at] * e + from[at * 64];
-    }
-
-  const char* ab = j.a.p + (b * j.a.sb + h / (args.H / j.Ha) * j.a.sh) * ESZ;
-  const char* bb = j.b.p + (b * j.b.sb + h / (args.H / j.Hb) * j.b.sh + c0 * j.b.sn) * ESZ;
-  const int bcols = j.Wb - c0 < 64 ? (int)(j.Wb - c0) : 64;
-  Staging<WA, SA, L, 256> ra;
-  Staging<64, SB, L, 256> rb;
-  double rg = 0.0, total = 0.0;
-  const auto fetch = [&](i64 o) {
-    const i64 t0 = (j.back ? nblocks - 1 - o : o) * L;
-    const int rows = len - t0 < L ? (int)(len - t0) : L;
-    ra.load(ab + t0 * j.a.st * ESZ, j.a, rows, (int)j.Wa, tid);
-    rb.load(bb + t0 * j.b.st * ESZ, j.b, rows, bcols, tid);
-    rg = tid < L && tid < rows ? gate_of(args.g, b, h, t0 + tid) : 0.0;
+  f4 S[NT];                 // column cw + p, rows 16 nt + 4 g + r
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) S[nt] = f4{0.f, 0.f, 0.f, 0.f};
+#if OUT
+  if (job.init.p) {
+    const i64 at = b * job.init.sb + h * job.init.sh + (cw + p) * job.init.sc;
+    const int rows = cw + p < C ? (int)job.width : 0;
+    if (job.init.type == FP32) load_state<FP32>(S, job.init.p, at, job.init.sr, rows, g);
+    else if (job.init.type == FP16) load_state<FP16>(S, job.init.p, at, job.init.sr, rows, g);
+    else load_state<BF16>(S, job.init.p, at, job.init.sr, rows, g);
+  }
+#endif
+#if OUT
+  for (i64 s = 0; s < seg; s++) {                // the state at this segment's start
+    const i64 at = bh * (nseg - 1) + s;
+    const float e = expf((float)job.totals[at]);
+    const f4* from = (const f4*)job.local + ((at * ntiles + tile) * 4 + w) * (NT * 64) + lane;
+    for (int nt = 0; nt < NT; nt++) S[nt] = S[nt] * e + from[nt * 64];
+  }
+  for (int i = tid; i < RP * L * SP / 8; i += 256) *(v4u*)(P + 8 * i) = v4u{0, 0, 0, 0};     // (stays zero above the diagonal)
+#endif
+#if DOTS
+  if (tid < LT * L) (&of_rows[0][0])[tid] = (&of_cols[0][0])[tid] = 0.f;
+  const i64 spans = (nall + args.span - 1) / args.span;
+  const auto mark = [&](i64 span) {
+    if (cw >= C) return;
+    f4* to = (f4*)job.marks + ((bh * spans + span) * ((C + 15) / 16) + cw / 16) * (NT * 64) + lane;
+    for (int nt = 0; nt < NT; nt++) to[nt * 64] = S[nt];
   };
-  const float scale = j.back ? (float)args.scale : 1.f;
-  if (first < last) fetch(first);
+#endif
+
+  // a block o's operands, from the first block that this segment has
+  const auto block_of = [&](i64 o) { return back ? nall - 1 - o : o; };
+  const auto start = [&](auto& r, const Tensor& t, i64 heads, int col, int n) {
+    r.init(t, t.p + (b * t.sb + h / (args.H / heads) * t.sh + block_of(first) * L * t.st + col * t.sn) * ESZ, n, back, tid);
+  };
+  Staging<W, SK> rk;
+  Staging<64, SV> rv;
+  start(rk, job.k, job.Hk, 0, (int)job.width);
+  start(rv, job.v, job.Hv, c0, cols);
+#if OUT
+  Staging<W, SQ> rq;
+  start(rq, job.q, job.Hq, 0, (int)job.width);
+#endif
+#if DOTS
+  Staging<64, SX> rx;
+  start(rx, job.x, job.Hx, c0, cols);
+#endif
+  const auto fetch = [&](i64 o) {
+    const i64 rest = len - block_of(o) * L;
+    const int tokens = rest < L ? (int)rest : L;
+#if OUT
+    rq.load(tokens);
+#endif
+    rk.load(tokens);
+    rv.load(tokens);
+#if DOTS
+    rx.load(tokens);
+#endif
+  };
+  const auto put = [&](u16* to) {
+#if OUT
+    rq.store(to, tid);
+#endif
+    rk.store(to + AT_K, tid);
+    rv.store(to + AT_V, tid);
+#if DOTS
+    rx.store(to + AT_X, tid);
+#endif
+  };
+  // wave 3's lanes hold g of a block and the one behind it, and those of two more in reserve; backwards a row's is the one
+  // of the token behind it
+  const auto gate = [&](i64 o) {
+    const int i = lane & (L - 1);
+    o += lane / L;
+    const i64 t = block_of(o) * L + (back ? L - i : i);
+    return o < last && t < len ? raw_gate(args.g, b, h, t) : 0u;         // (zero is 0.0 in every type)
+  };
+  u32 rg = 0;
+  double total = 0.0;
+  if (first < last) {
+    fetch(first);
+    if (w == 3) {
+      const u32 now = gate(first);
+      rg = gate(first + 2);
+      total = fill_decays(decays + (first & 3), decays + (first + 1 & 3), gate_value(args.g, now), lane);
+    }
+    put(stage[first % NBUF]);
+  }
+  __syncthreads();
+  const float in_scale = (float)job.in_scale;
+#if OUT
+  const float out_scale = (float)job.out_scale;
+  const bool wide = job.out_type == FP32;        // (or of the operands' type)
+  const int size = wide ? 4 : ESZ;
+  const i64 out_at = b * job.ob + h / job.share * job.og + h % job.share * job.os;
+  char* to = job.out + (out_at + block_of(first) * L * job.ot) * size;
+  const i64 to_step = (back ? -L : L) * job.ot * size;
+  u32 to_off[LT];
+#pragma unroll
+  for (int it = 0; it < LT; it++) to_off[it] = (u32)((back ? L - 1 - (16 * it + p) : 16 * it + p) * job.ot + cw + 4 * g) * size;
+#endif
+#if DOTS
+  // (the state behind the last token, and the gradient that comes in there, are the end of the last span)
+  if (back && first < last && block_of(first) == nreal - 1) mark((nreal - 1) / args.span);
+#endif
+  const auto next_decays = [&](i64 o) {          // every other block, for the two behind the next one
+    if (((o - first) & 1) != 0 && o + 1 < last) {
+      total += fill_decays(decays + (o + 1 & 3), decays + (o + 2 & 3), gate_value(args.g, rg), lane);
+      rg = gate(o + 3);
+    }
+  };
   for (i64 o = first; o < last; o++) {
-    __syncthreads();
-    ra.store(A, tid);
-    rb.store(Bt, tid);
-    if (w == 0) total += fill_decays<L>(D, rg, lane);
+    const u16* tiles = stage[o % NBUF];
+    const u16 *K = tiles + AT_K, *V = tiles + AT_V;
+    const Decays& D = decays[o & 3];
     if (o + 1 < last) fetch(o + 1);
-    if (!args.only_local && j.marks && cw < j.Wb) {
-      const i64 c = j.back ? nblocks - 1 - o : o;
-      f4* to = (f4*)j.marks + ((bh * nblocks + c) * ((j.Wb + 15) / 16) + cw / 16) * (AT * 64) + lane;
-      for (int at = 0; at < AT; at++) to[at * 64] = X[at];
+    // operands are read from LDS a group ahead of their use, and stay there: hence the fences for the scheduler
+    const Frag<RP> vf = down<SV>(V, 0, 16 * w, lane);
+    const f4 to0 = *(const f4*)(D.to_end + 4 * g), to1 = *(const f4*)(D.to_end + 16 + 4 * g);
+    const float all = D.from_start[L - 1];
+#if OUT
+    const u16* Q = tiles;
+    const float from[LT] = {D.from_start[p], D.from_start[16 + p]};
+    Frag<RP> qf[QB][LT];
+#pragma unroll
+    for (int x = 0; x < QB; x++)
+#pragma unroll
+      for (int it = 0; it < LT; it++) qf[x][it] = along<SQ>(Q, 16 * it + p, 32 * x, g);
+    FENCE;
+    if (w == 3) {
+      next_decays(o);
+    } else {
+      const int it = w > 0, jt = w > 1;
+      f4 x = {0.f, 0.f, 0.f, 0.f};               // column i = 16 it + p, rows j = 16 jt + 4 g + r
+#pragma unroll
+      for (int k0 = 0; k0 < W / 32; k0 += QB) {
+        Frag<RP> kj[QB], qi[QB];
+#pragma unroll
+        for (int ks = 0; ks < QB; ks++) {
+          kj[ks] = along8<SK>(K, 16 * jt + p, 32 * (k0 + ks), g);
+          qi[ks] = along8<SQ>(Q, 16 * it + p, 32 * (k0 + ks), g);
+        }
+        FENCE;
+#pragma unroll
+        for (int ks = 0; ks < QB; ks++) x = mul<RAW>(kj[ks], qi[ks], x);
+      }
+      const int i = 16 * it + p, j = 16 * jt + 4 * g;
+      const f4 e = decay_between(D, i, j) * in_scale;
+#pragma unroll
+      for (int r = 0; r < 4; r++) x[r] = j + r <= i ? x[r] * e[r] : 0.f;
+      u32 d[RP * 2];
+      split2<RP>(x[0], x[1], d, 2);
+      split2<RP>(x[2], x[3], d + 1, 2);
+#pragma unroll
+      for (int q = 0; q < RP; q++) *(v2u*)(P + (q * L + i) * SP + j) = v2u{d[2 * q], d[2 * q + 1]};
+#if DOTS
+      if (job.pairs) {
+        const u16* X = tiles + AT_X;
+        f4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) a = mul<RAW>(along8<SV>(V, 16 * jt + p, 32 * ks, g), along8<SX>(X, 16 * it + p, 32 * ks, g), a);
+        float row = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const float s = x[r] * a[r];
+          row += s;
+          const float col = sum16(s);
+          if (p == 0) of_cols[it][j + r] = col;
+        }
+        row = sum_groups(row);
+        if (g == 0) of_rows[jt][i] = row;
+      }
+#endif
     }
+#else
+    if (w == 3) next_decays(o);
+#endif
+    Frag<RP> kf[KB];
+#pragma unroll
+    for (int x = 0; x < KB; x++) kf[x] = down<SK>(K, 0, 16 * x, lane);
+    FENCE;
+#if OUT
+    f4 y[LT];                                    // column i = 16 it + p, rows cw + 4 g + r
+#pragma unroll
+    for (int it = 0; it < LT; it++) y[it] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k0 = 0; k0 < W / 32; k0 += QB) {
+#pragma unroll
+      for (int ks = 0; ks < QB; ks++) {
+        const f4 u = S[2 * (k0 + ks)], v = S[2 * (k0 + ks) + 1];
+        const float x[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+        const Frag<SPARTS> s = make_frag<SPARTS>(x);
+#pragma unroll
+        for (int it = 0; it < LT; it++) y[it] = mul<SLIM>(s, qf[ks][it], y[it]);
+      }
+      if (k0 + QB < W / 32) {
+#pragma unroll
+        for (int x = 0; x < QB; x++)
+#pragma unroll
+          for (int it = 0; it < LT; it++) qf[x][it] = along<SQ>(Q, 16 * it + p, 32 * (k0 + QB + x), g);
+        FENCE;
+      }
+    }
+#pragma unroll
+    for (int it = 0; it < LT; it++) y[it] *= from[it];
+#if DOTS
+#pragma unroll
+    for (int it = 0; it < LT; it++) {
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < RP; q++) {
+        const v2u x = *(const v2u*)(tiles + AT_X + (q * L + 16 * it + p) * SX + 16 * w + 4 * g);
+        s += y[it][0] * as_f(x[0] << 16) + y[it][1] * as_f(x[0] & 0xffff0000u) + y[it][2] * as_f(x[1] << 16) + y[it][3] * as_f(x[1] & 0xffff0000u);
+      }
+      s = sum_groups(s);
+      if (g == 0) of_state[w][16 * it + p] = s;
+    }
+#endif
+#endif
+    float vx[8];
+    frag_values(vf, vx);
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      vx[r] *= to0[r] * in_scale;
+      vx[4 + r] *= to1[r] * in_scale;
+    }
+    const Frag<3> vd = make_frag<3>(vx);
+#pragma unroll
+    for (int n0 = 0; n0 < NT; n0 += KB) {
+      Frag<RP> next[KB];
+      if (n0 + KB < NT) {
+#pragma unroll
+        for (int x = 0; x < KB; x++) next[x] = down<SK>(K, 0, 16 * (n0 + KB + x), lane);
+        FENCE;
+      }
+#pragma unroll
+      for (int x = 0; x < KB; x++) S[n0 + x] *= all;
+      mul_each<KB, 2>(kf, vd, S + n0);
+      if (n0 + KB < NT) {
+#pragma unroll
+        for (int x = 0; x < KB; x++) kf[x] = next[x];
+      }
+    }
+#if OUT
     __syncthreads();
-    const float all = D.all;
-    for (int at = 0; at < AT; at++) X[at] *= all;
+    {
+      const Frag<RP> p0 = along<SP>(P, p, 0, g), p1 = along<SP>(P, 16 + p, 0, g);
+      y[0] = mul<CALC>(vf, p0, y[0]);
+      y[1] = mul<CALC>(vf, p1, y[1]);
+    }
+#if DOTS
+    if (w == 3 && lane < L) {
+      const i64 t = block_of(o) * L + (back ? L - 1 - lane : lane);
+      float s = of_state[0][lane] + of_state[1][lane] + (of_state[2][lane] + of_state[3][lane]);
+      if (job.pairs) s += (of_rows[0][lane] + of_rows[1][lane]) - (of_cols[0][lane] + of_cols[1][lane]);
+      if (t < T) job.dots[((i64)tile * args.B * args.H + bh) * T + t] = s * out_scale;
+    }
+    if (o + 1 < nall) {
+      const i64 c = block_of(o);                 // (a border: in front of block c + 1, or backwards in front of block c)
+      if (!back && (c + 1) % args.span == 0 && c + 1 < nreal) mark((c + 1) / args.span - 1);
+      if (back && c % args.span == 0) mark(c / args.span - 1);
+    }
+#endif
+#endif
+    if (NBUF == 1) __syncthreads();
+    if (o + 1 < last) put(stage[(o + 1) % NBUF]);
+#if OUT
+    const Buffer into = buffer_at(to);
+    to += to_step;
 #pragma unroll
-    for (int jb = 0; jb < L / 32; jb++) {
-      float x[8];
-      frag_values(down<SB, L>(Bt, 32 * jb, 16 * w, lane), x);
-      const float* e = j.back ? D.from_start : D.to_end;
-      for (int r = 0; r < 4; r++) {
-        x[r] *= scale * e[32 * jb + 4 * g + r];
-        x[4 + r] *= scale * e[32 * jb + 16 + 4 * g + r];
-      }
-      const Frag<3> bd = make_frag<3>(x);
-#pragma unroll
-      for (int at = 0; at < AT; at++) X[at] = mul<2>(down<SA, L>(A, 32 * jb, 16 * at, lane), bd, X[at]);
+    for (int it = 0; it < LT; it++) {
+      const int i = back ? L - 1 - (16 * it + p) : 16 * it + p;
+      const i64 t0 = block_of(o) * L;
+      const f4 z = t0 + i < len ? y[it] * out_scale : f4{0.f, 0.f, 0.f, 0.f};
+      const u32 off = t0 + i < T ? to_off[it] : NOTHING;
+      if (wide) store_wide(into, off, z, C - cw - 4 * g, C % 4 == 0);
+      else store_in(into, off, z, C - cw - 4 * g, C % 4 == 0);
+    }
+#endif
+    __syncthreads();
+  }
+#if OUT
+#if DOTS
+  if (!back && first < last && last == nreal) mark((nreal - 1) / args.span);
+#endif
+  for (i64 o = s0; o < s1; o++) {                // blocks without a token
+    if (o >= first && o < last) continue;
+    for (int u = tid; u < L * 16; u += 256) {
+      const i64 t = block_of(o) * L + u / 16;
+      const int col = c0 + u % 16 * 4;
+      if (t < T)
+        for (int r = 0; r < 4 && col + r < C; r++) store_type(job.out, out_at + t * job.ot + col + r, wide ? FP32 : IN, 0.f);
     }
   }
-  if (args.only_local) {
-    const i64 at0 = bh * (args.nseg - 1) + seg;
-    f4* to = (f4*)j.local + (at0 * nct * 4 + ct * 4 + w) * (AT * 64) + lane;
-    for (int at = 0; at < AT; at++) to[at * 64] = X[at];
-    if (tid == 0 && ct == 0) j.totals[at0] = total;
-  } else if (j.fin.p && seg == args.nseg - 1) {
-    for (int at = 0; at < AT; at++)
-      for (int r = 0; r < 4; r++) {
-        const int row = 16 * at + 4 * g + r, col = cw + p;
-        if (row < j.Wa && col < j.Wb) store_type(j.fin.p, b * j.fin.sb + h * j.fin.sh + row * j.fin.sm + col * j.fin.sn, (int)j.fin.type, X[at][r]);
-      }
+  if (job.fin.p && seg == nseg - 1) {
+    const float e = back && len > 0 ? expf((float)gate_of(args.g, b, h, 0)) : 1.f;
+    int mine = p;
+    asm("" : "+v"(mine));                        // (or the addresses of the first state stay in registers all the while)
+    const i64 at = b * job.fin.sb + h * job.fin.sh + (cw + mine) * job.fin.sc;
+    const int rows = cw + mine < C ? (int)job.width : 0;
+    if (job.fin.type == FP32) store_state<FP32>(S, e, job.fin.p, at, job.fin.sr, rows, g);
+    else if (job.fin.type == FP16) store_state<FP16>(S, e, job.fin.p, at, job.fin.sr, rows, g);
+    else store_state<BF16>(S, e, job.fin.p, at, job.fin.sr, rows, g);
   }
+#else
+  const i64 at = bh * (args.nseg - 1) + seg;
+  f4* to = (f4*)job.local + ((at * ntiles + tile) * 4 + w) * (NT * 64) + lane;
+  for (int nt = 0; nt < NT; nt++) to[nt * 64] = S[nt];
+  if (tid == 192 && tile == 0) job.totals[at] = total;
+#endif
 }
 #endif
 
-// ================================================================== gradients
-#ifdef KERNEL_GRAD
-// One workgroup per (batch, shared head, slice of the heads that share it, block).  With E = exp(G_i - G_j) for i >= j,
-// P = (q_i.k_j) E, R = (dy_i.v_j) E scale, and the marks S (state in front) and X (gradient of the state behind):
-//   dq_i = sum_j R_ij k_j + scale exp(G_i) S^T dy_i        dk_j = sum_i R_ij q_i + exp(G_L - G_j) X^T v_j
-//   dv_j = scale sum_i P_ij dy_i + exp(G_L - G_j) X k_j
-//   dg_t = sum_{i>=t>j} P_ij (dy_i.v_j) scale + sum_{i>=t} q_i.dq^S_i + sum_{j<t} k_j.dk^X_j + exp(G_L) <X, S>
-// (the last line: the gradient of a step's logarithm is what the step carries over; no term is the difference of two sums
-// over the whole sequence, so slow and fast decays alike keep their precision).  Wave w owns every NW-th tile of 16 result
-// columns; marks come straight from memory in operand order.  Two operand tiles are in LDS at a time (q, k; then v, dy;
-// then k, q), which leaves room for two workgroups per compute unit to cover each other's loads.
-struct GradArgs {
-  Tensor q, k, v, dy;
-  Gate g;
-  const float* marks_s;     // [B*H][blocks][ceil(N/16)][WA/16][64][4]
+// ================================================================== gradient of the decays
+#ifdef KERNEL_GATE
+// The gradient of g_t is what token t's step carries over, <X, exp(g_t) S>: at a border between blocks the product of the
+// two marks there, and from one token to the one before it
+//     <X, S> + q_t.dq_t - k_t.dk_t.
+// Summed backwards from the nearest border that has marks (64 bits, at most `span` blocks away), never over a whole long
+// sequence, where what is left of a fast decay would drown in the rounding of what came before.  The dots hold the products;
+// their share within a block is the same number once as q.dq and once as k.dk, so it cancels to the last bit where it should.
+// One workgroup per (batch, head, span).
+struct GateArgs {
+  const float* dots_q;      // [tiles][B*H][T]
+  const float* dots_k;
+  const float* marks_s;     // [B*H][spans][size]
   const float* marks_x;
-  char *dq, *dk;            // [slices][B,T,Hk,N]: of the inputs' type with one slice, fp32 with more
-  char* dv;                 // [B,T,H,M]
-  char* dg;                 // [B,T,H] of type dg_type, or null
+  Gate g;
+  char* dg;                 // [B,T,H]
   const i64* lengths;
-  i64 B, T, H, Hk, M, N, slices, dg_type;
-  double scale;
+  i64 B, T, H, tiles, span, size, type;
 };
 
-// WA: padded M, WB: padded N
-constexpr int TH = NW * 64;
-constexpr int WX = WA > WB ? WA : WB;
-constexpr int SX = stride_down(WX), SP = stride_along(L);
-constexpr int LT = L / 16, MT = WA / 16, NT = WB / 16;
-constexpr int NTW = (NT + NW - 1) / NW, MTW = (MT + NW - 1) / NW;
-constexpr int TILES = LT * (LT + 1) / 2, TPW = (TILES + NW - 1) / NW;
-
-DEV void store4(char* at, int type, f4 o, int n, int N) {
-  if (N % 4 == 0) {
-    if (type == FP32) *(f4*)at = o;
-    else if (type == BF16) *(v2u*)at = v2u{pack_rne(o[0], o[1]), pack_rne(o[2], o[3])};
-    else {
-      typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-      *(h4*)at = __builtin_convertvector(o, h4);
-    }
-  } else {
-    for (int r = 0; r < 4; r++)
-      if (n + r < N) store_type(at, r, type, o[r]);
+extern "C" __global__ void __launch_bounds__(256) la_gate(GateArgs a) {
+  __shared__ double part[4];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const i64 nall = (a.T + L - 1) / L, spans = (nall + a.span - 1) / a.span;
+  const i64 bh = blockIdx.x / spans, s = blockIdx.x % spans, b = bh / a.H, h = bh % a.H, BH = a.B * a.H;
+  const i64 len = length_of(a.lengths, b, a.T);
+  const i64 t0 = s * a.span * L, t1 = t0 + a.span * L < a.T ? t0 + a.span * L : a.T, end = t1 < len ? t1 : len;
+  for (i64 t = end > t0 ? end + tid : t0 + tid; t < t1; t += 256) store_type(a.dg, (b * a.T + t) * a.H + h, (int)a.type, 0.f);
+  if (end <= t0) return;
+  double x = 0.0;
+  const f4 *ms = (const f4*)(a.marks_s + (bh * spans + s) * a.size), *mx = (const f4*)(a.marks_x + (bh * spans + s) * a.size);
+  for (i64 i = tid; i < a.size / 4; i += 256) {
+    const f4 u = ms[i], v = mx[i];
+    x += (double)(u[0] * v[0] + u[1] * v[1]) + (double)(u[2] * v[2] + u[3] * v[3]);
   }
-}
-
-extern "C" __global__ void __launch_bounds__(TH, 2) la_grad(GradArgs a) {
-  __shared__ __attribute__((aligned(16))) u16 X0[RP * L * SX], X1[RP * L * SX], P[RP * L * SP], R[RP * L * SP];
-  __shared__ Decays<L> D;
-  __shared__ float rows_pw[LT][L], cols_pw[LT][L], aq[NW][L], bk[NW][L], cs[NW];
-  const int tid = threadIdx.x, lane = tid & 63, p = lane & 15, g = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const i64 nblocks = (a.T + L - 1) / L;
-  const i64 share = a.H / a.Hk, per = (share + a.slices - 1) / a.slices;
-  const i64 id = blockIdx.x;
-  const i64 c = id % nblocks, sl = id / nblocks % a.slices, bhk = id / nblocks / a.slices, b = bhk / a.Hk, hk = bhk % a.Hk;
-  const i64 len = length_of(a.lengths, b, a.T), t0 = c * L;
-  const int rows = len - t0 < L ? (int)(len - t0) : L, rows_out = a.T - t0 < L ? (int)(a.T - t0) : L;
-  const float scale = (float)a.scale;
-  const int M = (int)a.M, N = (int)a.N;
-
-  for (int i = tid; i < RP * L * SP / 8; i += TH) {
-    *(v4u*)(P + 8 * i) = v4u{0, 0, 0, 0};
-    *(v4u*)(R + 8 * i) = v4u{0, 0, 0, 0};
-  }
-  for (int i = tid; i < LT * L; i += TH) (&rows_pw[0][0])[i] = (&cols_pw[0][0])[i] = 0.f;
-
-  const char* qb = a.q.p + (b * a.q.sb + hk * a.q.sh + t0 * a.q.st) * ESZ;
-  const char* kb = a.k.p + (b * a.k.sb + hk * a.k.sh + t0 * a.k.st) * ESZ;
-  f4 dq[NTW][LT], dk[NTW][LT];                   // column i (j) = 16 t + p, rows n = 16 nt + 4 g + r
-  for (int x = 0; x < NTW; x++)
-    for (int t = 0; t < LT; t++) dq[x][t] = dk[x][t] = f4{0.f, 0.f, 0.f, 0.f};
-
-  const i64 h1 = (sl + 1) * per < share ? (sl + 1) * per : share;
-  for (i64 hh = sl * per; hh < h1; hh++) {
-    const i64 h = hk * share + hh, bh = b * a.H + h;
-    const char* vb = a.v.p + (b * a.v.sb + h * a.v.sh + t0 * a.v.st) * ESZ;
-    const char* yb = a.dy.p + (b * a.dy.sb + h * a.dy.sh + t0 * a.dy.st) * ESZ;
-    const f4* ms = (const f4*)a.marks_s + (bh * nblocks + c) * ((N + 15) / 16) * (MT * 64);
-    const f4* mx = (const f4*)a.marks_x + (bh * nblocks + c) * ((N + 15) / 16) * (MT * 64);
-    {
-      Staging<WB, SX, L, TH> rq, rk;
-      rq.load(qb, a.q, rows, N, tid);
-      rk.load(kb, a.k, rows, N, tid);
-      const double rg = tid < L && tid < rows ? gate_of(a.g, b, h, t0 + tid) : 0.0;
-      __syncthreads();
-      rq.store(X0, tid);
-      rk.store(X1, tid);
-      if (w == 0) fill_decays<L>(D, rg, lane);
-    }
-    Staging<WA, SX, L, TH> rv, ry;
-    rv.load(vb, a.v, rows, M, tid);
-    ry.load(yb, a.dy, rows, M, tid);
+  x = read_lane(scan64(x), 63);
+  if (lane == 0) part[w] = x;
+  __syncthreads();
+  double carry = part[0] + part[1] + (part[2] + part[3]);
+  if (end < len) carry *= exp(gate_of(a.g, b, h, end));      // (a mark inside the sequence lacks its own step's decay)
+  __syncthreads();
+  for (i64 hi = end; hi > t0; hi -= 256) {                   // thread i has token hi - 1 - i
+    const i64 t = hi - 1 - tid;
+    double d = 0.0;
+    if (t >= t0)
+      for (i64 k = 0; k < a.tiles; k++) d += (double)a.dots_q[(k * BH + bh) * a.T + t] - (double)a.dots_k[(k * BH + bh) * a.T + t];
+    d = scan64(d);
+    if (lane == 63) part[w] = d;
     __syncthreads();
-    f4 A[TPW];                                   // q_i.k_j: column i = 16 it + p, rows j = 16 jt + 4 g + r
-#pragma unroll
-    for (int x = 0; x < TPW; x++) {
-      const int idx = w + x * NW;
-      A[x] = f4{0.f, 0.f, 0.f, 0.f};
-      if (idx < TILES) {
-        int it, jt;
-        tile_of(idx, &it, &jt);
-#pragma unroll
-        for (int ks = 0; ks < WB / 32; ks++)
-          A[x] = mul<RAW>(along8<SX, L>(X1, 16 * jt + p, 32 * ks, g), along8<SX, L>(X0, 16 * it + p, 32 * ks, g), A[x]);
-      }
+    double before = carry;
+    for (int i = 0; i < 4; i++) {
+      if (i < w) before += part[i];
+      carry += part[i];
     }
+    if (t >= t0) store_type(a.dg, (b * a.T + t) * a.H + h, (int)a.type, (float)(before + d));
     __syncthreads();
-    rv.store(X0, tid);
-    ry.store(X1, tid);
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < TPW; x++) {
-      const int idx = w + x * NW;
-      if (idx >= TILES) continue;
-      int it, jt;
-      tile_of(idx, &it, &jt);
-      f4 W = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < WA / 32; ks++)
-        W = mul<RAW>(along8<SX, L>(X0, 16 * jt + p, 32 * ks, g), along8<SX, L>(X1, 16 * it + p, 32 * ks, g), W);
-      const int i = 16 * it + p;
-      const float hi = D.hi[i], lo = D.lo[i];
-      float of_row = 0.f;
-      f4 pw, pe, re;
-      for (int r = 0; r < 4; r++) {
-        const int j = 16 * jt + 4 * g + r;
-        const float e = j <= i ? decay_between(D, hi, lo, j) * scale : 0.f;
-        pe[r] = j <= i ? A[x][r] * e : 0.f;
-        re[r] = j <= i ? W[r] * e : 0.f;
-        pw[r] = j <= i ? pe[r] * W[r] : 0.f;
-        of_row += pw[r];
-      }
-      u32 d[RP * 2], f[RP * 2];
-      split2<RP>(pe[0], pe[1], d, 2);
-      split2<RP>(pe[2], pe[3], d + 1, 2);
-      split2<RP>(re[0], re[1], f, 2);
-      split2<RP>(re[2], re[3], f + 1, 2);
-      for (int q = 0; q < RP; q++) {
-        *(v2u*)(P + (q * L + i) * SP + 16 * jt + 4 * g) = v2u{d[2 * q], d[2 * q + 1]};
-        *(v2u*)(R + (q * L + i) * SP + 16 * jt + 4 * g) = v2u{f[2 * q], f[2 * q + 1]};
-      }
-      if (a.dg) {
-        of_row = sum_groups(of_row);
-        if (g == 0) rows_pw[jt][i] = of_row;
-        for (int r = 0; r < 4; r++) {
-          const float s = sum16(pw[r]);
-          if (p == 0) cols_pw[it][16 * jt + 4 * g + r] = s;
-        }
-      }
-    }
-    __syncthreads();
-    // with v in X0, dy in X1: what the marks give to dq and dk, and the block's own share of dv
-    f4 qs[NTW][LT], kx[NTW][LT], dv[MTW][LT];
-    float inner = 0.f;
-#pragma unroll
-    for (int x = 0; x < NTW; x++) {
-      const int nt = w + x * NW;
-      for (int t = 0; t < LT; t++) qs[x][t] = kx[x][t] = f4{0.f, 0.f, 0.f, 0.f};
-      if (16 * nt >= N) continue;
-#pragma unroll
-      for (int ks = 0; ks < WA / 32; ks++) {
-        const f4 s0 = ms[(nt * MT + 2 * ks) * 64 + lane], s1 = ms[(nt * MT + 2 * ks + 1) * 64 + lane];
-        const f4 x0 = mx[(nt * MT + 2 * ks) * 64 + lane], x1 = mx[(nt * MT + 2 * ks + 1) * 64 + lane];
-        float s[8], y[8];
-        for (int r = 0; r < 4; r++) {
-          s[r] = s0[r];
-          s[4 + r] = s1[r];
-          y[r] = x0[r];
-          y[4 + r] = x1[r];
-          inner += s0[r] * x0[r] + s1[r] * x1[r];
-        }
-        const Frag<3> sf = make_frag<3>(s), xf = make_frag<3>(y);
-#pragma unroll
-        for (int t = 0; t < LT; t++) {
-          qs[x][t] = mul<2>(sf, along<SX, L>(X1, 16 * t + p, 32 * ks, g), qs[x][t]);
-          kx[x][t] = mul<2>(xf, along<SX, L>(X0, 16 * t + p, 32 * ks, g), kx[x][t]);
-        }
-      }
-    }
-#pragma unroll
-    for (int x = 0; x < MTW; x++) {
-      const int mt = w + x * NW;
-      for (int t = 0; t < LT; t++) dv[x][t] = f4{0.f, 0.f, 0.f, 0.f};
-      if (16 * mt >= M) continue;
-#pragma unroll
-      for (int ib = 0; ib < L / 32; ib++) {
-        const Frag<RP> yf = down<SX, L>(X1, 32 * ib, 16 * mt, lane);
-#pragma unroll
-        for (int t = 0; t < LT; t++)
-          if (16 * t < 32 * ib + 32) dv[x][t] = mul<CALC>(yf, down<SP, L>(P, 32 * ib, 16 * t, lane), dv[x][t]);
-      }
-    }
-    {
-      Staging<WB, SX, L, TH> rq, rk;
-      rq.load(qb, a.q, rows, N, tid);
-      rk.load(kb, a.k, rows, N, tid);
-      __syncthreads();
-      rk.store(X0, tid);
-      rq.store(X1, tid);
-    }
-    __syncthreads();
-    // with k in X0, q in X1
-#pragma unroll
-    for (int t = 0; t < LT; t++) {
-      const float from = D.from_start[16 * t + p] * scale, to = D.to_end[16 * t + p];
-      float sq = 0.f, sk = 0.f;
-#pragma unroll
-      for (int x = 0; x < NTW; x++) {
-        const int nt = w + x * NW;
-        if (nt >= NT) continue;
-        qs[x][t] *= from;
-        kx[x][t] *= to;
-        if (a.dg) {
-          for (int q = 0; q < RP; q++) {
-            const v2u qv = *(const v2u*)(X1 + (q * L + 16 * t + p) * SX + 16 * nt + 4 * g);
-            const v2u kv = *(const v2u*)(X0 + (q * L + 16 * t + p) * SX + 16 * nt + 4 * g);
-            sq += qs[x][t][0] * as_f(qv[0] << 16) + qs[x][t][1] * as_f(qv[0] & 0xffff0000u) + qs[x][t][2] * as_f(qv[1] << 16) + qs[x][t][3] * as_f(qv[1] & 0xffff0000u);
-            sk += kx[x][t][0] * as_f(kv[0] << 16) + kx[x][t][1] * as_f(kv[0] & 0xffff0000u) + kx[x][t][2] * as_f(kv[1] << 16) + kx[x][t][3] * as_f(kv[1] & 0xffff0000u);
-          }
-        }
-        dq[x][t] += qs[x][t];
-        dk[x][t] += kx[x][t];
-      }
-      if (a.dg) {
-        sq = sum_groups(sq);
-        sk = sum_groups(sk);
-        if (g == 0) {
-          aq[w][16 * t + p] = sq;
-          bk[w][16 * t + p] = sk;
-        }
-      }
-    }
-    if (a.dg) {
-      inner = sum_groups(sum16(inner));
-      if (lane == 0) cs[w] = inner;
-    }
-#pragma unroll
-    for (int x = 0; x < NTW; x++) {
-      const int nt = w + x * NW;
-      if (16 * nt >= N) continue;
-#pragma unroll
-      for (int tb = 0; tb < L / 32; tb++) {
-        const Frag<RP> kf = down<SX, L>(X0, 32 * tb, 16 * nt, lane), qf = down<SX, L>(X1, 32 * tb, 16 * nt, lane);
-#pragma unroll
-        for (int t = 0; t < LT; t++) {
-          if (t >= 2 * tb) dq[x][t] = mul<CALC>(kf, along<SP, L>(R, 16 * t + p, 32 * tb, g), dq[x][t]);
-          if (16 * t < 32 * tb + 32) dk[x][t] = mul<CALC>(qf, down<SP, L>(R, 32 * tb, 16 * t, lane), dk[x][t]);
-        }
-      }
-    }
-#pragma unroll
-    for (int x = 0; x < MTW; x++) {
-      const int mt = w + x * NW;
-      if (16 * mt >= M) continue;
-      f4 e[LT];
-      for (int t = 0; t < LT; t++) e[t] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < WB / 32; ks++) {
-        // lane p holds row m = 16 mt + p, columns n = 32 ks + {4g.., 16 + 4g..}: the marks' tiles read across
-        float s[8];
-        for (int r = 0; r < 8; r++) {
-          const int nt = 2 * ks + r / 4;
-          const float* at = (const float*)(mx + (nt * MT + mt) * 64 + (p >> 2) * 16 + 4 * g + r % 4) + (p & 3);
-          s[r] = 16 * nt < N ? *at : 0.f;
-        }
-        const Frag<RP> xf = make_frag<RP>(s);
-#pragma unroll
-        for (int t = 0; t < LT; t++) e[t] = mul<CALC>(xf, along<SX, L>(X0, 16 * t + p, 32 * ks, g), e[t]);
-      }
-      for (int t = 0; t < LT; t++) {
-        const int j = 16 * t + p, m = 16 * mt + 4 * g;
-        if (j >= rows_out || m >= M) continue;
-        f4 o = dv[x][t] + e[t] * D.to_end[j];
-        if (j >= rows) o = f4{0.f, 0.f, 0.f, 0.f};
-        store4(a.dv + (((b * a.T + t0 + j) * a.H + h) * M + m) * ESZ, IN, o, m, M);
-      }
-    }
-    if (a.dg) {
-      __syncthreads();
-      if (w == 0) {
-        double x = 0.0, y = 0.0, z = 0.0;
-        if (lane < L) {
-          for (int t = 0; t < LT; t++) x += (double)rows_pw[t][lane] - (double)cols_pw[t][lane];
-          for (int q = 0; q < NW; q++) {
-            x += aq[q][lane];
-            y += bk[q][lane];
-          }
-        }
-        for (int q = 0; q < NW; q++) z += cs[q];
-        // sum over i >= t of x_i, over j < t of y_j
-        const double sx = scan64(x), sy = scan64(y);
-        const double dg = (last_lane(sx) - sx + x) + (sy - y) + (double)D.all * z;
-        if (lane < rows_out)
-          store_type(a.dg, (b * a.T + t0 + lane) * a.H + h, (int)a.dg_type, lane < rows ? (float)dg : 0.f);
-      }
-    }
-  }
-  const int type = a.slices == 1 ? IN : FP32;
-  const i64 size = type == FP32 ? 4 : 2, skip = a.slices == 1 ? 0 : sl * a.B * a.T * a.Hk * a.N;
-#pragma unroll
-  for (int x = 0; x < NTW; x++) {
-    const int nt = w + x * NW;
-    for (int t = 0; t < LT; t++) {
-      const int i = 16 * t + p, n = 16 * nt + 4 * g;
-      if (i >= rows_out || n >= N) continue;
-      const i64 at = (skip + ((b * a.T + t0 + i) * a.Hk + hk) * N + n) * size;
-      const bool in = i < rows;
-      const f4 zero = {0.f, 0.f, 0.f, 0.f};
-      store4(a.dq + at, type, in ? dq[x][t] : zero, n, N);
-      store4(a.dk + at, type, in ? dk[x][t] : zero, n, N);
-    }
   }
 }
 #endif
@@ -976,11 +934,11 @@ DEV void step_rows(const StepArgs& a, i64 b, i64 h, int r0, int tid) {
     float acc = 0.f;
     if (m < end) {
       const float v = load_in(vp, m * a.v.sn);
-      char* row = a.s.p + (b * a.s.sb + h * a.s.sh + m * a.s.sm) * SZ;
+      char* row = a.s.p + (b * a.s.sb + h * a.s.sh + m * a.s.sr) * SZ;
       for (int n = sub * VE; n < N; n += gl * VE) {
         float s[VE];
         if constexpr (VE == 1) {
-          s[0] = load_type(row, n * a.s.sn, TYPE);
+          s[0] = load_type(row, n * a.s.sc, TYPE);
         } else if constexpr (TYPE == FP32) {
           const f4 t = *(const f4*)(row + n * 4);
           for (int i = 0; i < 4; i++) s[i] = t[i];
@@ -996,7 +954,7 @@ DEV void step_rows(const StepArgs& a, i64 b, i64 h, int r0, int tid) {
           acc += s[i] * load_in(qp, (n + i) * a.q.sn);
         }
         if constexpr (VE == 1) {
-          store_type(row, n * a.s.sn, TYPE, s[0]);
+          store_type(row, n * a.s.sc, TYPE, s[0]);
         } else if constexpr (TYPE == FP32) {
           *(f4*)(row + n * 4) = f4{s[0], s[1], s[2], s[3]};
         } else {

@@ -65,16 +65,21 @@ def kernel(device: th.device, source: str, name: str, defines: Tuple[Tuple[str, 
 _packers: Dict[str, struct.Struct] = {}
 
 
-def launch(k: runtime.Kernel, device: th.device, grid: int, threads: int, layout: str, *args, grid_y: int = 1):
+def launch(k: runtime.Kernel, device: th.device, grid: int, threads: int, layout: str, *args):
     """Launches `k` on the current stream of `device`; `layout` names the argument block's 8-byte fields (struct)."""
-    if grid <= 0:
-        return
-    require(grid * threads < 2 ** 32, f'{k.name}: a launch of {grid} workgroups is more than the hardware takes; split the batch')
     p = _packers.get(layout)
     if p is None:
         p = _packers[layout] = struct.Struct('<' + layout)
+    launch_bytes(k, device, grid, 1, threads, p.pack(*args))
+
+
+def launch_bytes(k: runtime.Kernel, device: th.device, grid: int, grid_y: int, threads: int, block: bytes):
+    """The same with a packed argument block."""
+    if grid <= 0:
+        return
+    require(grid * threads < 2 ** 32, f'{k.name}: a launch of {grid} workgroups is more than the hardware takes; split the batch')
     with (th.cuda.device(device) if th.cuda.current_device() != device.index else contextlib.nullcontext()):
-        k.launch((grid, grid_y, 1), (threads, 1, 1), p.pack(*args), stream=th.cuda.current_stream(device).cuda_stream)
+        k.launch((grid, grid_y, 1), (threads, 1, 1), block, stream=th.cuda.current_stream(device).cuda_stream)
 
 
 def slice_sum(x: th.Tensor, slices: int, out: th.Tensor):

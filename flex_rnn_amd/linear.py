@@ -15,6 +15,7 @@ and head sizes; `linear_attention.naive` and `linear_attention.naive_fp64` are t
 """
 from __future__ import annotations
 
+import struct
 from typing import Optional, Tuple
 
 import torch as th
@@ -25,14 +26,15 @@ from .handwritten import DTYPES, require
 SOURCE = 'linear_attention.hip'
 MAX_HEAD = 256                  # largest M and N
 WIDTHS = (64, 128, 256)         # what M and N are padded to
+BLOCK = 32                      # tokens per block
 WORKGROUPS = 512                # two per compute unit: below this a sequence is split into segments
 MAX_SEGMENTS = 16
+MARK_BLOCKS = 32                # blocks between the borders at which the gradient of g starts anew
 
 # argument blocks (see the structs in the source): Tensor 6 fields, Gate 5, States 6
-_FW = '6q6q6q5q6q6qqqqq8qd'
-_JOB = '6q6q6q6qqqq4qq'
-_WALK = _JOB + _JOB + '5qq7qd'
-_GRAD = '6q6q6q6q5qqqqqqqq8qd'
+_JOB = struct.Struct('<6q6q6q6q6q6q7q4q8q2d')
+_BLOCK = struct.Struct('<5qq7q')
+_GATE = '4q5qqq7q'
 _STEP = '6q6q6q5q6qq8qd'
 
 
@@ -40,32 +42,14 @@ def _width(n: int) -> int:
     return next(w for w in WIDTHS if n <= w)
 
 
-def _block(dtype: th.dtype, width: int) -> int:
-    """Tokens per block: 64, and 32 where the operands' parts (or 256 columns) would leave LDS for less than two
-    workgroups per compute unit."""
-    return 64 if dtype == th.bfloat16 and width <= 128 else 32
+def _block_defines(dtype, width, out=1, dots=0):
+    w = _width(width)
+    nbuf = 2 if dtype == th.bfloat16 and w <= 128 and not dots else 1
+    occ = 2
+    return (('KERNEL_BLOCK', 1), ('IN', DTYPES[dtype]), ('W', w), ('OUT', out), ('DOTS', dots), ('NBUF', nbuf), ('OCC', occ))
 
 
-def _grad_block(dtype: th.dtype) -> int:
-    """The same for the gradient kernel, which holds two operand tiles only."""
-    return 64 if dtype == th.bfloat16 else 32
-
-
-def _fw_defines(dtype, N):
-    w = _width(N)
-    return (('KERNEL_FW', 1), ('IN', DTYPES[dtype]), ('WA', w), ('L', _block(dtype, w)))
-
-
-def _walk_defines(dtype, width, block):
-    return (('KERNEL_WALK', 1), ('IN', DTYPES[dtype]), ('WA', _width(width)), ('L', block))
-
-
-def _grad_waves(M, N):
-    return 8 if max(_width(M), _width(N)) >= 128 else 4
-
-
-def _grad_defines(dtype, M, N):
-    return (('KERNEL_GRAD', 1), ('IN', DTYPES[dtype]), ('WA', _width(M)), ('WB', _width(N)), ('L', _grad_block(dtype)), ('NW', _grad_waves(M, N)))
+_GATE_DEFINES = (('KERNEL_GATE', 1), ('IN', 0))
 
 
 def _step_defines(dtype):
@@ -74,14 +58,11 @@ def _step_defines(dtype):
 
 def builds():
     """Every code object of this module: (source, kernel, defines)."""
-    out = []
+    out = [(SOURCE, 'la_gate', _GATE_DEFINES)]
     for dt in DTYPES:
-        for w in WIDTHS:
-            out.append((SOURCE, 'la_fw', _fw_defines(dt, w)))
-            for block in {_block(dt, w), _grad_block(dt)}:
-                out.append((SOURCE, 'la_walk', _walk_defines(dt, w, block)))
-            out += [(SOURCE, 'la_grad', _grad_defines(dt, m, w)) for m in WIDTHS]
         out.append((SOURCE, 'la_step', _step_defines(dt)))
+        for w in WIDTHS:
+            out += [(SOURCE, 'la_block', _block_defines(dt, w, o, d)) for o, d in ((1, 0), (1, 1), (0, 0))]
     return out
 
 
@@ -94,8 +75,9 @@ def _tensor(t: th.Tensor, batch: int, time: Optional[int], head: int):
     return t.data_ptr(), sb, st, sh, sn, int(wide)
 
 
-def _btH(t):
-    return _tensor(t, 0, 1, 2)
+def _near(t: th.Tensor) -> th.Tensor:
+    """`t` [B,T,heads,n], copied if a block of its tokens spans more than the 31 bits that offsets within a block have."""
+    return t if (BLOCK * t.stride(1) + MAX_HEAD * t.stride(3)) * t.element_size() < 2 ** 31 else t.contiguous()
 
 
 def _gate(g: th.Tensor):
@@ -108,6 +90,12 @@ def _gate(g: th.Tensor):
 
 
 def _states(s: Optional[th.Tensor]):
+    """[B,H,M,N] with rows N, columns M (as the walks that produce y and dv hold it)."""
+    return (0, 0, 0, 0, 0, 2) if s is None else (s.data_ptr(), s.stride(0), s.stride(1), s.stride(3), s.stride(2), DTYPES[s.dtype])
+
+
+def _states_t(s: Optional[th.Tensor]):
+    """[B,H,M,N] with rows M, columns N (dq and dk)."""
     return (0, 0, 0, 0, 0, 2) if s is None else (s.data_ptr(), *s.stride(), DTYPES[s.dtype])
 
 
@@ -117,7 +105,7 @@ def _ptr(t):
 
 def _segments(groups: int, blocks: int) -> Tuple[int, int]:
     """(segments, blocks per segment) of a walk over `blocks` blocks by `groups` workgroups side by side."""
-    n = min(-(-WORKGROUPS // max(groups, 1)), blocks // 4, MAX_SEGMENTS)
+    n = min(-(-WORKGROUPS // max(groups, 1)), blocks // 8, MAX_SEGMENTS)
     if n <= 1:
         return 1, blocks
     per = -(-blocks // n)
@@ -125,94 +113,94 @@ def _segments(groups: int, blocks: int) -> Tuple[int, int]:
 
 
 # ------------------------------------------------------------------ launches
+_NO_TENSOR = (0, 0, 0, 0, 0, 1)
+_NO_JOB = bytes(_JOB.size)
+
+
+class _Role:
+    """One operand of a walk: its tensor, argument fields and heads."""
+
+    def __init__(self, t: th.Tensor):
+        self.fields, self.heads = _tensor(t, 0, 1, 2), t.shape[2]
+
+
+def _job(q, k, v, x, width, C, init, fin, out, strides, out_type, back=0, pairs=0, in_scale=1.0, out_scale=1.0, dots=0, marks=0):
+    """The fields of struct Job that are known before segments are; `local` and `totals` follow in `_walk`."""
+    return [(*q.fields, *k.fields, *v.fields, *(_NO_TENSOR if x is None else x.fields), *init, *fin, out, *strides, out_type, dots, marks),
+            (q.heads, k.heads, v.heads, 1 if x is None else x.heads, width, C, back, pairs, in_scale, out_scale)]
+
+
+def _walk(dev, dtype, jobs, gate, lengths, B, T, H, dots=0):
+    """Runs up to two walks of one width side by side, each in segments where the batch alone does not fill the chip."""
+    width = _width(jobs[0][1][4])
+    tiles = max(-(-j[1][5] // 64) for j in jobs)
+    blocks = -(-T // BLOCK)
+    nseg, per = _segments(len(jobs) * B * H * tiles, blocks)
+    size = B * H * (nseg - 1)
+    local = totals = None
+    if nseg > 1:
+        local = th.empty((len(jobs), size * tiles * 64 * width), dtype=th.float32, device=dev)
+        totals = th.empty((len(jobs), size), dtype=th.float64, device=dev)
+    blob = b''.join([_JOB.pack(*head, 0 if local is None else local[i].data_ptr(), 0 if totals is None else totals[i].data_ptr(), *tail)
+                     for i, (head, tail) in enumerate(jobs)] + [_NO_JOB] * (2 - len(jobs))
+                    + [_BLOCK.pack(*gate, _ptr(lengths), B, T, H, nseg, per, tiles, MARK_BLOCKS)])
+    for out in ((0, 1) if nseg > 1 else (1,)):
+        k = hw.kernel(dev, SOURCE, 'la_block', _block_defines(dtype, width, out, dots if out else 0))
+        groups = B * H * (nseg if out else nseg - 1)
+        hw.launch_bytes(k, dev, -(-groups // 8) * 8 * tiles, len(jobs), 256, blob)
+
+
 def _forward(q, k, v, g, state, lengths, scale):
     B, T, Hk, N = k.shape
     H, M = v.shape[2], v.shape[3]
     dev = q.device
+    q, k, v = _near(q), _near(k), _near(v)
     y = th.empty((B, T, H, M), dtype=v.dtype, device=dev)
     out = th.empty((B, H, M, N), dtype=th.float32, device=dev) if state is None else th.empty_like(state)
-    defines = _fw_defines(q.dtype, N)
-    width, L = defines[2][1], defines[3][1]
-    blocks, tiles = -(-T // L), -(-M // 64)
-    nseg, per = _segments(B * H * tiles, blocks)
-    local = totals = None
-    gate, s0 = _gate(g), _states(state)
-    if nseg > 1:
-        local = th.empty(B * H * (nseg - 1) * tiles * 64 * width, dtype=th.float32, device=dev)
-        totals = th.empty(B * H * (nseg - 1), dtype=th.float64, device=dev)
-        job = (*_btH(k), *_btH(v), *_states(None), *_states(None), 0, local.data_ptr(), totals.data_ptr(), N, M, Hk, H, 0)
-        _walk(dev, q.dtype, N, L, [job], gate, lengths, B, T, H, nseg, per, True, tiles, scale)
-    groups = B * H * nseg
-    hw.launch(hw.kernel(dev, SOURCE, 'la_fw', defines), dev, -(-groups // 8) * 8 * tiles, 256, _FW,
-              *_btH(q), *_btH(k), *_btH(v), *gate, *s0, *_states(out), y.data_ptr(), _ptr(lengths), _ptr(local), _ptr(totals),
-              B, T, H, Hk, M, N, nseg, per, scale)
+    job = _job(_Role(q), _Role(k), _Role(v), None, N, M, _states(state), _states(out), y.data_ptr(), (T * H * M, H * M, M, 0, 1), DTYPES[v.dtype], out_scale=scale)
+    _walk(dev, q.dtype, [job], _gate(g), lengths, B, T, H)
     return y, out
-
-
-_NO_JOB = (0,) * 32
-
-
-def _walk(dev, dtype, width, L, jobs, gate, lengths, B, T, H, nseg, per, only_local, tiles, scale):
-    groups = B * H * (nseg - 1 if only_local else nseg)
-    flat = [*jobs[0], *(jobs[1] if len(jobs) > 1 else _NO_JOB)]
-    hw.launch(hw.kernel(dev, SOURCE, 'la_walk', _walk_defines(dtype, width, L)), dev, -(-groups // 8) * 8 * tiles, 256, _WALK,
-              *flat, *gate, _ptr(lengths), B, T, H, nseg, per, int(only_local), tiles, scale, grid_y=len(jobs))
 
 
 def _backward(q, k, v, g, state, lengths, dy, dstate, scale, need_g, need_state):
     B, T, Hk, N = k.shape
     H, M = v.shape[2], v.shape[3]
     dev, dt = q.device, q.dtype
-    defines = _grad_defines(dt, M, N)
-    wm, L = defines[2][1], defines[4][1]
-    blocks, tiles = -(-T // L), -(-N // 64)
+    q, k, v, dy = _near(q), _near(k), _near(v), _near(dy)
     gate = _gate(g)
     dq, dk, dv = (th.empty(x.shape, dtype=dt, device=dev) for x in (q, k, v))
-    ds = None
-    if need_state:
-        ds = th.empty_like(state)
-    # the state in front of every block and the gradient of the one behind it
-    marks = th.empty((2, B * H * blocks * -(-N // 16) * 16 * wm), dtype=th.float32, device=dev)
-    nseg, per = _segments(2 * B * H * tiles, blocks)
-    local = totals = None
-    if nseg > 1:
-        local = th.empty((2, B * H * (nseg - 1) * tiles * 64 * wm), dtype=th.float32, device=dev)
-        totals = th.empty((2, B * H * (nseg - 1)), dtype=th.float64, device=dev)
-
-    def jobs(only_local):
-        def one(i, a, b, init, fin):
-            scratch = (0, 0) if local is None else (local[i].data_ptr(), totals[i].data_ptr())
-            return (*_btH(a), *_btH(b), *_states(init), *_states(fin), 0 if only_local else marks[i].data_ptr(), *scratch, M, N, H, Hk, i)
-        return [one(0, v, k, state, None), one(1, dy, q, dstate, ds)]
-
-    for only_local in ((True, False) if nseg > 1 else (False,)):
-        _walk(dev, dt, M, L, jobs(only_local), gate, lengths, B, T, H, nseg, per, only_local, tiles, scale)
-    # heads that share a query and key: one workgroup sums what it can of them, as long as the chip stays full
+    ds = th.empty_like(state) if need_state else None
+    # heads that share a query and key each have their own share of its gradient
     share = H // Hk
-    slices = 1
-    while slices < share and B * blocks * Hk * slices < WORKGROUPS:
-        slices *= 2
-    slices = min(slices, share)
-    slices = -(-share // -(-share // slices))
-    if slices > 1:
-        part = th.empty((2, slices, B, T, Hk, N), dtype=th.float32, device=dev)
-        pq, pk = part[0], part[1]
-    else:
-        pq, pk = dq, dk
-    per_head = g.ndim == 1
-    dg = dg_out = None
+    pq, pk, type_ = (dq, dk, DTYPES[dt]) if share == 1 else (*th.empty((2, share, B, T, Hk, N), dtype=th.float32, device=dev), 2)
+    strides = (T * Hk * N, Hk * N, N, B * T * Hk * N, share)
+    dots = marks = None
+    tiles, spans = -(-N // 64), -(-T // (BLOCK * MARK_BLOCKS))
+    size = -(-N // 16) * 16 * _width(M)
     if need_g:
-        dg_out = dg = th.empty(g.shape, dtype=g.dtype, device=dev)
+        dots = th.empty((2, tiles, B * H, T), dtype=th.float32, device=dev)
+        marks = th.empty((2, B * H * spans * size), dtype=th.float32, device=dev)
+    rq, rk, rv, ry = (_Role(t) for t in (q, k, v, dy))
+    extra = [dict(dots=dots[i].data_ptr(), marks=marks[i].data_ptr()) if need_g else {} for i in range(2)]
+    none = _states(None)
+    _walk(dev, dt, [_job(ry, rv, rk, rq, M, N, _states_t(state), none, pq.data_ptr(), strides, type_, pairs=1, out_scale=scale, **extra[0]),
+                    _job(rv, ry, rq, rk, M, N, _states_t(dstate), _states_t(ds), pk.data_ptr(), strides, type_, back=1, in_scale=scale, **extra[1])],
+          gate, lengths, B, T, H, dots=int(need_g))
+    _walk(dev, dt, [_job(rk, rq, ry, None, N, M, _states(dstate), none, dv.data_ptr(), (T * H * M, H * M, M, 0, 1), DTYPES[dt], back=1, in_scale=scale)],
+          gate, lengths, B, T, H)
+    if share > 1:
+        hw.slice_sum(pq, share, dq)
+        hw.slice_sum(pk, share, dk)
+    dg = None
+    if need_g:
+        per_head = g.ndim == 1
+        dg = th.empty(g.shape, dtype=g.dtype, device=dev)
+        out = th.empty((B, T, H), dtype=th.float32, device=dev) if per_head else dg
+        hw.launch(hw.kernel(dev, SOURCE, 'la_gate', _GATE_DEFINES), dev, B * H * spans, 256, _GATE,
+                  dots[0].data_ptr(), dots[1].data_ptr(), marks[0].data_ptr(), marks[1].data_ptr(), *gate, out.data_ptr(), _ptr(lengths),
+                  B, T, H, tiles, MARK_BLOCKS, size, DTYPES[out.dtype])
         if per_head:
-            dg_out = th.empty((B, T, H), dtype=th.float32, device=dev)
-    hw.launch(hw.kernel(dev, SOURCE, 'la_grad', defines), dev, blocks * slices * B * Hk, 64 * defines[5][1], _GRAD,
-              *_btH(q), *_btH(k), *_btH(v), *_btH(dy), *gate, marks[0].data_ptr(), marks[1].data_ptr(), pq.data_ptr(), pk.data_ptr(),
-              dv.data_ptr(), _ptr(dg_out), _ptr(lengths), B, T, H, Hk, M, N, slices, 2 if dg_out is None else DTYPES[dg_out.dtype], scale)
-    if slices > 1:
-        hw.slice_sum(pq, slices, dq)
-        hw.slice_sum(pk, slices, dk)
-    if need_g and per_head:
-        hw.slice_sum(dg_out, B * T, dg)
+            hw.slice_sum(out, B * T, dg)
     return dq, dk, dv, dg, ds
 
 
@@ -229,7 +217,7 @@ def _step(q, k, v, g, state, scale):
         lanes *= 2
     rows = min(M, 256 // lanes * 4)
     hw.launch(hw.kernel(dev, SOURCE, 'la_step', _step_defines(q.dtype)), dev, B * H * -(-M // rows), 256, _STEP,
-              *_tensor(q, 0, None, 1), *_tensor(k, 0, None, 1), *_tensor(v, 0, None, 1), *_gate(g), *_states(state), y.data_ptr(),
+              *_tensor(q, 0, None, 1), *_tensor(k, 0, None, 1), *_tensor(v, 0, None, 1), *_gate(g), *_states_t(state), y.data_ptr(),
               B, H, Hk, M, N, int(wide), lanes, rows, scale)
     return y
 
