@@ -24,6 +24,9 @@
 //   W      padded width (64, 128 or 256) of q and k
 //   OUT    0: the state alone (what a segment of a sequence leaves behind)
 //   DOTS   1: also what the gradient of g is made of
+//   FAST   1: every operand allows 16-byte loads and rows of y are a multiple of four long.  Without the branches and the
+//          second set of loads and stores that any other layout needs, a block takes a fifth less time
+//   WIDE   with FAST, the type of y: 0 the operands', 1 float32
 //   NBUF   operand tiles in LDS: 2 lets a block's operands arrive while the one before is read, 1 saves LDS
 //   OCC    waves per SIMD to compile for
 //
@@ -63,8 +66,9 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 #define DEV_MEMBER __device__ __forceinline__
 #define FENCE __builtin_amdgcn_sched_barrier(0)
 
-#ifndef IN
-#error "IN is not defined"
+#ifndef FAST
+#define FAST 0
+#define WIDE 0
 #endif
 
 constexpr int ESZ = IN == 2 ? 4 : 2;          // bytes per element of q, k, v, dy
@@ -96,13 +100,14 @@ DEV u32 pack_rne(float a, float b) {           // two floats to bfloat16, to nea
 DEV u32 pack_top(float a, float b) { return __builtin_amdgcn_perm(as_u(b), as_u(a), 0x07060302u); }
 
 // NP parts of the two floats a, b: parts [0, NP-1) by truncation (what is left is exact), the last one to nearest.
-template <int NP>
+// With INF an infinity is a part by itself; without, it leaves a NaN behind (as its products with zeros would).
+template <int NP, bool INF = false>
 DEV void split2(float a, float b, u32* out, int stride) {
   for (int i = 0; i < NP - 1; i++) {
     const float ta = as_f(as_u(a) & 0xffff0000u), tb = as_f(as_u(b) & 0xffff0000u);
     out[i * stride] = pack_top(a, b);
-    a = a == ta ? 0.f : a - ta;                // (an infinity leaves nothing behind; a NaN stays one)
-    b = b == tb ? 0.f : b - tb;
+    a = INF && a == ta ? 0.f : a - ta;
+    b = INF && b == tb ? 0.f : b - tb;
   }
   out[(NP - 1) * stride] = pack_rne(a, b);
 }
@@ -112,11 +117,11 @@ struct Frag {        // 8 elements of the reduction index per lane, NP parts
   v4u d[NP];
 };
 
-template <int NP>
+template <int NP, bool INF = false>
 DEV Frag<NP> make_frag(const float* x) {
   Frag<NP> f;
   u32 t[NP * 4];
-  for (int i = 0; i < 4; i++) split2<NP>(x[2 * i], x[2 * i + 1], t + i, 4);
+  for (int i = 0; i < 4; i++) split2<NP, INF>(x[2 * i], x[2 * i + 1], t + i, 4);
   for (int p = 0; p < NP; p++) f.d[p] = v4u{t[4 * p], t[4 * p + 1], t[4 * p + 2], t[4 * p + 3]};
   return f;
 }
@@ -254,7 +259,7 @@ DEV void store_parts(u16* at, const Raw& r) {
       if constexpr (IN == FP16) x[e] = half_to_f((u16)(r.d[0][e / 2] >> (e % 2 * 16)));
       else x[e] = as_f(r.d[e / 4][e % 4]);
     }
-    const Frag<RP> f = make_frag<RP>(x);
+    const Frag<RP> f = make_frag<RP, true>(x);
     for (int p = 0; p < RP; p++) *(v4u*)(at + p * PLANE) = f.d[p];
   }
 }
@@ -289,7 +294,7 @@ struct Staging {
   DEV_MEMBER void load(int tokens) {
     const Buffer from = buffer_at(at);
     at += step;
-    if (vec) {
+    if (FAST || vec) {
 #pragma unroll
       for (int i = 0; i < N; i++) {
         const u32 o = token + i * dir < tokens ? off[i] : NOTHING;
@@ -298,7 +303,11 @@ struct Staging {
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < N; i++) r[i] = load_apart(from, off[i], sn, token + i * dir < tokens ? left : 0);
+      for (int i = 0; i < N; i++) {
+        u32 apart = sn;
+        asm volatile("" : "+s"(apart));          // (or eight addresses a piece are kept in registers for this path)
+        r[i] = load_apart(from, off[i], apart, token + i * dir < tokens ? left : 0);
+      }
     }
   }
   DEV_MEMBER void store(u16* tile, int tid) {
@@ -365,7 +374,7 @@ struct Decays {
   alignas(16) float hi[L];
   alignas(16) float lo[L];
   alignas(16) float from_start[L];             // exp(G_i); the last one is the whole block's
-  alignas(16) float to_end[L];                 // exp(G_L - G_i)
+  alignas(16) float to_end[L];                 // exp(G_L - G_i), times the scale of what enters the state
 };
 
 DEV float exp2_sum(float hi, float lo) {       // 2^(hi + lo), |lo| far below 1
@@ -374,7 +383,7 @@ DEV float exp2_sum(float hi, float lo) {       // 2^(hi + lo), |lo| far below 1
 }
 
 // one wave prepares two blocks: lane i of either half holds token i's g (0 behind the last token); returns the sum of g
-DEV double fill_decays(Decays* first, Decays* second, double g, int lane) {
+DEV double fill_decays(Decays* first, Decays* second, double g, float in_scale, int lane) {
   const double G = scan32(g);
   const double end0 = read_lane(G, 31), end1 = read_lane(G, 63);
   const double G2 = G * LOG2E, E2 = (lane < L ? end0 : end1) * LOG2E;
@@ -386,13 +395,8 @@ DEV double fill_decays(Decays* first, Decays* second, double g, int lane) {
   d->lo[i] = lo;
   d->from_start[i] = exp2_sum(hi, lo);
   const float th = (float)to;
-  d->to_end[i] = exp2_sum(th, (float)(to - (double)th));
+  d->to_end[i] = exp2_sum(th, (float)(to - (double)th)) * in_scale;
   return end0 + end1;
-}
-
-DEV f4 decay_between(const Decays& d, int i, int j) {     // tokens j..j+3 to token i
-  const f4 x = (d.hi[i] - *(const f4*)(d.hi + j)) + (d.lo[i] - *(const f4*)(d.lo + j));
-  return f4{__builtin_amdgcn_exp2f(x[0]), __builtin_amdgcn_exp2f(x[1]), __builtin_amdgcn_exp2f(x[2]), __builtin_amdgcn_exp2f(x[3])};
 }
 
 // Workgroups go to the 8 XCDs in turn; the `n` workgroups of one group (which read the same operands) get numbers 8 apart
@@ -444,18 +448,14 @@ DEV void store_in(Buffer to, u32 off, f4 x, int n, bool whole) {
 #ifdef KERNEL_BLOCK
 // One workgroup walks the blocks of one (batch, head, segment) for 64 of v's columns; wave w owns 16 of them: its share of
 // the state, S^T [W x 16], stays in accumulators.  q and k are read by every workgroup of a head (up to four, on one XCD).
-// A block: waves 0..2 form the three 16 x 16 tiles of P on and below the diagonal while wave 3 prepares the next block's
-// decays; every wave then adds the state's share of its columns of y, updates its state, and, once P is complete, adds the
-// block's own share.  The next block's operands are on their way into registers meanwhile.
+// A block: three waves form the 16 x 16 tiles of P on and below the diagonal; every wave adds the state's share of its
+// columns of y, the block's own share, and updates its state.  The operands of blocks to come are on their way into
+// registers meanwhile.
 //
 // With DOTS the walk also leaves, per token, what the gradient of g is made of (see la_gate): forwards (dq) the products
 // q_i.dq_i with the block's own share taken from unrounded numbers, less the share of each j; backwards (dk) the products
 // k_j.dk_j of the state's share.  x is the operand of these products (q, k), in the 64 columns that the workgroup owns;
 // sums over column tiles are left to la_gate.  At every MARK-th block's border the state is written down too.
-#ifndef DOTS
-#define DOTS 0
-#endif
-
 struct Job {
   Tensor q, k, v, x;
   States init, fin;
@@ -477,10 +477,11 @@ struct BlockArgs {
 };
 
 constexpr int NT = W / 16, LT = 2;
+constexpr int SPARTS = DOTS ? 3 : RP, SLIM = DOTS ? 2 : CALC;
 constexpr int QB = RP == 1 ? (W < 128 ? W / 32 : 4) : RP == 2 ? 2 : 1;       // operands read ahead: what 32 registers hold
 constexpr int KB = RP == 1 ? 4 : RP == 2 ? 2 : 2;
+constexpr bool AHEAD = OUT && RP == 1 && SPARTS == 1 && W <= 128;            // the state as a factor: what 16 registers hold
 constexpr int SQ = stride_along(W), SK = stride_down(W), SV = stride_down(64), SX = stride_along(64), SP = stride_along(L);
-constexpr int SPARTS = DOTS ? 3 : RP, SLIM = DOTS ? 2 : CALC;
 constexpr int AT_K = OUT ? RP * L * SQ : 0, AT_V = AT_K + RP * L * SK, AT_X = AT_V + RP * L * SV, STAGE = AT_X + (DOTS ? RP * L * SX : 0);
 
 template <int TYPE>
@@ -504,14 +505,23 @@ DEV void store_state(const f4* S, float e, char* to, i64 at, i64 step, int rows,
     }
 }
 
+DEV Frag<SPARTS> state_frag(const f4* S, int ks) {             // rows 32 ks + {4g..4g+3, 16+4g..16+4g+3} of a column
+  const f4 u = S[2 * ks], v = S[2 * ks + 1];
+  const float x[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+  return make_frag<SPARTS>(x);
+}
+
 extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) {
   __shared__ __attribute__((aligned(16))) u16 stage[NBUF][STAGE];
-  __shared__ Decays decays[4];
+  __shared__ Decays decays[16];
 #if OUT
-  __shared__ __attribute__((aligned(16))) u16 P[RP * L * SP];
+  __shared__ __attribute__((aligned(16))) u16 P[NBUF][RP * L * SP];
+#endif
+#if !OUT
+  __shared__ double totals[4];
 #endif
 #if DOTS
-  __shared__ float of_rows[LT][L], of_cols[LT][L], of_state[4][L];
+  __shared__ float of_rows[NBUF][LT][L], of_cols[NBUF][LT][L], of_state[4][L];
 #endif
   const Job& job = args.job[blockIdx.y];
   const int tid = threadIdx.x, lane = tid & 63, p = lane & 15, g = lane >> 4;
@@ -524,12 +534,12 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   const i64 bh = group / nseg, seg = group % nseg, b = bh / args.H, h = bh % args.H;
   const int c0 = tile * 64, cw = c0 + 16 * w, cols = C - c0 < 64 ? C - c0 : 64;
   const bool back = job.back != 0;
-  const i64 T = args.T, len = length_of(args.lengths, b, T);
-  const i64 nall = (T + L - 1) / L, nreal = (len + L - 1) / L;       // blocks; blocks with a token
+  const int T = (int)args.T, len = (int)length_of(args.lengths, b, T);
+  const int nall = (T + L - 1) / L, nreal = (len + L - 1) / L;       // blocks; blocks with a token
   // this segment's steps: step o is block o, or nall - 1 - o backwards; those without a token only clear y
-  const i64 s0 = seg * args.per, s1 = s0 + args.per < nall ? s0 + args.per : nall;
-  const i64 first = back && s0 < nall - nreal ? (nall - nreal < s1 ? nall - nreal : s1) : s0;
-  const i64 last = back || s1 < nreal ? s1 : (nreal > s0 ? nreal : s0);
+  const int s0 = (int)(seg * args.per), s1 = s0 + (int)args.per < nall ? s0 + (int)args.per : nall;
+  const int first = back && s0 < nall - nreal ? (nall - nreal < s1 ? nall - nreal : s1) : s0;
+  const int last = back || s1 < nreal ? s1 : (nreal > s0 ? nreal : s0);
 
   f4 S[NT];                 // column cw + p, rows 16 nt + 4 g + r
 #pragma unroll
@@ -550,22 +560,23 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     const f4* from = (const f4*)job.local + ((at * ntiles + tile) * 4 + w) * (NT * 64) + lane;
     for (int nt = 0; nt < NT; nt++) S[nt] = S[nt] * e + from[nt * 64];
   }
-  for (int i = tid; i < RP * L * SP / 8; i += 256) *(v4u*)(P + 8 * i) = v4u{0, 0, 0, 0};     // (stays zero above the diagonal)
+  for (int i = tid; i < NBUF * RP * L * SP / 8; i += 256) *(v4u*)(&P[0][0] + 8 * i) = v4u{0, 0, 0, 0};     // (stays zero above the diagonal)
 #endif
 #if DOTS
-  if (tid < LT * L) (&of_rows[0][0])[tid] = (&of_cols[0][0])[tid] = 0.f;
-  const i64 spans = (nall + args.span - 1) / args.span;
-  const auto mark = [&](i64 span) {
+  if (tid < NBUF * LT * L) (&of_rows[0][0][0])[tid] = (&of_cols[0][0][0])[tid] = 0.f;
+  const int span = (int)args.span, spans = (nall + span - 1) / span;
+  const auto mark = [&](int at) {
     if (cw >= C) return;
-    f4* to = (f4*)job.marks + ((bh * spans + span) * ((C + 15) / 16) + cw / 16) * (NT * 64) + lane;
+    f4* to = (f4*)job.marks + ((bh * spans + at) * ((C + 15) / 16) + cw / 16) * (NT * 64) + lane;
     for (int nt = 0; nt < NT; nt++) to[nt * 64] = S[nt];
   };
 #endif
 
+  const float in_scale = (float)job.in_scale;
   // a block o's operands, from the first block that this segment has
-  const auto block_of = [&](i64 o) { return back ? nall - 1 - o : o; };
+  const auto block_of = [&](int o) { return back ? nall - 1 - o : o; };
   const auto start = [&](auto& r, const Tensor& t, i64 heads, int col, int n) {
-    r.init(t, t.p + (b * t.sb + h / (args.H / heads) * t.sh + block_of(first) * L * t.st + col * t.sn) * ESZ, n, back, tid);
+    r.init(t, t.p + (b * t.sb + h / (args.H / heads) * t.sh + (i64)block_of(first) * L * t.st + col * t.sn) * ESZ, n, back, tid);
   };
   Staging<W, SK> rk;
   Staging<64, SV> rv;
@@ -579,9 +590,9 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   Staging<64, SX> rx;
   start(rx, job.x, job.Hx, c0, cols);
 #endif
-  const auto fetch = [&](i64 o) {
-    const i64 rest = len - block_of(o) * L;
-    const int tokens = rest < L ? (int)rest : L;
+  // (always a block further; behind the last one nothing is read)
+  const auto fetch = [&](int o) {
+    const int tokens = o < last ? len - block_of(o) * L : 0;
 #if OUT
     rq.load(tokens);
 #endif
@@ -601,164 +612,197 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     rx.store(to + AT_X, tid);
 #endif
   };
-  // wave 3's lanes hold g of a block and the one behind it, and those of two more in reserve; backwards a row's is the one
-  // of the token behind it
-  const auto gate = [&](i64 o) {
+  // Decays are prepared for eight blocks at a time, two by each wave (a block per half); backwards a row's gate is the one
+  // of the token behind it.  `rg`: the gates of the eight blocks after those.
+  const auto gates = [&](int o) {
     const int i = lane & (L - 1);
-    o += lane / L;
-    const i64 t = block_of(o) * L + (back ? L - i : i);
+    o += 2 * w + lane / L;
+    const int t = block_of(o) * L + (back ? L - i : i);
     return o < last && t < len ? raw_gate(args.g, b, h, t) : 0u;         // (zero is 0.0 in every type)
   };
-  u32 rg = 0;
   double total = 0.0;
+  const auto fill = [&](int o, u32 raw) {
+    const int at = (o - first + 2 * w) & 15;
+    total += fill_decays(decays + at, decays + at + 1, gate_value(args.g, raw), in_scale, lane);
+  };
+  u32 rg = 0;
   if (first < last) {
     fetch(first);
-    if (w == 3) {
-      const u32 now = gate(first);
-      rg = gate(first + 2);
-      total = fill_decays(decays + (first & 3), decays + (first + 1 & 3), gate_value(args.g, now), lane);
+    const u32 now = gates(first);
+    rg = gates(first + 8);
+    fill(first, now);
+    put(stage[0]);
+    if constexpr (NBUF == 2) {
+      fetch(first + 1);
+      put(stage[1]);
     }
-    put(stage[first % NBUF]);
   }
   __syncthreads();
-  const float in_scale = (float)job.in_scale;
 #if OUT
   const float out_scale = (float)job.out_scale;
-  const bool wide = job.out_type == FP32;        // (or of the operands' type)
+  const bool wide = FAST ? WIDE != 0 : job.out_type == FP32;       // (or of the operands' type)
+  const bool whole = FAST || C % 4 == 0;
   const int size = wide ? 4 : ESZ;
   const i64 out_at = b * job.ob + h / job.share * job.og + h % job.share * job.os;
-  char* to = job.out + (out_at + block_of(first) * L * job.ot) * size;
+  char* to = job.out + (out_at + (i64)block_of(first) * L * job.ot) * size;
   const i64 to_step = (back ? -L : L) * job.ot * size;
   u32 to_off[LT];
 #pragma unroll
-  for (int it = 0; it < LT; it++) to_off[it] = (u32)((back ? L - 1 - (16 * it + p) : 16 * it + p) * job.ot + cw + 4 * g) * size;
+  for (int i = 0; i < LT; i++) to_off[i] = (u32)((back ? L - 1 - (16 * i + p) : 16 * i + p) * job.ot + cw + 4 * g) * size;
+
+  // waves 0..2 each form a tile of P: column pi, rows pj..pj+3 (wave 3 goes along and keeps nothing)
+  const int it = w > 0, jt = w > 1, pi = 16 * it + p, pj = 16 * jt + 4 * g;
+  struct Pair {
+    f4 apart;
+    Frag<RP> kj[QB], qi[QB];
+  };
+  const auto pair_operands = [&](Pair& x, const u16* tiles, int k0) {
+#pragma unroll
+    for (int ks = 0; ks < QB; ks++) {
+      x.kj[ks] = along8<SK>(tiles + AT_K, 16 * jt + p, 32 * (k0 + ks), g);
+      x.qi[ks] = along8<SQ>(tiles, pi, 32 * (k0 + ks), g);
+    }
+  };
+  const auto pair_begin = [&](Pair& x, const u16* tiles, const Decays& D) {
+    x.apart = (D.hi[pi] - *(const f4*)(D.hi + pj)) + (D.lo[pi] - *(const f4*)(D.lo + pj));
+    pair_operands(x, tiles, 0);
+  };
+  const auto pair_product = [&](Pair& x, const u16* tiles) {
+    f4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k0 = 0; k0 < W / 32; k0 += QB) {
+      if (k0 > 0) pair_operands(x, tiles, k0);
+#pragma unroll
+      for (int ks = 0; ks < QB; ks++) c = mul<RAW>(x.kj[ks], x.qi[ks], c);
+    }
+    return c;
+  };
+  const auto pair_end = [&](const Pair& x, f4 c, const u16* tiles, int o) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) c[r] = pj + r <= pi ? c[r] * (__builtin_amdgcn_exp2f(x.apart[r]) * in_scale) : 0.f;
+    u32 d[RP * 2];
+    split2<RP>(c[0], c[1], d, 2);
+    split2<RP>(c[2], c[3], d + 1, 2);
+    if (w < 3) {
+#pragma unroll
+      for (int q = 0; q < RP; q++) *(v2u*)(P[o % NBUF] + (q * L + pi) * SP + pj) = v2u{d[2 * q], d[2 * q + 1]};
+    }
+#if DOTS
+    if (job.pairs && w < 3) {
+      f4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < 2; ks++) a = mul<RAW>(along8<SV>(tiles + AT_V, 16 * jt + p, 32 * ks, g), along8<SX>(tiles + AT_X, pi, 32 * ks, g), a);
+      float row = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float s = c[r] * a[r];
+        row += s;
+        const float col = sum16(s);
+        if (p == 0) of_cols[o % NBUF][it][pj + r] = col;
+      }
+      row = sum_groups(row);
+      if (g == 0) of_rows[o % NBUF][jt][pi] = row;
+    }
+#endif
+  };
+  if constexpr (NBUF == 2) {
+    Pair x;
+    pair_begin(x, stage[0], decays[0]);
+    pair_end(x, pair_product(x, stage[0]), stage[0], 0);
+    __syncthreads();
+  }
 #endif
 #if DOTS
   // (the state behind the last token, and the gradient that comes in there, are the end of the last span)
-  if (back && first < last && block_of(first) == nreal - 1) mark((nreal - 1) / args.span);
+  if (back && first < last && block_of(first) == nreal - 1) mark((nreal - 1) / span);
 #endif
-  const auto next_decays = [&](i64 o) {          // every other block, for the two behind the next one
-    if (((o - first) & 1) != 0 && o + 1 < last) {
-      total += fill_decays(decays + (o + 1 & 3), decays + (o + 2 & 3), gate_value(args.g, rg), lane);
-      rg = gate(o + 3);
-    }
-  };
-  for (i64 o = first; o < last; o++) {
-    const u16* tiles = stage[o % NBUF];
+  for (int o = first; o < last; o++) {
+    // With two tiles in LDS, P of the block behind this one is formed here, so that nothing waits for it; with one, this
+    // block's.
+    const int n = o - first, pn = NBUF == 2 ? n + 1 : n;
+    const u16* tiles = stage[n % NBUF];
     const u16 *K = tiles + AT_K, *V = tiles + AT_V;
-    const Decays& D = decays[o & 3];
-    if (o + 1 < last) fetch(o + 1);
-    // operands are read from LDS a group ahead of their use, and stay there: hence the fences for the scheduler
-    const Frag<RP> vf = down<SV>(V, 0, 16 * w, lane);
-    const f4 to0 = *(const f4*)(D.to_end + 4 * g), to1 = *(const f4*)(D.to_end + 16 + 4 * g);
+    const Decays& D = decays[n & 15];
+    fetch(o + NBUF);
+    // What a block needs is read from LDS well ahead of its use, and what can be computed without it - the state as a
+    // factor, the decayed state, the parts of the decayed v - fills the wait; the fences keep it in that order.
     const float all = D.from_start[L - 1];
+    const f4 to0 = *(const f4*)(D.to_end + 4 * g), to1 = *(const f4*)(D.to_end + 16 + 4 * g);
+    const Frag<RP> vf = down<SV>(V, 0, 16 * w, lane);
 #if OUT
     const u16* Q = tiles;
     const float from[LT] = {D.from_start[p], D.from_start[16 + p]};
+    Pair pair;
+    pair_begin(pair, stage[pn % NBUF], decays[pn & 15]);
     Frag<RP> qf[QB][LT];
 #pragma unroll
     for (int x = 0; x < QB; x++)
 #pragma unroll
-      for (int it = 0; it < LT; it++) qf[x][it] = along<SQ>(Q, 16 * it + p, 32 * x, g);
+      for (int i = 0; i < LT; i++) qf[x][i] = along<SQ>(Q, 16 * i + p, 32 * x, g);
     FENCE;
-    if (w == 3) {
-      next_decays(o);
-    } else {
-      const int it = w > 0, jt = w > 1;
-      f4 x = {0.f, 0.f, 0.f, 0.f};               // column i = 16 it + p, rows j = 16 jt + 4 g + r
+    Frag<SPARTS> sf[AHEAD ? NT / 2 : 1];
+    if constexpr (AHEAD) {
 #pragma unroll
-      for (int k0 = 0; k0 < W / 32; k0 += QB) {
-        Frag<RP> kj[QB], qi[QB];
+      for (int x = 0; x < NT / 2; x++) sf[x] = state_frag(S, x);
 #pragma unroll
-        for (int ks = 0; ks < QB; ks++) {
-          kj[ks] = along8<SK>(K, 16 * jt + p, 32 * (k0 + ks), g);
-          qi[ks] = along8<SQ>(Q, 16 * it + p, 32 * (k0 + ks), g);
-        }
-        FENCE;
-#pragma unroll
-        for (int ks = 0; ks < QB; ks++) x = mul<RAW>(kj[ks], qi[ks], x);
-      }
-      const int i = 16 * it + p, j = 16 * jt + 4 * g;
-      const f4 e = decay_between(D, i, j) * in_scale;
-#pragma unroll
-      for (int r = 0; r < 4; r++) x[r] = j + r <= i ? x[r] * e[r] : 0.f;
-      u32 d[RP * 2];
-      split2<RP>(x[0], x[1], d, 2);
-      split2<RP>(x[2], x[3], d + 1, 2);
-#pragma unroll
-      for (int q = 0; q < RP; q++) *(v2u*)(P + (q * L + i) * SP + j) = v2u{d[2 * q], d[2 * q + 1]};
-#if DOTS
-      if (job.pairs) {
-        const u16* X = tiles + AT_X;
-        f4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++) a = mul<RAW>(along8<SV>(V, 16 * jt + p, 32 * ks, g), along8<SX>(X, 16 * it + p, 32 * ks, g), a);
-        float row = 0.f;
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const float s = x[r] * a[r];
-          row += s;
-          const float col = sum16(s);
-          if (p == 0) of_cols[it][j + r] = col;
-        }
-        row = sum_groups(row);
-        if (g == 0) of_rows[jt][i] = row;
-      }
-#endif
+      for (int nt = 0; nt < NT; nt++) S[nt] *= all;
     }
 #else
-    if (w == 3) next_decays(o);
+    FENCE;
+#endif
+    float vx[8];
+    frag_values(vf, vx);
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      vx[r] *= to0[r];
+      vx[4 + r] *= to1[r];
+    }
+    const Frag<3> vd = make_frag<3>(vx);
+    FENCE;
+#if OUT
+    f4 y[LT];                                    // column i = 16 it + p, rows cw + 4 g + r
+#pragma unroll
+    for (int i = 0; i < LT; i++) y[i] = f4{0.f, 0.f, 0.f, 0.f};
+    const f4 product = pair_product(pair, stage[pn % NBUF]);
 #endif
     Frag<RP> kf[KB];
 #pragma unroll
     for (int x = 0; x < KB; x++) kf[x] = down<SK>(K, 0, 16 * x, lane);
     FENCE;
 #if OUT
-    f4 y[LT];                                    // column i = 16 it + p, rows cw + 4 g + r
-#pragma unroll
-    for (int it = 0; it < LT; it++) y[it] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k0 = 0; k0 < W / 32; k0 += QB) {
 #pragma unroll
       for (int ks = 0; ks < QB; ks++) {
-        const f4 u = S[2 * (k0 + ks)], v = S[2 * (k0 + ks) + 1];
-        const float x[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-        const Frag<SPARTS> s = make_frag<SPARTS>(x);
+        const Frag<SPARTS> s = AHEAD ? sf[AHEAD ? k0 + ks : 0] : state_frag(S, k0 + ks);
 #pragma unroll
-        for (int it = 0; it < LT; it++) y[it] = mul<SLIM>(s, qf[ks][it], y[it]);
+        for (int i = 0; i < LT; i++) y[i] = mul<SLIM>(s, qf[ks][i], y[i]);
       }
       if (k0 + QB < W / 32) {
 #pragma unroll
         for (int x = 0; x < QB; x++)
 #pragma unroll
-          for (int it = 0; it < LT; it++) qf[x][it] = along<SQ>(Q, 16 * it + p, 32 * (k0 + QB + x), g);
+          for (int i = 0; i < LT; i++) qf[x][i] = along<SQ>(Q, 16 * i + p, 32 * (k0 + QB + x), g);
         FENCE;
       }
     }
+    pair_end(pair, product, stage[pn % NBUF], pn);
 #pragma unroll
-    for (int it = 0; it < LT; it++) y[it] *= from[it];
+    for (int i = 0; i < LT; i++) y[i] *= from[i];
 #if DOTS
 #pragma unroll
-    for (int it = 0; it < LT; it++) {
+    for (int i = 0; i < LT; i++) {
       float s = 0.f;
 #pragma unroll
       for (int q = 0; q < RP; q++) {
-        const v2u x = *(const v2u*)(tiles + AT_X + (q * L + 16 * it + p) * SX + 16 * w + 4 * g);
-        s += y[it][0] * as_f(x[0] << 16) + y[it][1] * as_f(x[0] & 0xffff0000u) + y[it][2] * as_f(x[1] << 16) + y[it][3] * as_f(x[1] & 0xffff0000u);
+        const v2u x = *(const v2u*)(tiles + AT_X + (q * L + 16 * i + p) * SX + 16 * w + 4 * g);
+        s += y[i][0] * as_f(x[0] << 16) + y[i][1] * as_f(x[0] & 0xffff0000u) + y[i][2] * as_f(x[1] << 16) + y[i][3] * as_f(x[1] & 0xffff0000u);
       }
       s = sum_groups(s);
-      if (g == 0) of_state[w][16 * it + p] = s;
+      if (g == 0) of_state[w][16 * i + p] = s;
     }
 #endif
 #endif
-    float vx[8];
-    frag_values(vf, vx);
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      vx[r] *= to0[r] * in_scale;
-      vx[4 + r] *= to1[r] * in_scale;
-    }
-    const Frag<3> vd = make_frag<3>(vx);
 #pragma unroll
     for (int n0 = 0; n0 < NT; n0 += KB) {
       Frag<RP> next[KB];
@@ -767,8 +811,10 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
         for (int x = 0; x < KB; x++) next[x] = down<SK>(K, 0, 16 * (n0 + KB + x), lane);
         FENCE;
       }
+      if constexpr (!AHEAD) {
 #pragma unroll
-      for (int x = 0; x < KB; x++) S[n0 + x] *= all;
+        for (int x = 0; x < KB; x++) S[n0 + x] *= all;
+      }
       mul_each<KB, 2>(kf, vd, S + n0);
       if (n0 + KB < NT) {
 #pragma unroll
@@ -776,51 +822,56 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
       }
     }
 #if OUT
-    __syncthreads();
+    if constexpr (NBUF == 1) __syncthreads();
     {
-      const Frag<RP> p0 = along<SP>(P, p, 0, g), p1 = along<SP>(P, 16 + p, 0, g);
+      const u16* own = P[n % NBUF];
+      const Frag<RP> p0 = along<SP>(own, p, 0, g), p1 = along<SP>(own, 16 + p, 0, g);
       y[0] = mul<CALC>(vf, p0, y[0]);
       y[1] = mul<CALC>(vf, p1, y[1]);
     }
+#endif
+    if ((n & 7) == 6) {
+      fill(o + 2, rg);
+      rg = gates(o + 10);
+    }
+    if constexpr (NBUF == 2 || !OUT) __syncthreads();        // (everybody is done with this block's tile)
+    put(stage[n % NBUF]);
 #if DOTS
     if (w == 3 && lane < L) {
-      const i64 t = block_of(o) * L + (back ? L - 1 - lane : lane);
+      const int t = block_of(o) * L + (back ? L - 1 - lane : lane);
       float s = of_state[0][lane] + of_state[1][lane] + (of_state[2][lane] + of_state[3][lane]);
-      if (job.pairs) s += (of_rows[0][lane] + of_rows[1][lane]) - (of_cols[0][lane] + of_cols[1][lane]);
+      if (job.pairs) s += (of_rows[n % NBUF][0][lane] + of_rows[n % NBUF][1][lane]) - (of_cols[n % NBUF][0][lane] + of_cols[n % NBUF][1][lane]);
       if (t < T) job.dots[((i64)tile * args.B * args.H + bh) * T + t] = s * out_scale;
     }
     if (o + 1 < nall) {
-      const i64 c = block_of(o);                 // (a border: in front of block c + 1, or backwards in front of block c)
-      if (!back && (c + 1) % args.span == 0 && c + 1 < nreal) mark((c + 1) / args.span - 1);
-      if (back && c % args.span == 0) mark(c / args.span - 1);
+      const int c = block_of(o);                 // (a border: in front of block c + 1, or backwards in front of block c)
+      if (!back && (c + 1) % span == 0 && c + 1 < nreal) mark((c + 1) / span - 1);
+      if (back && c % span == 0) mark(c / span - 1);
     }
 #endif
-#endif
-    if (NBUF == 1) __syncthreads();
-    if (o + 1 < last) put(stage[(o + 1) % NBUF]);
 #if OUT
     const Buffer into = buffer_at(to);
     to += to_step;
 #pragma unroll
     for (int it = 0; it < LT; it++) {
       const int i = back ? L - 1 - (16 * it + p) : 16 * it + p;
-      const i64 t0 = block_of(o) * L;
+      const int t0 = block_of(o) * L;
       const f4 z = t0 + i < len ? y[it] * out_scale : f4{0.f, 0.f, 0.f, 0.f};
       const u32 off = t0 + i < T ? to_off[it] : NOTHING;
-      if (wide) store_wide(into, off, z, C - cw - 4 * g, C % 4 == 0);
-      else store_in(into, off, z, C - cw - 4 * g, C % 4 == 0);
+      if (wide) store_wide(into, off, z, C - cw - 4 * g, whole);
+      else store_in(into, off, z, C - cw - 4 * g, whole);
     }
 #endif
     __syncthreads();
   }
 #if OUT
 #if DOTS
-  if (!back && first < last && last == nreal) mark((nreal - 1) / args.span);
+  if (!back && first < last && last == nreal) mark((nreal - 1) / span);
 #endif
-  for (i64 o = s0; o < s1; o++) {                // blocks without a token
+  for (int o = s0; o < s1; o++) {                // blocks without a token
     if (o >= first && o < last) continue;
     for (int u = tid; u < L * 16; u += 256) {
-      const i64 t = block_of(o) * L + u / 16;
+      const int t = block_of(o) * L + u / 16;
       const int col = c0 + u % 16 * 4;
       if (t < T)
         for (int r = 0; r < 4 && col + r < C; r++) store_type(job.out, out_at + t * job.ot + col + r, wide ? FP32 : IN, 0.f);
@@ -840,7 +891,9 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   const i64 at = bh * (args.nseg - 1) + seg;
   f4* to = (f4*)job.local + ((at * ntiles + tile) * 4 + w) * (NT * 64) + lane;
   for (int nt = 0; nt < NT; nt++) to[nt * 64] = S[nt];
-  if (tid == 192 && tile == 0) job.totals[at] = total;
+  if (lane == 0) totals[w] = total;
+  __syncthreads();
+  if (tid == 0 && tile == 0) job.totals[at] = totals[0] + totals[1] + (totals[2] + totals[3]);
 #endif
 }
 #endif

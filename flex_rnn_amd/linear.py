@@ -42,11 +42,11 @@ def _width(n: int) -> int:
     return next(w for w in WIDTHS if n <= w)
 
 
-def _block_defines(dtype, width, out=1, dots=0):
+def _block_defines(dtype, width, out=1, dots=0, fast=1, wide=0):
     w = _width(width)
-    nbuf = 2 if dtype == th.bfloat16 and w <= 128 and not dots else 1
+    nbuf = 2 if dtype == th.bfloat16 and w <= 128 else 1
     occ = 2
-    return (('KERNEL_BLOCK', 1), ('IN', DTYPES[dtype]), ('W', w), ('OUT', out), ('DOTS', dots), ('NBUF', nbuf), ('OCC', occ))
+    return (('KERNEL_BLOCK', 1), ('IN', DTYPES[dtype]), ('W', w), ('OUT', out), ('DOTS', dots), ('FAST', fast), ('WIDE', wide), ('NBUF', nbuf), ('OCC', occ))
 
 
 _GATE_DEFINES = (('KERNEL_GATE', 1), ('IN', 0))
@@ -62,7 +62,8 @@ def builds():
     for dt in DTYPES:
         out.append((SOURCE, 'la_step', _step_defines(dt)))
         for w in WIDTHS:
-            out += [(SOURCE, 'la_block', _block_defines(dt, w, o, d)) for o, d in ((1, 0), (1, 1), (0, 0))]
+            out += [(SOURCE, 'la_block', _block_defines(dt, w, *x)) for x in
+                    [(o, d, fast, 0) for o, d in ((1, 0), (1, 1), (0, 0)) for fast in (0, 1)] + [(1, d, 1, 1) for d in (0, 1) if dt != th.float32]]
     return out
 
 
@@ -115,6 +116,7 @@ def _segments(groups: int, blocks: int) -> Tuple[int, int]:
 # ------------------------------------------------------------------ launches
 _NO_TENSOR = (0, 0, 0, 0, 0, 1)
 _NO_JOB = bytes(_JOB.size)
+_OUT_TYPE = 6 * 6 + 6           # its field
 
 
 class _Role:
@@ -127,7 +129,8 @@ class _Role:
 def _job(q, k, v, x, width, C, init, fin, out, strides, out_type, back=0, pairs=0, in_scale=1.0, out_scale=1.0, dots=0, marks=0):
     """The fields of struct Job that are known before segments are; `local` and `totals` follow in `_walk`."""
     return [(*q.fields, *k.fields, *v.fields, *(_NO_TENSOR if x is None else x.fields), *init, *fin, out, *strides, out_type, dots, marks),
-            (q.heads, k.heads, v.heads, 1 if x is None else x.heads, width, C, back, pairs, in_scale, out_scale)]
+            (q.heads, k.heads, v.heads, 1 if x is None else x.heads, width, C, back, pairs, in_scale, out_scale),
+            C % 4 == 0 and all(r is None or r.fields[5] for r in (q, k, v, x))]
 
 
 def _walk(dev, dtype, jobs, gate, lengths, B, T, H, dots=0):
@@ -136,16 +139,18 @@ def _walk(dev, dtype, jobs, gate, lengths, B, T, H, dots=0):
     tiles = max(-(-j[1][5] // 64) for j in jobs)
     blocks = -(-T // BLOCK)
     nseg, per = _segments(len(jobs) * B * H * tiles, blocks)
+    fast = int(all(j[2] for j in jobs))
+    wide = int(fast and jobs[0][0][_OUT_TYPE] == 2 and dtype != th.float32)
     size = B * H * (nseg - 1)
     local = totals = None
     if nseg > 1:
         local = th.empty((len(jobs), size * tiles * 64 * width), dtype=th.float32, device=dev)
         totals = th.empty((len(jobs), size), dtype=th.float64, device=dev)
     blob = b''.join([_JOB.pack(*head, 0 if local is None else local[i].data_ptr(), 0 if totals is None else totals[i].data_ptr(), *tail)
-                     for i, (head, tail) in enumerate(jobs)] + [_NO_JOB] * (2 - len(jobs))
+                     for i, (head, tail, _) in enumerate(jobs)] + [_NO_JOB] * (2 - len(jobs))
                     + [_BLOCK.pack(*gate, _ptr(lengths), B, T, H, nseg, per, tiles, MARK_BLOCKS)])
     for out in ((0, 1) if nseg > 1 else (1,)):
-        k = hw.kernel(dev, SOURCE, 'la_block', _block_defines(dtype, width, out, dots if out else 0))
+        k = hw.kernel(dev, SOURCE, 'la_block', _block_defines(dtype, width, out, dots if out else 0, fast, wide if out else 0))
         groups = B * H * (nseg if out else nseg - 1)
         hw.launch_bytes(k, dev, -(-groups // 8) * 8 * tiles, len(jobs), 256, blob)
 
@@ -291,6 +296,7 @@ def _check(q, k, v, g, state, lead, what):
     require(q.shape == k.shape, f'{what}: q {list(q.shape)} and k {list(k.shape)} differ')
     require(q.shape[:n] == v.shape[:n], f'{what}: q {list(q.shape)} and v {list(v.shape)} differ in {names[1:-2]}')
     B, Hk, N = q.shape[0], q.shape[-2], q.shape[-1]
+    require(n == 1 or q.shape[1] < 2 ** 31 - 64, f'{what}: sequences of up to 2^31 - 65 tokens')
     H, M = v.shape[-2], v.shape[-1]
     require(Hk >= 1 and H >= 1 and H % Hk == 0, f'{what}: {H} heads of v do not divide into {Hk} heads of q and k')
     require(1 <= N <= MAX_HEAD and 1 <= M <= MAX_HEAD, f'{what}: head sizes from 1 to {MAX_HEAD} (q and k have {N}, v has {M})')
