@@ -15,7 +15,7 @@
 //
 // Sums over a row are fp32 and two passes over registers (mean first, then squares of what is left): no cancellation.
 //
-// Compiled by flex_rnn_amd/norm.py with IN (0 bfloat16, 1 float16, 2 float32), K, TH (threads), WIDE and BACKWARD.
+// Compiled by flex_rnn_amd/norm.py with IN (0 bfloat16, 1 float16, 2 float32), K, TH (threads), GL, WIDE and BACKWARD.
 #include <hip/hip_runtime.h>
 
 typedef unsigned int u32;
@@ -38,7 +38,7 @@ struct Args {
   char* y;                  // forward: y; backward: dx; [rows, C] without gaps
   const char *w, *b;        // [heads, C] or null
   float *dw, *db;           // backward: [teams / heads][heads][C] or null
-  i64 rows, heads, C, sx, hx, sy, hy, w_type, b_type, vec, gl, teams;
+  i64 rows, heads, C, sx, hx, sy, hy, w_type, b_type, vec, teams;
   double eps;
 };
 
@@ -97,12 +97,40 @@ DEV void store_piece(char* row, int n, int C, bool vec, const float* x) {
   }
 }
 
+template <int CTRL>
+DEV float dpp_add(float x) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+// Sums over the 2, 4, 8 and 16 neighbours of a lane (swaps within quads, then mirrors: no LDS), and over the lanes 16 and 32
+// further (row swaps), known to all of them.
+DEV float sum2(float x) { return dpp_add<0xb1>(x); }
+DEV float sum4(float x) { return dpp_add<0x4e>(sum2(x)); }
+DEV float sum8(float x) { return dpp_add<0x141>(sum4(x)); }
+DEV float sum16(float x) { return dpp_add<0x140>(sum8(x)); }
+DEV float sum_rows16(float x) {
+  const u32 u = __builtin_bit_cast(u32, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (u32)r[0]) + __builtin_bit_cast(float, (u32)r[1]);
+}
+DEV float sum_rows32(float x) {
+  const u32 u = __builtin_bit_cast(u32, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (u32)r[0]) + __builtin_bit_cast(float, (u32)r[1]);
+}
+DEV float sum_lanes(float x, int lanes) {      // over groups of 1 to 64 lanes, a power of two (the same in a whole wave)
+  if (lanes >= 2) x = sum2(x);
+  if (lanes >= 4) x = dpp_add<0x4e>(x);
+  if (lanes >= 8) x = dpp_add<0x141>(x);
+  if (lanes >= 16) x = dpp_add<0x140>(x);
+  if (lanes >= 32) x = sum_rows16(x);
+  if (lanes >= 64) x = sum_rows32(x);
+  return x;
+}
+
 // sums of two numbers over a team, known to all its lanes afterwards
 DEV f2 team_sum(f2 s, int gl, float (*lds)[2], int tid) {
-  for (int x = 1; x < gl; x <<= 1) {
-    s[0] += __shfl_xor(s[0], x, 64);
-    s[1] += __shfl_xor(s[1], x, 64);
-  }
+  s[0] = sum_lanes(s[0], gl);
+  s[1] = sum_lanes(s[1], gl);
 #if WIDE
   __syncthreads();
   if ((tid & 63) == 0) {
@@ -130,7 +158,7 @@ ln_fw(Args a) {
 #else
   float (*lds)[2] = nullptr;
 #endif
-  const int tid = threadIdx.x, gl = WIDE ? 64 : (int)a.gl;
+  const int tid = threadIdx.x, gl = WIDE ? 64 : GL;
   const int sub = WIDE ? tid : tid % gl, lanes = WIDE ? TH : gl;
   const i64 team = WIDE ? (i64)blockIdx.x : (i64)blockIdx.x * (TH / gl) + tid / gl;
   const int C = (int)a.C;

@@ -414,13 +414,35 @@ DEV i64 length_of(const i64* lengths, i64 b, i64 T) {
   return n < 0 ? 0 : n > T ? T : n;
 }
 
-DEV float sum16(float x) {                     // over the 16 lanes of a row
-  for (int m = 1; m < 16; m <<= 1) x += __shfl_xor(x, m, 64);
-  return x;
+template <int CTRL>
+DEV float dpp_add(float x) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
-DEV float sum_groups(float x) {                // over the 4 lanes with the same lane % 16
-  x += __shfl_xor(x, 16, 64);
-  return x + __shfl_xor(x, 32, 64);
+// Sums over the 2, 4, 8 and 16 neighbours of a lane (swaps within quads, then mirrors: no LDS), and over the lanes 16 and 32
+// further (row swaps), known to all of them.
+DEV float sum2(float x) { return dpp_add<0xb1>(x); }
+DEV float sum4(float x) { return dpp_add<0x4e>(sum2(x)); }
+DEV float sum8(float x) { return dpp_add<0x141>(sum4(x)); }
+DEV float sum16(float x) { return dpp_add<0x140>(sum8(x)); }
+DEV float sum_rows16(float x) {
+  const u32 u = __builtin_bit_cast(u32, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (u32)r[0]) + __builtin_bit_cast(float, (u32)r[1]);
+}
+DEV float sum_rows32(float x) {
+  const u32 u = __builtin_bit_cast(u32, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (u32)r[0]) + __builtin_bit_cast(float, (u32)r[1]);
+}
+DEV float sum_groups(float x) { return sum_rows32(sum_rows16(x)); }       // over the 4 lanes with the same lane % 16
+DEV float sum_lanes(float x, int lanes) {      // over groups of 1 to 64 lanes, a power of two (the same in a whole wave)
+  if (lanes >= 2) x = sum2(x);
+  if (lanes >= 4) x = dpp_add<0x4e>(x);
+  if (lanes >= 8) x = dpp_add<0x141>(x);
+  if (lanes >= 16) x = dpp_add<0x140>(x);
+  if (lanes >= 32) x = sum_rows16(x);
+  if (lanes >= 64) x = sum_rows32(x);
+  return x;
 }
 
 // Four neighbours of a block's result, the first n of them inside; in one piece where `whole` says that rows are a multiple
@@ -918,28 +940,29 @@ struct GateArgs {
   i64 B, T, H, tiles, span, size, type;
 };
 
-extern "C" __global__ void __launch_bounds__(256) la_gate(GateArgs a) {
-  __shared__ double part[4];
+extern "C" __global__ void __launch_bounds__(1024) la_gate(GateArgs a) {
+  __shared__ double part[16];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const i64 nall = (a.T + L - 1) / L, spans = (nall + a.span - 1) / a.span;
   const i64 bh = blockIdx.x / spans, s = blockIdx.x % spans, b = bh / a.H, h = bh % a.H, BH = a.B * a.H;
   const i64 len = length_of(a.lengths, b, a.T);
   const i64 t0 = s * a.span * L, t1 = t0 + a.span * L < a.T ? t0 + a.span * L : a.T, end = t1 < len ? t1 : len;
-  for (i64 t = end > t0 ? end + tid : t0 + tid; t < t1; t += 256) store_type(a.dg, (b * a.T + t) * a.H + h, (int)a.type, 0.f);
+  for (i64 t = end > t0 ? end + tid : t0 + tid; t < t1; t += 1024) store_type(a.dg, (b * a.T + t) * a.H + h, (int)a.type, 0.f);
   if (end <= t0) return;
   double x = 0.0;
   const f4 *ms = (const f4*)(a.marks_s + (bh * spans + s) * a.size), *mx = (const f4*)(a.marks_x + (bh * spans + s) * a.size);
-  for (i64 i = tid; i < a.size / 4; i += 256) {
+  for (i64 i = tid; i < a.size / 4; i += 1024) {
     const f4 u = ms[i], v = mx[i];
     x += (double)(u[0] * v[0] + u[1] * v[1]) + (double)(u[2] * v[2] + u[3] * v[3]);
   }
   x = read_lane(scan64(x), 63);
   if (lane == 0) part[w] = x;
   __syncthreads();
-  double carry = part[0] + part[1] + (part[2] + part[3]);
+  double carry = 0.0;
+  for (int i = 0; i < 16; i++) carry += part[i];
   if (end < len) carry *= exp(gate_of(a.g, b, h, end));      // (a mark inside the sequence lacks its own step's decay)
   __syncthreads();
-  for (i64 hi = end; hi > t0; hi -= 256) {                   // thread i has token hi - 1 - i
+  for (i64 hi = end; hi > t0; hi -= 1024) {                   // thread i has token hi - 1 - i
     const i64 t = hi - 1 - tid;
     double d = 0.0;
     if (t >= t0)
@@ -948,7 +971,7 @@ extern "C" __global__ void __launch_bounds__(256) la_gate(GateArgs a) {
     if (lane == 63) part[w] = d;
     __syncthreads();
     double before = carry;
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < 16; i++) {
       if (i < w) before += part[i];
       carry += part[i];
     }
@@ -960,8 +983,9 @@ extern "C" __global__ void __launch_bounds__(256) la_gate(GateArgs a) {
 
 // ================================================================== one token
 #ifdef KERNEL_STEP
-// S = exp(g) S + v k^T in place, y = scale S q.  Bound by reading and writing the state once.  A group of GL lanes owns a
-// row of the state, each lane VE neighbouring columns of it per turn (16 bytes where layout and type allow).
+// S = exp(g) S + v k^T in place, y = scale S q.  Bound by reading and writing the state once.  A group of `gl` lanes owns
+// rows of the state, a lane VE neighbouring columns (16 bytes) of each, whose q and k it holds; R rows are in flight at a
+// time.  States that do not allow 16-byte accesses go column by column.
 struct StepArgs {
   Tensor q, k, v;           // st unused
   Gate g;
@@ -972,74 +996,103 @@ struct StepArgs {
 };
 DEV float load_in(const char* p, i64 i) { return load_type(p, i, IN); }
 
-template <int TYPE, int VE>
-DEV void step_rows(const StepArgs& a, i64 b, i64 h, int r0, int tid) {
-  const int gl = (int)a.gl, sub = tid % gl, grp = tid / gl, groups = 256 / gl;
-  const i64 hk = h / (a.H / a.Hk);
-  const float e = expf((float)gate_of(a.g, b, h, 0)), scale = (float)a.scale;
-  const char* qp = a.q.p + (b * a.q.sb + hk * a.q.sh) * ESZ;
-  const char* kp = a.k.p + (b * a.k.sb + hk * a.k.sh) * ESZ;
-  const char* vp = a.v.p + (b * a.v.sb + h * a.v.sh) * ESZ;
-  constexpr int SZ = TYPE == FP32 ? 4 : 2;
-  const int M = (int)a.M, N = (int)a.N;
-  const int end = r0 + (int)a.rows < M ? r0 + (int)a.rows : M;
-  for (int m = r0 + grp; m < ((end - r0 + groups - 1) / groups) * groups + r0; m += groups) {
+template <int TYPE>
+DEV void unpack(const v4u t, float* s) {
+  if constexpr (TYPE == FP32) {
+    for (int i = 0; i < 4; i++) s[i] = as_f(t[i]);
+  } else {
+    for (int i = 0; i < 8; i++) {
+      const u16 x = (u16)(t[i / 2] >> (i % 2 * 16));
+      s[i] = TYPE == FP16 ? half_to_f(x) : as_f((u32)x << 16);
+    }
+  }
+}
+template <int TYPE>
+DEV v4u pack(const float* s) {
+  v4u t;
+  for (int i = 0; i < 4; i++) {
+    if constexpr (TYPE == FP32) t[i] = as_u(s[i]);
+    else if constexpr (TYPE == BF16) t[i] = pack_rne(s[2 * i], s[2 * i + 1]);
+    else t[i] = (u32)__builtin_bit_cast(u16, (_Float16)s[2 * i]) | (u32)__builtin_bit_cast(u16, (_Float16)s[2 * i + 1]) << 16;
+  }
+  return t;
+}
+
+struct Token {              // one head's operands
+  const char *q, *k, *v;
+  char *s, *y;
+  float e, scale;
+};
+
+template <int TYPE>
+DEV void step_rows(const StepArgs& a, const Token& t, int r0, int end, int tid) {
+  constexpr int VE = TYPE == FP32 ? 4 : 8, SZ = 16 / VE, R = 4;
+  const int gl = (int)a.gl, sub = tid % gl, grp = tid / gl, groups = 256 / gl, N = (int)a.N, n = sub * VE;
+  float q[VE], k[VE];
+  for (int i = 0; i < VE; i++) {
+    q[i] = n < N ? load_in(t.q, (n + i) * a.q.sn) * t.scale : 0.f;
+    k[i] = n < N ? load_in(t.k, (n + i) * a.k.sn) : 0.f;
+  }
+  char* at = t.s + (i64)n * SZ;
+  for (int m0 = r0; m0 < end; m0 += groups * R) {
+    v4u raw[R];
+    float v[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const int m = m0 + i * groups + grp;
+      const bool in = m < end && n < N;
+      raw[i] = in ? *(const v4u*)(at + m * a.s.sr * SZ) : v4u{0, 0, 0, 0};
+      v[i] = m < end ? load_in(t.v, m * a.v.sn) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const int m = m0 + i * groups + grp;
+      float s[VE], acc = 0.f;
+      unpack<TYPE>(raw[i], s);
+      for (int x = 0; x < VE; x++) {
+        s[x] = t.e * s[x] + v[i] * k[x];
+        acc += s[x] * q[x];
+      }
+      if (m < end && n < N) *(v4u*)(at + m * a.s.sr * SZ) = pack<TYPE>(s);
+      acc = sum_lanes(acc, gl);
+      if (m < end && sub == 0) store_type(t.y, m, IN, acc);
+    }
+  }
+}
+
+DEV void step_columns(const StepArgs& a, const Token& t, int r0, int end, int tid) {
+  const int gl = (int)a.gl, sub = tid % gl, grp = tid / gl, groups = 256 / gl, type = (int)a.s.type;
+  for (int m0 = r0; m0 < end; m0 += groups) {
+    const int m = m0 + grp;
     float acc = 0.f;
     if (m < end) {
-      const float v = load_in(vp, m * a.v.sn);
-      char* row = a.s.p + (b * a.s.sb + h * a.s.sh + m * a.s.sr) * SZ;
-      for (int n = sub * VE; n < N; n += gl * VE) {
-        float s[VE];
-        if constexpr (VE == 1) {
-          s[0] = load_type(row, n * a.s.sc, TYPE);
-        } else if constexpr (TYPE == FP32) {
-          const f4 t = *(const f4*)(row + n * 4);
-          for (int i = 0; i < 4; i++) s[i] = t[i];
-        } else {
-          const v4u t = *(const v4u*)(row + n * 2);
-          for (int i = 0; i < VE; i++) {
-            const u16 x = (u16)(t[i / 2] >> (i % 2 * 16));
-            s[i] = TYPE == FP16 ? half_to_f(x) : as_f((u32)x << 16);
-          }
-        }
-        for (int i = 0; i < VE; i++) {
-          s[i] = e * s[i] + v * load_in(kp, (n + i) * a.k.sn);
-          acc += s[i] * load_in(qp, (n + i) * a.q.sn);
-        }
-        if constexpr (VE == 1) {
-          store_type(row, n * a.s.sc, TYPE, s[0]);
-        } else if constexpr (TYPE == FP32) {
-          *(f4*)(row + n * 4) = f4{s[0], s[1], s[2], s[3]};
-        } else {
-          v4u t;
-          for (int i = 0; i < VE / 2; i++) {
-            if constexpr (TYPE == BF16) t[i] = pack_rne(s[2 * i], s[2 * i + 1]);
-            else t[i] = (u32)__builtin_bit_cast(u16, (_Float16)s[2 * i]) | (u32)__builtin_bit_cast(u16, (_Float16)s[2 * i + 1]) << 16;
-          }
-          *(v4u*)(row + n * 2) = t;
-        }
+      const float v = load_in(t.v, m * a.v.sn);
+      for (int n = sub; n < a.N; n += gl) {
+        const i64 i = m * a.s.sr + n * a.s.sc;
+        const float s = t.e * load_type(t.s, i, type) + v * load_in(t.k, n * a.k.sn);
+        acc += s * load_in(t.q, n * a.q.sn) * t.scale;
+        store_type(t.s, i, type, s);
       }
     }
-    for (int x = 1; x < gl; x <<= 1) acc += __shfl_xor(acc, x, 64);
-    if (m < end && sub == 0) store_type(a.y, (b * a.H + h) * M + m, IN, acc * scale);
+    acc = sum_lanes(acc, gl);
+    if (m < end && sub == 0) store_type(t.y, m, IN, acc);
   }
 }
 
 extern "C" __global__ void __launch_bounds__(256) la_step(StepArgs a) {
-  const i64 per = (a.M + a.rows - 1) / a.rows;
-  const i64 bh = blockIdx.x / per;
-  const int r0 = (int)(blockIdx.x % per * a.rows);
-  const i64 b = bh / a.H, h = bh % a.H;
-  const int tid = threadIdx.x;
-  if (a.s.type == FP32) {
-    if (a.vec) step_rows<FP32, 4>(a, b, h, r0, tid);
-    else step_rows<FP32, 1>(a, b, h, r0, tid);
-  } else if (a.s.type == BF16) {
-    if (a.vec) step_rows<BF16, 8>(a, b, h, r0, tid);
-    else step_rows<BF16, 1>(a, b, h, r0, tid);
-  } else {
-    if (a.vec) step_rows<FP16, 8>(a, b, h, r0, tid);
-    else step_rows<FP16, 1>(a, b, h, r0, tid);
-  }
+  const i64 per = (a.M + a.rows - 1) / a.rows, bh = blockIdx.x / per, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
+  const int r0 = (int)(blockIdx.x % per * a.rows), end = r0 + (int)a.rows < a.M ? r0 + (int)a.rows : (int)a.M, tid = threadIdx.x;
+  Token t;
+  t.q = a.q.p + (b * a.q.sb + hk * a.q.sh) * ESZ;
+  t.k = a.k.p + (b * a.k.sb + hk * a.k.sh) * ESZ;
+  t.v = a.v.p + (b * a.v.sb + h * a.v.sh) * ESZ;
+  t.s = a.s.p + (b * a.s.sb + h * a.s.sh) * (a.s.type == FP32 ? 4 : 2);
+  t.y = a.y + bh * a.M * ESZ;
+  t.e = expf((float)gate_of(a.g, b, h, 0));
+  t.scale = (float)a.scale;
+  if (!a.vec) step_columns(a, t, r0, end, tid);
+  else if (a.s.type == FP32) step_rows<FP32>(a, t, r0, end, tid);
+  else if (a.s.type == BF16) step_rows<BF16>(a, t, r0, end, tid);
+  else step_rows<FP16>(a, t, r0, end, tid);
 }
 #endif

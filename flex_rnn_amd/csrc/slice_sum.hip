@@ -7,13 +7,17 @@
 typedef long long i64;
 
 struct Args {
-  const float* in;
-  char* out;
+  struct {
+    const float* in;
+    char* out;
+  } pair[2];                       // blockIdx.y chooses
   i64 S, X, type, cw, parts;       // type: 0 bfloat16, 1 float16, 2 float32; cw: a power of two from 1 to 256
 };
 
 extern "C" __global__ void __launch_bounds__(256) slice_sum(Args a) {
   __shared__ double part[256];
+  const float* in = a.pair[blockIdx.y].in;
+  char* out = a.pair[blockIdx.y].out;
   const int tid = threadIdx.x, cw = (int)a.cw, col = tid % cw, row = tid / cw, nr = 256 / cw;
   const i64 groups = (a.X + cw - 1) / cw, x = (i64)(blockIdx.x % groups) * cw + col, pt = blockIdx.x / groups;
   const i64 per = (a.S + a.parts - 1) / a.parts, s0 = pt * per, s1 = s0 + per < a.S ? s0 + per : a.S;
@@ -21,10 +25,10 @@ extern "C" __global__ void __launch_bounds__(256) slice_sum(Args a) {
   if (x < a.X) {
     i64 i = s0 + row;
     for (; i + 3 * nr < s1; i += 4 * nr) {
-      const float v0 = a.in[i * a.X + x], v1 = a.in[(i + nr) * a.X + x], v2 = a.in[(i + 2 * nr) * a.X + x], v3 = a.in[(i + 3 * nr) * a.X + x];
+      const float v0 = in[i * a.X + x], v1 = in[(i + nr) * a.X + x], v2 = in[(i + 2 * nr) * a.X + x], v3 = in[(i + 3 * nr) * a.X + x];
       s += (double)v0 + (double)v1 + ((double)v2 + (double)v3);
     }
-    for (; i < s1; i += nr) s += (double)a.in[i * a.X + x];
+    for (; i < s1; i += nr) s += (double)in[i * a.X + x];
   }
   part[tid] = s;
   __syncthreads();
@@ -35,8 +39,8 @@ extern "C" __global__ void __launch_bounds__(256) slice_sum(Args a) {
   if (row == 0 && x < a.X) {
     const float v = (float)part[col];
     const i64 at = pt * a.X + x;
-    if (a.type == 2) ((float*)a.out)[at] = v;
-    else if (a.type == 1) ((_Float16*)a.out)[at] = (_Float16)v;
-    else ((__bf16*)a.out)[at] = (__bf16)v;
+    if (a.type == 2) ((float*)out)[at] = v;
+    else if (a.type == 1) ((_Float16*)out)[at] = (_Float16)v;
+    else ((__bf16*)out)[at] = (__bf16)v;
   }
 }

@@ -1,7 +1,7 @@
 """Hand-written kernels (flex_rnn_amd/csrc/*.hip): compiled per set of preprocessor constants into the same on-disk cache as
 the generated ones, loaded once per device, launched through the same C-ABI runtime on the current stream.
 
-`kernel()` finds or builds one; `launch()` packs the argument block and launches; `slice_sum()` is the reduction over
+`kernel()` finds or builds one; `launch()` packs the argument block and launches; `slice_sums()` is the reduction over
 leading slices that the backward passes of `linear.py` and `norm.py` share.
 """
 from __future__ import annotations
@@ -82,21 +82,31 @@ def launch_bytes(k: runtime.Kernel, device: th.device, grid: int, grid_y: int, t
         k.launch((grid, grid_y, 1), (threads, 1, 1), block, stream=th.cuda.current_stream(device).cuda_stream)
 
 
-def slice_sum(x: th.Tensor, slices: int, out: th.Tensor):
-    """out[...] = the sum of `slices` leading fp32 slices of `x`, in `out`'s type."""
-    X = out.numel()
-    if X == 0:
+def slice_sums(pairs, slices: int):
+    """For one or two `(x, out)` of one size and type: out[...] = the sum of `slices` leading fp32 slices of `x`."""
+    out = pairs[0][1] if pairs else None
+    if not pairs or out.numel() == 0:
         return
-    k = kernel(x.device, 'slice_sum.hip', 'slice_sum')
-    # columns side by side while there are enough of them to fill a row of threads; else the threads share the slices
+    X, dev = out.numel(), out.device
+    k = kernel(dev, 'slice_sum.hip', 'slice_sum')
+    # as many columns side by side as leave 256 workgroups (up to a 256-byte row of them); the other threads share the slices
     cw = 1
-    while cw < 64 and cw < X:
+    while cw < 64 and cw < X and X // (2 * cw) * len(pairs) >= 256:
         cw *= 2
     groups = -(-X // cw)
-    # many slices over few columns: parts of at least 64 trips per thread row, joined by a second launch
-    parts = max(1, min(512 // groups, slices // (64 * (256 // cw))))
+    # many slices over few columns: parts of at least 16 trips per thread, joined by a second launch
+    parts = max(1, min(512 // (groups * len(pairs)), slices // (16 * (256 // cw))))
+    ins, outs = [x for x, _ in pairs], [o for _, o in pairs]
+
+    def run(ins, outs, slices, type_, parts):
+        ptrs = [t.data_ptr() for t in (ins[0], outs[0], ins[-1], outs[-1])]
+        launch_bytes(k, dev, groups * parts, len(pairs), 256, _SUM.pack(*ptrs, slices, X, type_, cw, parts))
+
     if parts > 1:
-        part = th.empty((parts, X), dtype=th.float32, device=x.device)
-        launch(k, x.device, groups * parts, 256, '7q', x.data_ptr(), part.data_ptr(), slices, X, 2, cw, parts)
-        x, slices = part, parts
-    launch(k, x.device, groups, 256, '7q', x.data_ptr(), out.data_ptr(), slices, X, DTYPES[out.dtype], cw, 1)
+        part = th.empty((len(pairs), parts, X), dtype=th.float32, device=dev)
+        run(ins, list(part), slices, 2, parts)
+        ins, slices = list(part), parts
+    run(ins, outs, slices, DTYPES[out.dtype], 1)
+
+
+_SUM = struct.Struct('<9q')

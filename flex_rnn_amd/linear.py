@@ -194,18 +194,17 @@ def _backward(q, k, v, g, state, lengths, dy, dstate, scale, need_g, need_state)
     _walk(dev, dt, [_job(rk, rq, ry, None, N, M, _states(dstate), none, dv.data_ptr(), (T * H * M, H * M, M, 0, 1), DTYPES[dt], back=1, in_scale=scale)],
           gate, lengths, B, T, H)
     if share > 1:
-        hw.slice_sum(pq, share, dq)
-        hw.slice_sum(pk, share, dk)
+        hw.slice_sums([(pq, dq), (pk, dk)], share)
     dg = None
     if need_g:
         per_head = g.ndim == 1
         dg = th.empty(g.shape, dtype=g.dtype, device=dev)
         out = th.empty((B, T, H), dtype=th.float32, device=dev) if per_head else dg
-        hw.launch(hw.kernel(dev, SOURCE, 'la_gate', _GATE_DEFINES), dev, B * H * spans, 256, _GATE,
+        hw.launch(hw.kernel(dev, SOURCE, 'la_gate', _GATE_DEFINES), dev, B * H * spans, 1024, _GATE,
                   dots[0].data_ptr(), dots[1].data_ptr(), marks[0].data_ptr(), marks[1].data_ptr(), *gate, out.data_ptr(), _ptr(lengths),
                   B, T, H, tiles, MARK_BLOCKS, size, DTYPES[out.dtype])
         if per_head:
-            hw.slice_sum(out, B * T, dg)
+            hw.slice_sums([(out, dg)], B * T)
     return dq, dk, dv, dg, ds
 
 

@@ -19,23 +19,26 @@ SOURCE = 'layer_norm.hip'
 MAX_COLUMNS = 16384
 TEAMS = 256 * 8 * 256           # threads in flight: eight workgroups of 256 per compute unit
 
-_ARGS = '3q2q2q12qd'
+_ARGS = '3q2q2q11qd'
 
 
 def _shape_rule(C: int, dtype: th.dtype):
-    """(WIDE, threads, 16-byte pieces per lane): a row stays in the registers of up to 64 lanes with four pieces each; wider
-    rows take a workgroup of 256, then 1024 threads."""
+    """(WIDE, threads, 16-byte pieces per lane, lanes per row): a row stays in the registers of up to 64 lanes with four
+    pieces each; wider rows take a workgroup of 256, then 1024 threads."""
     pieces = -(-C * (4 if dtype == th.float32 else 2) // 16)
     for k in (1, 2, 4):
         if pieces <= 64 * k:
-            return 0, 256, k
+            lanes = 1
+            while lanes * k < pieces:
+                lanes *= 2
+            return 0, 256, k, lanes
     k = 4 if dtype == th.float32 else 2
-    return (1, 256, k) if pieces <= 256 * k else (1, 1024, k)
+    return (1, 256, k, 256) if pieces <= 256 * k else (1, 1024, k, 1024)
 
 
 def _defines(C, dtype, backward):
-    wide, threads, k = _shape_rule(C, dtype)
-    return (('IN', DTYPES[dtype]), ('K', k), ('TH', threads), ('WIDE', wide), ('BACKWARD', int(backward)))
+    wide, threads, k, lanes = _shape_rule(C, dtype)
+    return (('IN', DTYPES[dtype]), ('K', k), ('TH', threads), ('GL', lanes), ('WIDE', wide), ('BACKWARD', int(backward)))
 
 
 def builds():
@@ -68,24 +71,19 @@ def _wide(x, C, *strides):
 def _launch(name, x, dy, out, weight, bias, dw, db, heads, teams, eps, lanes, strides):
     C = x.shape[-1]
     defines = _defines(C, x.dtype, name == 'ln_bw')
-    threads, wide = defines[2][1], defines[3][1]
+    threads, wide = defines[2][1], defines[4][1]
     vec = _wide(x, C, *strides[:2]) and (dy is None or _wide(dy, C, *strides[2:]))
     grid = teams if wide else -(-teams * lanes // threads)
     ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     code = lambda t: 2 if t is None else DTYPES[t.dtype]  # noqa: E731
     hw.launch(hw.kernel(x.device, SOURCE, name, defines), x.device, grid, threads, _ARGS, x.data_ptr(), ptr(dy), out.data_ptr(), ptr(weight), ptr(bias),
-              ptr(dw), ptr(db), x.numel() // C, heads, C, *strides, code(weight), code(bias), int(vec), lanes, teams, eps)
+              ptr(dw), ptr(db), x.numel() // C, heads, C, *strides, code(weight), code(bias), int(vec), teams, eps)
 
 
 def _teams(x, heads, dtype, most):
     """(teams, lanes per team): as many rows side by side as fit the chip, a multiple of `heads` (a team keeps its head)."""
     C = x.shape[-1]
-    wide, threads, k = _shape_rule(C, dtype)
-    lanes = threads
-    if not wide:
-        pieces, lanes = -(-C * x.element_size() // 16), 1
-        while lanes * k < pieces:
-            lanes *= 2
+    lanes = _shape_rule(C, dtype)[3]
     outers = x.numel() // C // heads
     return min(outers, max(1, most // (lanes * heads))) * heads, lanes
 
@@ -126,10 +124,7 @@ def _backward(x, weight, bias, dy, eps, need_w, need_b):
     pw = th.empty((teams, C), dtype=th.float32, device=x.device) if need_w else None
     pb = th.empty((teams, C), dtype=th.float32, device=x.device) if need_b else None
     _launch('ln_bw', x, dy, dx, weight, None, pw, pb, heads, teams, eps, lanes, (so, sh, yo, yh))
-    if need_w:
-        hw.slice_sum(pw, teams // heads, dw)
-    if need_b:
-        hw.slice_sum(pb, teams // heads, db)
+    hw.slice_sums([(p, d) for p, d in ((pw, dw), (pb, db)) if p is not None], teams // heads)
     return dx, dw, db
 
 
