@@ -4,6 +4,7 @@ the pure-PyTorch loop or benchmarked.
 
     python -m flex_rnn_amd.examples --op rwkv7 --check-flex
     python -m flex_rnn_amd.examples --op mamba2 --benchmark-flex [--forward] [--torch-compile]
+    python -m flex_rnn_amd.examples --op retention --chunked --head-norm --check-flex
 
 Counterpart of /root/reference/tests/examples.py (ops 37-426, modes 433-466).  The comparisons
 with third-party kernels (fla, mamba_ssm, ...) are not available here; `--check-flex` compares
@@ -20,6 +21,11 @@ from flex_rnn_amd import ops
 OPS = ['rwkv7', 'rwkv6', 'gla', 'retention', 'delta_rule', 'gated_delta_rule', 'mamba2', 'longhorn', 'rwkv4',
        'hgrn', 'mamba', 's4d', 'gsa', 'mlstm']
 
+
+# recurrences whose decay is one number per head and token: `flex_rnn_amd.linear_attention` computes them in blocks
+CHUNKED_OPS = ['retention', 'mamba2']
+# layers whose first result is [B,T,H,C]: a norm of each head's output may follow
+HEAD_OPS = ['rwkv7', 'rwkv6', 'gla', 'retention', 'delta_rule', 'gated_delta_rule', 'mamba2', 'gsa']
 
 RAW_OPS = ['rwkv7', 'gla', 'delta_rule', 'gated_delta_rule', 'mamba2', 'mamba', 'hgrn']
 
@@ -266,6 +272,35 @@ def build(op, B, T, D, C, device, raw=False):
     return inputs, layer, steps
 
 
+def chunked(op, layer_inputs):
+    """The layer of `build(op, ...)` (not `raw`) as blocks of matrix products instead of a compiled step."""
+    assert op in CHUNKED_OPS, f'no chunked form of {op}'
+    if op == 'retention':
+        H = layer_inputs[0].shape[2]
+        log_decay = (1 - 2 ** (-5 - th.arange(H).float())).log().to(layer_inputs[0].device)
+
+        def layer(q, k, v, s):
+            y, s = flex_rnn_amd.linear_attention(q, k, v, log_decay, s.mT)
+            return y, s.mT
+    else:
+        def layer(x, dt, A, b, c, s):
+            return flex_rnn_amd.linear_attention(c, b, dt.unsqueeze(-1) * x, dt * A, s)
+    return layer
+
+
+def head_norm(op, layer, H, C, device, norm=None):
+    """(weight, bias, the layer with its first result normed per head; its arguments are weight, bias, then the layer's)."""
+    assert op in HEAD_OPS, f'the result of {op} is not [B,T,H,C]'
+    norm = norm or flex_rnn_amd.layer_norm
+    g = th.Generator().manual_seed(1)
+    weight, bias = [(o + 0.2 * th.randn(H, C, generator=g)).to(device) for o in (1.0, 0.0)]
+
+    def normed(weight, bias, *args):
+        y, *rest = layer(*args)
+        return (norm(y, weight, bias), *rest)
+    return weight, bias, normed
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument('--batchsz', type=int, default=8)
@@ -280,7 +315,13 @@ def main(argv=None):
     ap.add_argument('--raw', action='store_true', help='the layer takes raw projections and prepares them itself (ops: ' + ', '.join(RAW_OPS) + ')')
     ap.add_argument('--fuse', action='store_true', help='run the layer through flex_rnn_amd.layer (input preparation moves into the step)')
     ap.add_argument('--fuse-reductions', action='store_true', help='with --fuse: also move sums and norms along the column axis')
+    ap.add_argument('--chunked', action='store_true', help='blocks of matrix products instead of a compiled step (ops: ' + ', '.join(CHUNKED_OPS) + ')')
+    ap.add_argument('--head-norm', action='store_true', help='follow the layer with a layer norm of each head (ops: ' + ', '.join(HEAD_OPS) + ')')
     a = ap.parse_args(argv)
+    if a.chunked and (a.raw or a.fuse or a.op not in CHUNKED_OPS):
+        ap.error('--chunked goes with --op ' + ' or '.join(CHUNKED_OPS) + ', without --raw and --fuse')
+    if a.head_norm and a.op not in HEAD_OPS:
+        ap.error('--head-norm goes with --op ' + ', '.join(HEAD_OPS))
     check = a.check_flex or not a.benchmark_flex
     D = a.modeldim or (256 if check else 4096)
     T = a.seqlen or (256 if check else 1024)
@@ -289,6 +330,12 @@ def main(argv=None):
     eager_layer = layer
     if a.fuse:
         layer = flex_rnn_amd.layer(layer, reductions=a.fuse_reductions)
+    if a.chunked:
+        layer = chunked(a.op, inputs)
+    if a.head_norm:
+        w, b, layer = head_norm(a.op, layer, D // a.headsz, a.headsz, 'cuda')
+        eager_layer = head_norm(a.op, eager_layer, D // a.headsz, a.headsz, 'cuda', flex_rnn_amd.layer_norm.naive_fp64)[2]
+        inputs = (w, b, *inputs)
     if not check:
         if a.op not in ('s4d', 'mamba'):
             inputs = tuple(i.to(th.bfloat16) for i in inputs)

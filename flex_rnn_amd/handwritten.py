@@ -6,7 +6,6 @@ leading slices that the backward passes of `linear.py` and `norm.py` share.
 """
 from __future__ import annotations
 
-import contextlib
 import os
 import struct
 import threading
@@ -62,6 +61,22 @@ def kernel(device: th.device, source: str, name: str, defines: Tuple[Tuple[str, 
     return k
 
 
+class Once(th.autograd.Function):
+    """Calls `op(*args)`, the gradient of an operator; a gradient of that is refused (it would silently miss terms)."""
+
+    @staticmethod
+    def forward(ctx, op, *args):
+        return op(*args)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise AssertionError('linear_attention and layer_norm can be differentiated once')
+
+
+def once(op, *args):
+    return Once.apply(op, *args) if th.is_grad_enabled() else op(*args)
+
+
 _packers: Dict[str, struct.Struct] = {}
 
 
@@ -77,9 +92,18 @@ def launch_bytes(k: runtime.Kernel, device: th.device, grid: int, grid_y: int, t
     """The same with a packed argument block."""
     if grid <= 0:
         return
-    require(grid * threads < 2 ** 32, f'{k.name}: a launch of {grid} workgroups is more than the hardware takes; split the batch')
-    with (th.cuda.device(device) if th.cuda.current_device() != device.index else contextlib.nullcontext()):
-        k.launch((grid, grid_y, 1), (threads, 1, 1), block, stream=th.cuda.current_stream(device).cuda_stream)
+    if grid * threads >= 2 ** 32:
+        require(False, f'{k.name}: a launch of {grid} workgroups is more than the hardware takes; split the batch')
+    index = device.index
+    if th.cuda.current_device() != index:
+        with th.cuda.device(device):
+            k.launch((grid, grid_y, 1), (threads, 1, 1), block, stream=_raw_stream(index))
+    else:
+        k.launch((grid, grid_y, 1), (threads, 1, 1), block, stream=_raw_stream(index))
+
+
+def _raw_stream(index: int) -> int:
+    return th._C._cuda_getCurrentRawStream(index)
 
 
 def slice_sums(pairs, slices: int):

@@ -25,6 +25,7 @@ from .handwritten import DTYPES, require
 
 SOURCE = 'linear_attention.hip'
 MAX_HEAD = 256                  # largest M and N
+MAX_TOKENS = 2 ** 31 - 65       # longest sequence (positions are 32 bits, rounded up to blocks)
 WIDTHS = (64, 128, 256)         # what M and N are padded to
 BLOCK = 32                      # tokens per block
 WORKGROUPS = 512                # two per compute unit: below this a sequence is split into segments
@@ -68,12 +69,15 @@ def builds():
 
 
 # ------------------------------------------------------------------ argument blocks
-def _tensor(t: th.Tensor, batch: int, time: Optional[int], head: int):
-    sb, sh, sn = t.stride(batch), t.stride(head), t.stride(-1)
-    st = 0 if time is None else t.stride(time)
-    size = t.element_size()
-    wide = sn == 1 and t.shape[-1] % 8 == 0 and t.data_ptr() % 16 == 0 and sb * size % 16 == 0 and st * size % 16 == 0 and sh * size % 16 == 0
-    return t.data_ptr(), sb, st, sh, sn, int(wide)
+def _tensor(t: th.Tensor, time: bool):
+    """Fields of struct Tensor for [batch, (time,) heads, width]."""
+    at, size = t.data_ptr(), t.element_size()
+    if time:
+        sb, st, sh, sn = t.stride()
+    else:
+        (sb, sh, sn), st = t.stride(), 0
+    wide = sn == 1 and t.shape[-1] % 8 == 0 and (at | sb * size | st * size | sh * size) % 16 == 0
+    return at, sb, st, sh, sn, int(wide)
 
 
 def _near(t: th.Tensor) -> th.Tensor:
@@ -123,7 +127,7 @@ class _Role:
     """One operand of a walk: its tensor, argument fields and heads."""
 
     def __init__(self, t: th.Tensor):
-        self.fields, self.heads = _tensor(t, 0, 1, 2), t.shape[2]
+        self.fields, self.heads = _tensor(t, True), t.shape[2]
 
 
 def _job(q, k, v, x, width, C, init, fin, out, strides, out_type, back=0, pairs=0, in_scale=1.0, out_scale=1.0, dots=0, marks=0):
@@ -131,6 +135,16 @@ def _job(q, k, v, x, width, C, init, fin, out, strides, out_type, back=0, pairs=
     return [(*q.fields, *k.fields, *v.fields, *(_NO_TENSOR if x is None else x.fields), *init, *fin, out, *strides, out_type, dots, marks),
             (q.heads, k.heads, v.heads, 1 if x is None else x.heads, width, C, back, pairs, in_scale, out_scale),
             C % 4 == 0 and all(r is None or r.fields[5] for r in (q, k, v, x))]
+
+
+_block_kernels = {}
+
+
+def _block_kernel(dev, *key):
+    k = _block_kernels.get((dev.index, key))
+    if k is None:
+        k = _block_kernels[dev.index, key] = hw.kernel(dev, SOURCE, 'la_block', _block_defines(*key))
+    return k
 
 
 def _walk(dev, dtype, jobs, gate, lengths, B, T, H, dots=0):
@@ -150,7 +164,7 @@ def _walk(dev, dtype, jobs, gate, lengths, B, T, H, dots=0):
                      for i, (head, tail, _) in enumerate(jobs)] + [_NO_JOB] * (2 - len(jobs))
                     + [_BLOCK.pack(*gate, _ptr(lengths), B, T, H, nseg, per, tiles, MARK_BLOCKS)])
     for out in ((0, 1) if nseg > 1 else (1,)):
-        k = hw.kernel(dev, SOURCE, 'la_block', _block_defines(dtype, width, out, dots if out else 0, fast, wide if out else 0))
+        k = _block_kernel(dev, dtype, width, out, dots if out else 0, fast, wide if out else 0)
         groups = B * H * (nseg if out else nseg - 1)
         hw.launch_bytes(k, dev, -(-groups // 8) * 8 * tiles, len(jobs), 256, blob)
 
@@ -221,7 +235,7 @@ def _step(q, k, v, g, state, scale):
         lanes *= 2
     rows = min(M, 256 // lanes * 4)
     hw.launch(hw.kernel(dev, SOURCE, 'la_step', _step_defines(q.dtype)), dev, B * H * -(-M // rows), 256, _STEP,
-              *_tensor(q, 0, None, 1), *_tensor(k, 0, None, 1), *_tensor(v, 0, None, 1), *_gate(g), *_states_t(state), y.data_ptr(),
+              *_tensor(q, False), *_tensor(k, False), *_tensor(v, False), *_gate(g), *_states_t(state), y.data_ptr(),
               B, H, Hk, M, N, int(wide), lanes, rows, scale)
     return y
 
@@ -275,7 +289,6 @@ class _LinearAttention(th.autograd.Function):
         return _fw_op(q, k, v, g, state, lengths, scale)
 
     @staticmethod
-    @th.autograd.function.once_differentiable
     def backward(ctx, dy, dstate):
         q, k, v, g, state, lengths = ctx.saved_tensors
         if dy is None and dstate is None:
@@ -283,36 +296,41 @@ class _LinearAttention(th.autograd.Function):
         if dy is None:
             dy = th.zeros_like(v)
         need = ctx.needs_input_grad
-        dq, dk, dv, dg, ds = _bw_op(q, k, v, g, state, lengths, dy, dstate, ctx.scale, need[3], need[4])
+        dq, dk, dv, dg, ds = hw.once(_bw_op, q, k, v, g, state, lengths, dy, dstate, ctx.scale, need[3], need[4])
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dg if need[3] else None, ds if need[4] else None, None, None
 
 
-def _check(q, k, v, g, state, lead, what):
+def _check(q, k, v, g, state, lead, what, types=True):
     """Argument checks shared by the prompt and the single-token form; `lead`: the dimensions in front of the heads."""
-    n = len(lead)
-    names = '[' + ', '.join(lead) + (', ' if lead else '')
+    n, sq, sv, dt = len(lead), q.shape, v.shape, q.dtype
+    if len(sq) == len(sv) == n + 2 and sq == k.shape and sq[:n] == sv[:n] and sq[n] >= 1 and sv[n] >= 1 and sv[n] % sq[n] == 0 \
+            and 1 <= sq[-1] <= MAX_HEAD and 1 <= sv[-1] <= MAX_HEAD and (n == 1 or sq[1] <= MAX_TOKENS) \
+            and dt in DTYPES and k.dtype == dt and v.dtype == dt and g.dtype in (dt, th.float32) and g.shape in (sv[n:n + 1], sv[:n + 1]) \
+            and (state is None or (state.shape == (sq[0], sv[n], sv[-1], sq[-1]) and state.dtype in (dt, th.float32))):
+        return
+    names = '[' + ', '.join(lead) + ', '
     require(q.ndim == n + 2 and k.ndim == n + 2 and v.ndim == n + 2, f'{what}: q and k are {names}Hk, N] and v is {names}H, M]')
     require(q.shape == k.shape, f'{what}: q {list(q.shape)} and k {list(k.shape)} differ')
     require(q.shape[:n] == v.shape[:n], f'{what}: q {list(q.shape)} and v {list(v.shape)} differ in {names[1:-2]}')
     B, Hk, N = q.shape[0], q.shape[-2], q.shape[-1]
-    require(n == 1 or q.shape[1] < 2 ** 31 - 64, f'{what}: sequences of up to 2^31 - 65 tokens')
     H, M = v.shape[-2], v.shape[-1]
     require(Hk >= 1 and H >= 1 and H % Hk == 0, f'{what}: {H} heads of v do not divide into {Hk} heads of q and k')
     require(1 <= N <= MAX_HEAD and 1 <= M <= MAX_HEAD, f'{what}: head sizes from 1 to {MAX_HEAD} (q and k have {N}, v has {M})')
-    require(q.dtype in DTYPES and q.dtype == k.dtype == v.dtype, f'{what}: q, k and v are of one type, bfloat16, float16 or float32 '
-            f'(got {q.dtype}, {k.dtype}, {v.dtype})')
-    require(g.dtype in (q.dtype, th.float32), f'{what}: g is float32 or of the type of q (got {g.dtype})')
+    require(n == 1 or q.shape[1] <= MAX_TOKENS, f'{what}: sequences of up to {MAX_TOKENS} tokens')
+    require(not types or dt in DTYPES and dt == k.dtype == v.dtype, f'{what}: q, k and v are of one type, bfloat16, float16 or float32 (got {dt}, {k.dtype}, {v.dtype})')
+    require(not types or g.dtype in (dt, th.float32), f'{what}: g is float32 or of the type of q (got {g.dtype})')
     require(tuple(g.shape) in ((H,), (*v.shape[:n], H)), f'{what}: g is [H] or {names}H] with H = {H} (got {list(g.shape)})')
-    if state is not None:
-        require(tuple(state.shape) == (B, H, M, N), f'{what}: the state is [B, H, M, N] = {[B, H, M, N]} (got {list(state.shape)})')
-        require(state.dtype in (q.dtype, th.float32), f'{what}: the state is float32 or of the type of q (got {state.dtype})')
+    require(state is None or tuple(state.shape) == (B, H, M, N), f'{what}: the state is [B, H, M, N] = {[B, H, M, N]} (got {list(state.shape) if state is not None else None})')
+    require(state is None or not types or state.dtype in (dt, th.float32), f'{what}: the state is float32 or of the type of q (got {state.dtype if state is not None else None})')
 
 
-def _check_device(tensors, what):
-    dev = tensors[0].device
-    require(dev.type in ('cuda', 'meta'), f'{what} runs on the GPU only (got a {dev} tensor); `.naive` is the plain PyTorch loop')
-    for t in tensors[1:]:
-        require(t is None or t.device == dev, f'{what}: all tensors must live on the same device ({t.device if t is not None else ""} and {dev})')
+def _check_device(what, first, *others):
+    dev = first.device
+    if dev.type not in ('cuda', 'meta'):
+        require(False, f'{what} runs on the GPU only (got a {dev} tensor); `.naive` is the plain PyTorch loop')
+    for t in others:
+        if t is not None and t.device != dev:
+            require(False, f'{what}: all tensors must live on the same device ({t.device} and {dev})')
 
 
 def linear_attention(q: th.Tensor, k: th.Tensor, v: th.Tensor, g: th.Tensor, state: Optional[th.Tensor] = None, *,
@@ -329,7 +347,7 @@ def linear_attention(q: th.Tensor, k: th.Tensor, v: th.Tensor, g: th.Tensor, sta
     Any strides.  Sums and the state are fp32.  Differentiable once in q, k, v, g and state; gradients are deterministic.
     """
     _check(q, k, v, g, state, ('B', 'T'), 'linear_attention')
-    _check_device((q, k, v, g, state, lengths), 'linear_attention')
+    _check_device('linear_attention', q, k, v, g, state, lengths)
     if lengths is not None:
         require(tuple(lengths.shape) == (q.shape[0],) and lengths.dtype in (th.int64, th.int32),
                 f'linear_attention: lengths is int64 or int32 [B] = [{q.shape[0]}] (got {lengths.dtype} {list(lengths.shape)})')
@@ -346,17 +364,16 @@ def linear_attention_step(q: th.Tensor, k: th.Tensor, v: th.Tensor, g: th.Tensor
     share memory.  Not differentiable: with T = 1, `linear_attention` is.
     """
     _check(q, k, v, g, state, ('B',), 'linear_attention_step')
-    _check_device((q, k, v, g, state), 'linear_attention_step')
-    require(not th.is_grad_enabled() or not any(t.requires_grad for t in (q, k, v, g, state)),
-            'linear_attention_step updates the state in place and cannot be differentiated: use linear_attention, or th.no_grad()')
-    require(not _overlaps(state), 'linear_attention_step: elements of the state share memory')
+    _check_device('linear_attention_step', q, k, v, g, state)
+    if th.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or state.requires_grad):
+        require(False, 'linear_attention_step updates the state in place and cannot be differentiated: use linear_attention, or th.no_grad()')
+    if not state.is_contiguous():
+        require(not _overlaps(state), 'linear_attention_step: elements of the state share memory')
     return _step_op(q, k, v, g, state, float(scale))
 
 
 def _overlaps(t: th.Tensor) -> bool:
     """Whether two indices of `t` may name the same element (the dimensions do not nest)."""
-    if t.is_contiguous():
-        return False
     end = 0
     for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
         if stride <= end:
@@ -366,8 +383,8 @@ def _overlaps(t: th.Tensor) -> bool:
 
 
 def _naive(q, k, v, g, state=None, *, lengths=None, scale=1.0, dtype=th.float32):
-    """The same operator as a loop over tokens in plain PyTorch (any device, differentiable), computed in `dtype`."""
-    _check(q, k, v, g, state, ('B', 'T'), 'linear_attention')
+    """The same operator as a loop over tokens in plain PyTorch (any device and type, differentiable), computed in `dtype`."""
+    _check(q, k, v, g, state, ('B', 'T'), 'linear_attention', types=False)
     B, T, Hk, N = q.shape
     H, M = v.shape[2:]
     s_dtype = th.float32 if state is None else state.dtype

@@ -17,7 +17,7 @@ from .handwritten import DTYPES, require
 
 SOURCE = 'layer_norm.hip'
 MAX_COLUMNS = 16384
-TEAMS = 256 * 8 * 256           # threads in flight: eight workgroups of 256 per compute unit
+THREADS = 256 * 2 * 256         # in flight: two workgroups of 256 per compute unit (measured from one half to sixteen: 5.0 TB/s at two, 3.9 at eight)
 
 _ARGS = '3q2q2q11qd'
 
@@ -80,12 +80,12 @@ def _launch(name, x, dy, out, weight, bias, dw, db, heads, teams, eps, lanes, st
               ptr(dw), ptr(db), x.numel() // C, heads, C, *strides, code(weight), code(bias), int(vec), teams, eps)
 
 
-def _teams(x, heads, dtype, most):
-    """(teams, lanes per team): as many rows side by side as fit the chip, a multiple of `heads` (a team keeps its head)."""
+def _teams(x, heads):
+    """(teams, lanes per team): as many rows side by side as keep the chip busy, a multiple of `heads` (a team keeps its head)."""
     C = x.shape[-1]
-    lanes = _shape_rule(C, dtype)[3]
+    lanes = _shape_rule(C, x.dtype)[3]
     outers = x.numel() // C // heads
-    return min(outers, max(1, most // (lanes * heads))) * heads, lanes
+    return min(outers, max(1, THREADS // (lanes * heads))) * heads, lanes
 
 
 def _per_head(x, weight, bias):
@@ -100,7 +100,7 @@ def _forward(x, weight, bias, eps):
     per_head = _per_head(x, weight, bias)
     heads = x.shape[-2] if per_head else 1
     x, so, sh = _rows(x, per_head)
-    teams, lanes = _teams(x, heads, x.dtype, TEAMS)
+    teams, lanes = _teams(x, heads)
     _launch('ln_fw', x, None, y, weight, bias, None, None, heads, teams, eps, lanes, (so, sh, 0, 0))
     return y
 
@@ -119,8 +119,7 @@ def _backward(x, weight, bias, dy, eps, need_w, need_b):
     heads = x.shape[-2] if per_head else 1
     x, so, sh = _rows(x, per_head)
     dy, yo, yh = _rows(dy, per_head)
-    # a team's share of dw and db is written once: a quarter of the forward pass' teams keeps that small beside the rows
-    teams, lanes = _teams(x, heads, x.dtype, TEAMS // 4)
+    teams, lanes = _teams(x, heads)
     pw = th.empty((teams, C), dtype=th.float32, device=x.device) if need_w else None
     pb = th.empty((teams, C), dtype=th.float32, device=x.device) if need_b else None
     _launch('ln_bw', x, dy, dx, weight, None, pw, pb, heads, teams, eps, lanes, (so, sh, yo, yh))
@@ -163,12 +162,32 @@ class _LayerNorm(th.autograd.Function):
         return _fw_op(x, weight, bias, eps)
 
     @staticmethod
-    @th.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, bias = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dw, db = _bw_op(x, weight, bias, dy, ctx.eps, need[1], need[2])
+        dx, dw, db = hw.once(_bw_op, x, weight, bias, dy, ctx.eps, need[1], need[2])
         return dx if need[0] else None, dw if need[1] else None, db if need[2] else None, None
+
+
+def _check(x, weight, bias):
+    C = x.shape[-1] if x.ndim else 0
+    fits = lambda p: p is None or ((p.shape == (C,) or p.shape == x.shape[-2:]) and p.dtype in (x.dtype, th.float32) and p.device == x.device)  # noqa: E731
+    if 1 <= C <= MAX_COLUMNS and x.dtype in DTYPES and x.device.type in _DEVICES and fits(weight) and fits(bias) \
+            and (weight is None or bias is None or weight.shape == bias.shape):
+        return
+    what = 'layer_norm'
+    require(x.ndim >= 1 and x.dtype in DTYPES, f'{what}: x is bfloat16, float16 or float32 with at least one dimension (got {x.dtype} {list(x.shape)})')
+    require(1 <= C <= MAX_COLUMNS, f'{what}: rows of 1 to {MAX_COLUMNS} columns (got {C})')
+    for name, p in (('weight', weight), ('bias', bias)):
+        if p is not None:
+            require(p.shape == (C,) or p.shape == x.shape[-2:], f'{what}: {name} is [C] = [{C}] or [H, C] of x {list(x.shape)} (got {list(p.shape)})')
+            require(p.dtype in (x.dtype, th.float32), f'{what}: {name} is float32 or of the type of x (got {p.dtype})')
+            require(p.device == x.device, f'{what}: all tensors must live on the same device ({p.device} and {x.device})')
+    require(weight is None or bias is None or weight.shape == bias.shape, f'{what}: weight and bias have the same shape')
+    require(False, f'{what} runs on the GPU only (got a {x.device} tensor); `.naive` is plain PyTorch')
+
+
+_DEVICES = ('cuda', 'meta')
 
 
 def layer_norm(x: th.Tensor, weight: Optional[th.Tensor] = None, bias: Optional[th.Tensor] = None, eps: float = 1e-5) -> th.Tensor:
@@ -181,18 +200,7 @@ def layer_norm(x: th.Tensor, weight: Optional[th.Tensor] = None, bias: Optional[
     Sums are fp32 (mean first, then squares of the differences).  Differentiable once in x, weight and bias; gradients are
     deterministic.
     """
-    what = 'layer_norm'
-    require(x.ndim >= 1 and x.dtype in DTYPES, f'{what}: x is bfloat16, float16 or float32 with at least one dimension (got {x.dtype} {list(x.shape)})')
-    C = x.shape[-1]
-    require(1 <= C <= MAX_COLUMNS, f'{what}: rows of 1 to {MAX_COLUMNS} columns (got {C})')
-    for name, p in (('weight', weight), ('bias', bias)):
-        if p is not None:
-            require(tuple(p.shape) == (C,) or (x.ndim >= 2 and tuple(p.shape) == tuple(x.shape[-2:])),
-                    f'{what}: {name} is [C] = [{C}] or [H, C] of x {list(x.shape)} (got {list(p.shape)})')
-            require(p.dtype in (x.dtype, th.float32), f'{what}: {name} is float32 or of the type of x (got {p.dtype})')
-            require(p.device == x.device, f'{what}: all tensors must live on the same device ({p.device} and {x.device})')
-    require(weight is None or bias is None or weight.shape == bias.shape, f'{what}: weight and bias have the same shape')
-    require(x.device.type in ('cuda', 'meta'), f'{what} runs on the GPU only (got a {x.device} tensor); `.naive` is plain PyTorch')
+    _check(x, weight, bias)
     weight, bias = (p if p is None or p.is_contiguous() else p.contiguous() for p in (weight, bias))
     if th.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNorm.apply(x, weight, bias, float(eps))

@@ -234,8 +234,9 @@ class Kernel:
     def launch(self, grid: Sequence[int], block: Sequence[int], args: bytes, stream: int = 0, lds_bytes: int = 0):
         g = _U3(*grid)
         b = _U3(*block)
-        _check(lib().frnn_launch(self.handle, g, b, lds_bytes, ctypes.c_void_p(stream), args, len(args)),
-               f'launching kernel {self.name}')
+        rc = lib().frnn_launch(self.handle, g, b, lds_bytes, stream, args, len(args))
+        if rc:
+            _check(rc, f'launching kernel {self.name}')
 
 
     def launch_static(self, grid: Sequence[int], block: Sequence[int], args: bytes, slots, stream: int = 0, lds_bytes: int = 0):

@@ -1,0 +1,196 @@
+"""Linear attention and layer norm without a GPU: refusals, the plain loop that the GPU tests compare with (against
+`jit.naive` of the recurrences that it covers, and against differences), metadata, host-side planning."""
+import pytest
+import torch as th
+
+import flex_rnn_amd as F
+from flex_rnn_amd import examples, handwritten, linear, norm, ops, prebuild
+
+import linear_cases as lc
+
+
+def _meta(*shape, dtype=th.bfloat16):
+    return th.empty(shape, dtype=dtype, device='meta')
+
+
+def test_public_names():
+    import flex_rnn
+    for name in ('linear_attention', 'linear_attention_step', 'layer_norm'):
+        assert getattr(flex_rnn, name) is getattr(F, name)
+
+
+BAD = [
+    (dict(q=(2, 8, 4)), r'q and k are \[B, T, Hk, N\]'),
+    (dict(k=(2, 8, 2, 16)), 'q .* and k .* differ'),
+    (dict(v=(2, 9, 4, 16)), r'q .* and v .* differ in B, T'),
+    (dict(v=(2, 8, 6, 16)), '6 heads of v do not divide into 4 heads'),
+    (dict(v=(2, 8, 4, 257)), 'head sizes from 1 to 256'),
+    (dict(q=(2, 8, 4, 0), k=(2, 8, 4, 0)), 'head sizes from 1 to 256'),
+    (dict(v_dtype=th.float32), 'q, k and v are of one type'),
+    (dict(dtype=th.float64, v_dtype=th.float64), 'q, k and v are of one type'),
+    (dict(g=(2, 8, 3)), r'g is \[H\] or \[B, T, H\] with H = 4'),
+    (dict(g=(2,)), r'g is \[H\]'),
+    (dict(g_dtype=th.float16), 'g is float32 or of the type of q'),
+    (dict(state=(2, 4, 16, 17)), r'the state is \[B, H, M, N\]'),
+    (dict(state_dtype=th.float16), 'the state is float32 or of the type of q'),
+    (dict(lengths=(3,)), r'lengths is int64 or int32 \[B\] = \[2\]'),
+    (dict(lengths_dtype=th.float32), 'lengths is int64 or int32'),
+]
+
+
+@pytest.mark.parametrize('change,message', BAD)
+def test_linear_attention_refuses(change, message):
+    c = dict(q=(2, 8, 4, 16), k=(2, 8, 4, 16), v=(2, 8, 4, 16), g=(2, 8, 4), state=(2, 4, 16, 16), lengths=(2,), dtype=th.bfloat16,
+             g_dtype=th.float32, state_dtype=th.float32, lengths_dtype=th.int64)
+    c.update(change)
+    c.setdefault('v_dtype', c['dtype'])
+    args = [_meta(*c['q'], dtype=c['dtype']), _meta(*c['k'], dtype=c['dtype']), _meta(*c['v'], dtype=c['v_dtype']), _meta(*c['g'], dtype=c['g_dtype']),
+            _meta(*c['state'], dtype=c['state_dtype'])]
+    with pytest.raises(AssertionError, match=message):
+        F.linear_attention(*args, lengths=_meta(*c['lengths'], dtype=c['lengths_dtype']))
+
+
+def test_gpu_only_and_one_device():
+    q = th.zeros(1, 4, 2, 8)
+    with pytest.raises(AssertionError, match='runs on the GPU only'):
+        F.linear_attention(q, q, q, th.zeros(2))
+    with pytest.raises(AssertionError, match='runs on the GPU only'):
+        F.layer_norm(q)
+    with pytest.raises(AssertionError, match='runs on the GPU only'):
+        F.linear_attention_step(q[:, 0], q[:, 0], q[:, 0], th.zeros(2), th.zeros(1, 2, 8, 8))
+    m = _meta(1, 4, 2, 8, dtype=th.float32)
+    with pytest.raises(AssertionError, match='the same device'):
+        F.linear_attention(m, m, m, th.zeros(2))
+    with pytest.raises(AssertionError, match='the same device'):
+        F.layer_norm(m, th.zeros(8))
+
+
+def test_step_refuses():
+    m, s = _meta(2, 4, 16), _meta(2, 4, 16, 16, dtype=th.float32)
+    g = _meta(2, 4, dtype=th.float32)
+    assert F.linear_attention_step(m, m, m, g, s).shape == (2, 4, 16)
+    with pytest.raises(AssertionError, match='elements of the state share memory'):
+        F.linear_attention_step(m, m, m, g, s[:1].expand(2, 4, 16, 16))
+    with pytest.raises(AssertionError, match='cannot be differentiated'):
+        F.linear_attention_step(m, m, m, g, s.clone().requires_grad_())
+    with th.no_grad():
+        F.linear_attention_step(m, m, m, g, s.clone().requires_grad_())
+    with pytest.raises(AssertionError, match=r'g is \[H\] or \[B, H\]'):
+        F.linear_attention_step(m, m, m, _meta(2, 3, dtype=th.float32), s)
+
+
+def test_overlap_rule():
+    x = th.zeros(4, 6, 8, 10)
+    assert not linear._overlaps(x) and not linear._overlaps(x.mT) and not linear._overlaps(x[:, ::2, 1:5]) and not linear._overlaps(x.permute(2, 0, 3, 1))
+    assert linear._overlaps(x[:1].expand(4, 6, 8, 10)) and linear._overlaps(th.zeros(64).as_strided((1, 1, 8, 8), (64, 64, 4, 1)))
+
+
+@pytest.mark.parametrize('kwargs,message', [
+    (dict(x=(3, 16), weight=(15,)), r'weight is \[C\] = \[16\]'),
+    (dict(x=(3, 16), weight=(2, 16)), r'weight is \[C\]'),
+    (dict(x=(3, 2, 16), weight=(2, 16), bias=(16,)), 'the same shape'),
+    (dict(x=(3, 16), weight=(16,), weight_dtype=th.float16), 'float32 or of the type of x'),
+    (dict(x=(3, 16385)), 'rows of 1 to 16384 columns'),
+    (dict(x=(3, 0)), 'rows of 1 to 16384 columns'),
+    (dict(x=()), 'at least one dimension'),
+    (dict(x=(3, 16), x_dtype=th.float64), 'x is bfloat16, float16 or float32'),
+])
+def test_layer_norm_refuses(kwargs, message):
+    make = lambda n, dt: None if n not in kwargs else _meta(*kwargs[n], dtype=dt)  # noqa: E731
+    with pytest.raises(AssertionError, match=message):
+        F.layer_norm(make('x', kwargs.get('x_dtype', th.bfloat16)), make('weight', kwargs.get('weight_dtype', th.bfloat16)), make('bias', th.bfloat16))
+
+
+def test_metadata_and_autograd_on_meta():
+    q, v = _meta(2, 8, 2, 16).requires_grad_(), _meta(2, 8, 4, 32).requires_grad_()
+    g, s = _meta(4, dtype=th.float32).requires_grad_(), _meta(2, 4, 32, 16).requires_grad_()
+    y, sT = F.linear_attention(q, q, v, g, s)
+    assert y.shape == v.shape and y.dtype == v.dtype and sT.shape == s.shape and sT.dtype == s.dtype
+    grads = th.autograd.grad((y, sT), (q, v, g, s), (y, sT))
+    assert [x.shape for x in grads] == [x.shape for x in (q, v, g, s)] and [x.dtype for x in grads] == [x.dtype for x in (q, v, g, s)]
+    assert F.linear_attention(q, q, v, g)[1].dtype == th.float32
+    w = _meta(4, 32, dtype=th.float32).requires_grad_()
+    z = F.layer_norm(v, w, w)
+    dv, dw = th.autograd.grad(z, (v, w), z)
+    assert z.shape == v.shape and dv.shape == v.shape and dw.shape == w.shape and dw.dtype == th.float32
+
+
+def test_plain_loop_is_the_recurrence_of_retention_and_mamba2():
+    B, T, H, C = 2, 5, 3, 4
+    gen = th.Generator().manual_seed(0)
+    randn = lambda *s: th.randn(*s, generator=gen, dtype=th.float64)  # noqa: E731
+    inputs, layer, steps = examples.build('mamba2', B, T, H * C, C, 'cpu')
+    steps['step'].apply = steps['step'].naive_fp64
+    want = layer(*inputs)
+    x, dt, A, b, c, s = inputs
+    got = F.linear_attention.naive_fp64(c, b, dt.unsqueeze(-1) * x, dt * A, s)
+    for u, v in zip(got, want):
+        assert th.allclose(u.double(), v.double(), rtol=1e-5, atol=1e-5)        # (both are rounded to float32 once)
+    q, k, v, w = randn(B, T, H, C), randn(B, T, H, C), randn(B, T, H, C), th.rand(B, T, H, generator=gen, dtype=th.float64)
+    s = randn(B, H, C, C)
+    ret = F.jit(ops.retention)
+    want = ret.naive_fp64(w[..., None, None], q.unsqueeze(-2), k.unsqueeze(-2), v.unsqueeze(-1), s)
+    got = F.linear_attention.naive_fp64(q, k, v, w.log(), s)
+    for u, x in zip(got, want):
+        assert th.allclose(u, x, rtol=1e-12, atol=1e-12)
+
+
+def test_plain_loop_lengths_and_gradients():
+    inputs, lens = lc.make(th.float32, 3, 6, 4, 2, 5, 3, lengths=(0, 4, 9), resets=0.2)
+    xs = [x.double() for x in inputs]
+    y, s = F.linear_attention.naive(*xs, lengths=lens, scale=0.5, dtype=th.float64)
+    assert bool((y[0] == 0).all()) and th.equal(s[0], xs[4][0]) and bool((y[1, 4:] == 0).all())
+    cut = [xs[0][1:2, :4], xs[1][1:2, :4], xs[2][1:2, :4], xs[3][1:2, :4], xs[4][1:2]]
+    y1, s1 = F.linear_attention.naive(*cut, scale=0.5, dtype=th.float64)
+    assert th.equal(y[1, :4], y1[0]) and th.equal(s[1], s1[0])
+    # gradients of the loop against differences
+    xs[3] = xs[3].clamp(min=-3)
+    f = lambda *a: F.linear_attention.naive(*a, lengths=lens, scale=0.5, dtype=th.float64)  # noqa: E731
+    assert th.autograd.gradcheck(f, [x.requires_grad_() for x in xs], eps=1e-6, atol=1e-6)
+    x, w, b = th.randn(3, 2, 5, dtype=th.float64), th.randn(2, 5, dtype=th.float64), th.randn(2, 5, dtype=th.float64)
+    assert th.autograd.gradcheck(lambda *a: F.layer_norm.naive(*a, dtype=th.float64), [t.requires_grad_() for t in (x, w, b)], eps=1e-6, atol=1e-6)
+
+
+def test_segments_cover_the_blocks():
+    for groups in (1, 2, 7, 64, 511, 512, 5000):
+        for blocks in (0, 1, 7, 16, 17, 35, 1024, 4097):
+            nseg, per = linear._segments(groups, blocks)
+            assert nseg >= 1 and nseg * per >= blocks and nseg <= linear.MAX_SEGMENTS
+            assert nseg == 1 or (nseg - 1) * per < blocks          # no segment without a block
+            assert groups < linear.WORKGROUPS or nseg == 1
+
+
+def test_teams_keep_their_head():
+    for shape, heads in (((8192, 32, 128), 32), ((1, 5, 64), 5), ((37, 1000), 1), ((3, 64, 4096), 64), ((70000, 8), 1), ((2, 300, 512), 300)):
+        for dt in (th.bfloat16, th.float32):
+            x = _meta(*shape, dtype=dt)
+            teams, lanes = norm._teams(x, heads)
+            assert teams % heads == 0 and heads <= teams <= x.numel() // shape[-1]
+            wide, threads, k, gl = norm._shape_rule(shape[-1], dt)
+            assert lanes == gl and gl * k * 16 >= shape[-1] * x.element_size() and (gl <= 64 or wide)
+
+
+def test_rows_fold_or_are_copied():
+    x = th.zeros(4, 6, 3, 8)
+    for view, heads, copied in ((x, False, False), (x, True, False), (x.transpose(0, 1), False, True), (x[:, :, :, ::2], False, True),
+                                (x[:, :3], False, True), (x[:, :, 1:], True, False), (x[:2].transpose(1, 2), True, True), (x[..., 2:6], True, False)):
+        got, so, sh = norm._rows(view, heads)
+        assert th.equal(got, view) and (got.data_ptr() == view.data_ptr()) != copied
+        lead = got.shape[:-2] if heads else got.shape[:-1]
+        flat = got.as_strided((lead.numel(), got.shape[-2] if heads else 1, got.shape[-1]), (so, sh, 1))
+        assert th.equal(flat.reshape(-1), view.reshape(-1))
+
+
+def test_every_code_object_of_the_rules_is_prebuilt(runtime_lib, monkeypatch):
+    built = set(linear.builds()) | set(norm.builds())
+    for dt in handwritten.DTYPES:
+        for n in (1, 16, 64, 65, 128, 129, 256):
+            for out, dots in ((1, 0), (1, 1), (0, 0)):
+                for fast in (0, 1):
+                    assert (linear.SOURCE, 'la_block', linear._block_defines(dt, n, out, dots, fast, 0)) in built
+        for C in (1, 5, 64, 100, 513, 600, 1000, 2047, 2049, 3000, 5000, 16384):
+            for name, back in (('ln_fw', False), ('ln_bw', True)):
+                assert (norm.SOURCE, name, norm._defines(C, dt, back)) in built
+    seen = []
+    monkeypatch.setattr(handwritten, 'build', lambda *c, force=False: seen.append(c))
+    assert prebuild.warm_handwritten() == len(seen) == len(built) + 1
