@@ -347,6 +347,22 @@ DEV double scan64(double x) {                  // over all of them
   x = scan32(x);
   return x + dpp_or_zero<0x143, 0xc>(x);       // lane 31 into the upper half
 }
+DEV double row_of_16(double x) {               // over 16 lanes, in the last of them
+  x += dpp_or_zero<0x111, 0xf>(x);
+  x += dpp_or_zero<0x112, 0xf>(x);
+  x += dpp_or_zero<0x114, 0xf>(x);
+  return x + dpp_or_zero<0x118, 0xf>(x);
+}
+template <class SWAP>
+DEV double add_swapped(double x, SWAP swap) {
+  const u64 b = __builtin_bit_cast(u64, x);
+  const auto lo = swap((u32)b), hi = swap((u32)(b >> 32));
+  return __builtin_bit_cast(double, (u64)(u32)hi[0] << 32 | (u32)lo[0]) + __builtin_bit_cast(double, (u64)(u32)hi[1] << 32 | (u32)lo[1]);
+}
+DEV double over_rows(double x) {               // over the 4 lanes with the same lane % 16
+  x = add_swapped(x, [](u32 u) { return __builtin_amdgcn_permlane16_swap(u, u, false, false); });
+  return add_swapped(x, [](u32 u) { return __builtin_amdgcn_permlane32_swap(u, u, false, false); });
+}
 DEV double read_lane(double x, int lane) {
   const u64 b = __builtin_bit_cast(u64, x);
   const u32 lo = __builtin_amdgcn_readlane((int)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
@@ -377,25 +393,18 @@ struct Decays {
   alignas(16) float to_end[L];                 // exp(G_L - G_i), times the scale of what enters the state
 };
 
-DEV float exp2_sum(float hi, float lo) {       // 2^(hi + lo), |lo| far below 1
-  const float e = __builtin_amdgcn_exp2f(hi);
-  return e + e * (lo * 0.693147181f);
-}
-
 // one wave prepares two blocks: lane i of either half holds token i's g (0 behind the last token); returns the sum of g
 DEV double fill_decays(Decays* first, Decays* second, double g, float in_scale, int lane) {
   const double G = scan32(g);
   const double end0 = read_lane(G, 31), end1 = read_lane(G, 63);
-  const double G2 = G * LOG2E, E2 = (lane < L ? end0 : end1) * LOG2E;
+  const double G2 = G * LOG2E;
+  const float hi = (float)G2;
   Decays* d = lane < L ? first : second;
   const int i = lane & (L - 1);
-  const float hi = (float)G2, lo = (float)(G2 - (double)hi);
-  const double to = E2 - G2;
   d->hi[i] = hi;
-  d->lo[i] = lo;
-  d->from_start[i] = exp2_sum(hi, lo);
-  const float th = (float)to;
-  d->to_end[i] = exp2_sum(th, (float)(to - (double)th)) * in_scale;
+  d->lo[i] = (float)(G2 - (double)hi);
+  d->from_start[i] = (float)exp(G);
+  d->to_end[i] = (float)exp((lane < L ? end0 : end1) - G) * in_scale;
   return end0 + end1;
 }
 
@@ -466,6 +475,16 @@ DEV void store_in(Buffer to, u32 off, f4 x, int n, bool whole) {
   }
 }
 
+// Borders: in front of every BORDER-th block, where the last block begins (the gradient that comes in behind a sequence may be
+// far larger than what is left of it a block earlier) and behind it.
+constexpr int BORDER = 8;
+DEV i64 borders_of(int nall) { return (nall + BORDER - 1) / BORDER + 2; }
+DEV bool is_border(int c, int nreal) { return c % BORDER == 0 || c + 1 >= nreal; }
+DEV i64 border_at(int c, int nreal, int nall) {
+  const int n = (nall + BORDER - 1) / BORDER;
+  return c == nreal ? n : c + 1 == nreal ? n + 1 : c / BORDER;
+}
+
 // ================================================================== the walk over a sequence's blocks
 #ifdef KERNEL_BLOCK
 // One workgroup walks the blocks of one (batch, head, segment) for 64 of v's columns; wave w owns 16 of them: its share of
@@ -476,15 +495,17 @@ DEV void store_in(Buffer to, u32 off, f4 x, int n, bool whole) {
 //
 // With DOTS the walk also leaves, per token, what the gradient of g is made of (see la_gate): forwards (dq) the products
 // q_i.dq_i with the block's own share taken from unrounded numbers, less the share of each j; backwards (dk) the products
-// k_j.dk_j of the state's share.  x is the operand of these products (q, k), in the 64 columns that the workgroup owns;
-// sums over column tiles are left to la_gate.  At every MARK-th block's border the state is written down too.
+// k_j.dk_j of the state's share.  x is the operand of these products (q, k), in the 64 columns that the workgroup owns.  At
+// borders between blocks the backward walk writes its state down, and the forward walk, which runs after it, multiplies its own
+// with that.  Sums over column tiles are left to la_gate.  These sums are 64 bits: they are added up over many tokens.
 struct Job {
   Tensor q, k, v, x;
   States init, fin;
   char* out;                // element (b, t, h, column): b * ob + t * ot + h / share * og + h % share * os + column
   i64 ob, ot, og, os, share, out_type;
-  float* dots;              // [column tiles][B*H][T]
-  float* marks;             // [B*H][spans][ceil(C/16)][W/16][64][4]
+  float* dots;              // [column tiles][B*H][T], or null: this job only goes along with one that has them
+  float* marks;             // [B*H][borders][ceil(C/16)][W/16][64][4]: written backwards, read forwards
+  double* inner;            // [B*H][borders][column tiles][4]: written forwards
   float* local;             // [B*H][nseg-1][column tiles][4][W/16][64][4]: states that segments leave behind, from zero
   double* totals;           // [B*H][nseg-1]: their sums of g
   i64 Hq, Hk, Hv, Hx;       // heads of the operands
@@ -495,13 +516,14 @@ struct BlockArgs {
   Job job[2];
   Gate g;
   const i64* lengths;
-  i64 B, T, H, nseg, per, tiles, span;    // per: blocks per segment; tiles: most column tiles of a job; span: blocks per mark
+  i64 B, T, H, nseg, per, tiles;          // per: blocks per segment; tiles: most column tiles of a job
 };
 
 constexpr int NT = W / 16, LT = 2;
 constexpr int SPARTS = DOTS ? 3 : RP, SLIM = DOTS ? 2 : CALC;
 constexpr int QB = RP == 1 ? (W < 128 ? W / 32 : 4) : RP == 2 ? 2 : 1;       // operands read ahead: what 32 registers hold
 constexpr int KB = RP == 1 ? 4 : RP == 2 ? 2 : 2;
+constexpr bool EARLY = RP == 1 && W <= 128;                                  // registers for what dots need, ahead of its use
 constexpr bool AHEAD = OUT && RP == 1 && SPARTS == 1 && W <= 128;            // the state as a factor: what 16 registers hold
 constexpr int SQ = stride_along(W), SK = stride_down(W), SV = stride_down(64), SX = stride_along(64), SP = stride_along(L);
 constexpr int AT_K = OUT ? RP * L * SQ : 0, AT_V = AT_K + RP * L * SK, AT_X = AT_V + RP * L * SV, STAGE = AT_X + (DOTS ? RP * L * SX : 0);
@@ -543,7 +565,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   __shared__ double totals[4];
 #endif
 #if DOTS
-  __shared__ float of_rows[NBUF][LT][L], of_cols[NBUF][LT][L], of_state[4][L];
+  __shared__ double of_rows[NBUF][LT][L], of_cols[NBUF][LT][L], of_state[4][L];
 #endif
   const Job& job = args.job[blockIdx.y];
   const int tid = threadIdx.x, lane = tid & 63, p = lane & 15, g = lane >> 4;
@@ -585,12 +607,36 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   for (int i = tid; i < NBUF * RP * L * SP / 8; i += 256) *(v4u*)(&P[0][0] + 8 * i) = v4u{0, 0, 0, 0};     // (stays zero above the diagonal)
 #endif
 #if DOTS
-  if (tid < NBUF * LT * L) (&of_rows[0][0][0])[tid] = (&of_cols[0][0][0])[tid] = 0.f;
-  const int span = (int)args.span, spans = (nall + span - 1) / span;
-  const auto mark = [&](int at) {
-    if (cw >= C) return;
-    f4* to = (f4*)job.marks + ((bh * spans + at) * ((C + 15) / 16) + cw / 16) * (NT * 64) + lane;
-    for (int nt = 0; nt < NT; nt++) to[nt * 64] = S[nt];
+  if (tid < NBUF * LT * L) (&of_rows[0][0][0])[tid] = (&of_cols[0][0][0])[tid] = 0.0;
+  // the border in front of block c (behind the last one: c = nreal), of those that count
+  const i64 borders = borders_of(nall);
+  const auto counts = [&](int c) { return job.dots && c > 0 && c <= nreal && is_border(c, nreal); };
+  const auto mark_of = [&](int c) {
+    return (f4*)job.marks + ((bh * borders + border_at(c, nreal, nall)) * ((C + 15) / 16) + cw / 16) * (NT * 64) + lane;
+  };
+  f4 mark[NT];              // the backward walk's at this block's end, on its way while the block is worked on
+  const auto mark_down = [&](int c) {
+    if (!counts(c) || cw >= C) return;
+    f4* at = mark_of(c);
+    for (int nt = 0; nt < NT; nt++) at[nt * 64] = S[nt];
+  };
+  const auto mark_ahead = [&](int c) {
+    if (!counts(c) || cw >= C) return;
+    const f4* at = mark_of(c);
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) mark[nt] = at[nt * 64];
+  };
+  const auto mark_product = [&](int c) {
+    if (!counts(c)) return;
+    if (!EARLY) mark_ahead(c);
+    double s = 0.0;
+    if (cw < C) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+        s += (double)(mark[nt][0] * S[nt][0] + mark[nt][1] * S[nt][1]) + (double)(mark[nt][2] * S[nt][2] + mark[nt][3] * S[nt][3]);
+    }
+    s = read_lane(scan64(s), 63);
+    if (lane == 0) job.inner[((bh * borders + border_at(c, nreal, nall)) * ntiles + tile) * 4 + w] = s;
   };
 #endif
 
@@ -610,7 +656,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 #endif
 #if DOTS
   Staging<64, SX> rx;
-  start(rx, job.x, job.Hx, c0, cols);
+  start(rx, job.x, job.Hx, c0, job.dots ? cols : 0);
 #endif
   // (always a block further; behind the last one nothing is read)
   const auto fetch = [&](int o) {
@@ -677,6 +723,9 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   struct Pair {
     f4 apart;
     Frag<RP> kj[QB], qi[QB];
+#if DOTS
+    Frag<RP> vj[2], xi[2];
+#endif
   };
   const auto pair_operands = [&](Pair& x, const u16* tiles, int k0) {
 #pragma unroll
@@ -685,9 +734,21 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
       x.qi[ks] = along8<SQ>(tiles, pi, 32 * (k0 + ks), g);
     }
   };
+#if DOTS
+  const auto own_operands = [&](Pair& x, const u16* tiles) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) {
+      x.vj[ks] = along8<SV>(tiles + AT_V, 16 * jt + p, 32 * ks, g);
+      x.xi[ks] = along8<SX>(tiles + AT_X, pi, 32 * ks, g);
+    }
+  };
+#endif
   const auto pair_begin = [&](Pair& x, const u16* tiles, const Decays& D) {
     x.apart = (D.hi[pi] - *(const f4*)(D.hi + pj)) + (D.lo[pi] - *(const f4*)(D.lo + pj));
     pair_operands(x, tiles, 0);
+#if DOTS
+    if (EARLY) own_operands(x, tiles);
+#endif
   };
   const auto pair_product = [&](Pair& x, const u16* tiles) {
     f4 c = {0.f, 0.f, 0.f, 0.f};
@@ -699,7 +760,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     }
     return c;
   };
-  const auto pair_end = [&](const Pair& x, f4 c, const u16* tiles, int o) {
+  const auto pair_end = [&](Pair& x, f4 c, const u16* tiles, int o) {
 #pragma unroll
     for (int r = 0; r < 4; r++) c[r] = pj + r <= pi ? c[r] * (__builtin_amdgcn_exp2f(x.apart[r]) * in_scale) : 0.f;
     u32 d[RP * 2];
@@ -712,18 +773,19 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 #if DOTS
     if (job.pairs && w < 3) {
       f4 a = {0.f, 0.f, 0.f, 0.f};
+      if (!EARLY) own_operands(x, tiles);
 #pragma unroll
-      for (int ks = 0; ks < 2; ks++) a = mul<RAW>(along8<SV>(tiles + AT_V, 16 * jt + p, 32 * ks, g), along8<SX>(tiles + AT_X, pi, 32 * ks, g), a);
-      float row = 0.f;
+      for (int ks = 0; ks < 2; ks++) a = mul<RAW>(x.vj[ks], x.xi[ks], a);
+      double row = 0.0;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const float s = c[r] * a[r];
+        const double s = (double)(c[r] * a[r]);
         row += s;
-        const float col = sum16(s);
-        if (p == 0) of_cols[o % NBUF][it][pj + r] = col;
+        const double col = row_of_16(s);
+        if (p == 15) of_cols[o % NBUF][it][pj + r] = col;
       }
-      row = sum_groups(row);
-      if (g == 0) of_rows[o % NBUF][jt][pi] = row;
+      row = over_rows(row);
+      if (g == 3) of_rows[o % NBUF][jt][pi] = row;
     }
 #endif
   };
@@ -735,8 +797,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   }
 #endif
 #if DOTS
-  // (the state behind the last token, and the gradient that comes in there, are the end of the last span)
-  if (back && first < last && block_of(first) == nreal - 1) mark((nreal - 1) / span);
+  if (back && first < last && block_of(first) == nreal - 1) mark_down(nreal);
 #endif
   for (int o = first; o < last; o++) {
     // With two tiles in LDS, P of the block behind this one is formed here, so that nothing waits for it; with one, this
@@ -746,6 +807,9 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     const u16 *K = tiles + AT_K, *V = tiles + AT_V;
     const Decays& D = decays[n & 15];
     fetch(o + NBUF);
+#if DOTS
+    if (EARLY && !back) mark_ahead(o + 1);
+#endif
     // What a block needs is read from LDS well ahead of its use, and what can be computed without it - the state as a
     // factor, the decayed state, the parts of the decayed v - fills the wait; the fences keep it in that order.
     const float all = D.from_start[L - 1];
@@ -814,14 +878,15 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 #if DOTS
 #pragma unroll
     for (int i = 0; i < LT; i++) {
-      float s = 0.f;
+      double s = 0.0;
 #pragma unroll
       for (int q = 0; q < RP; q++) {
         const v2u x = *(const v2u*)(tiles + AT_X + (q * L + 16 * i + p) * SX + 16 * w + 4 * g);
-        s += y[i][0] * as_f(x[0] << 16) + y[i][1] * as_f(x[0] & 0xffff0000u) + y[i][2] * as_f(x[1] << 16) + y[i][3] * as_f(x[1] & 0xffff0000u);
+        s += (double)y[i][0] * (double)as_f(x[0] << 16) + (double)y[i][1] * (double)as_f(x[0] & 0xffff0000u);
+        s += (double)y[i][2] * (double)as_f(x[1] << 16) + (double)y[i][3] * (double)as_f(x[1] & 0xffff0000u);
       }
-      s = sum_groups(s);
-      if (g == 0) of_state[w][16 * i + p] = s;
+      s = over_rows(s);
+      if (g == 3) of_state[w][16 * i + p] = s;
     }
 #endif
 #endif
@@ -861,15 +926,12 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 #if DOTS
     if (w == 3 && lane < L) {
       const int t = block_of(o) * L + (back ? L - 1 - lane : lane);
-      float s = of_state[0][lane] + of_state[1][lane] + (of_state[2][lane] + of_state[3][lane]);
+      double s = of_state[0][lane] + of_state[1][lane] + (of_state[2][lane] + of_state[3][lane]);
       if (job.pairs) s += (of_rows[n % NBUF][0][lane] + of_rows[n % NBUF][1][lane]) - (of_cols[n % NBUF][0][lane] + of_cols[n % NBUF][1][lane]);
-      if (t < T) job.dots[((i64)tile * args.B * args.H + bh) * T + t] = s * out_scale;
+      if (job.dots && t < T) job.dots[((i64)tile * args.B * args.H + bh) * T + t] = (float)(s * job.out_scale);
     }
-    if (o + 1 < nall) {
-      const int c = block_of(o);                 // (a border: in front of block c + 1, or backwards in front of block c)
-      if (!back && (c + 1) % span == 0 && c + 1 < nreal) mark((c + 1) / span - 1);
-      if (back && c % span == 0) mark(c / span - 1);
-    }
+    if (back) mark_down(block_of(o));
+    else mark_product(o + 1);
 #endif
 #if OUT
     const Buffer into = buffer_at(to);
@@ -887,9 +949,6 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     __syncthreads();
   }
 #if OUT
-#if DOTS
-  if (!back && first < last && last == nreal) mark((nreal - 1) / span);
-#endif
   for (int o = s0; o < s1; o++) {                // blocks without a token
     if (o >= first && o < last) continue;
     for (int u = tid; u < L * 16; u += 256) {
@@ -922,62 +981,56 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 
 // ================================================================== gradient of the decays
 #ifdef KERNEL_GATE
-// The gradient of g_t is what token t's step carries over, <X, exp(g_t) S>: at a border between blocks the product of the
-// two marks there, and from one token to the one before it
+// The gradient of g_t is what token t's step carries over, <X, exp(g_t) S>: at a border between blocks the product that the
+// walks left there, and from one token to the one before it
 //     <X, S> + q_t.dq_t - k_t.dk_t.
-// Summed backwards from the nearest border that has marks (64 bits, at most `span` blocks away), never over a whole long
-// sequence, where what is left of a fast decay would drown in the rounding of what came before.  The dots hold the products;
-// their share within a block is the same number once as q.dq and once as k.dk, so it cancels to the last bit where it should.
-// One workgroup per (batch, head, span).
+// Summed backwards in 64 bits from the nearest border (at most BORDER blocks away), never over a whole sequence, where what
+// is left of a fast decay would drown in the rounding of what came before.  The block's own share of q.dq and k.dk is the same
+// numbers once by rows and once by columns, so it cancels where it should.
+// One workgroup per (batch, head, 32 blocks), a token per thread, a block per half wave.
 struct GateArgs {
   const float* dots_q;      // [tiles][B*H][T]
   const float* dots_k;
-  const float* marks_s;     // [B*H][spans][size]
-  const float* marks_x;
+  const double* inner;      // [B*H][borders][parts]
   Gate g;
   char* dg;                 // [B,T,H]
   const i64* lengths;
-  i64 B, T, H, tiles, span, size, type;
+  i64 B, T, H, tiles, type;
 };
 
 extern "C" __global__ void __launch_bounds__(1024) la_gate(GateArgs a) {
-  __shared__ double part[16];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const i64 nall = (a.T + L - 1) / L, spans = (nall + a.span - 1) / a.span;
-  const i64 bh = blockIdx.x / spans, s = blockIdx.x % spans, b = bh / a.H, h = bh % a.H, BH = a.B * a.H;
-  const i64 len = length_of(a.lengths, b, a.T);
-  const i64 t0 = s * a.span * L, t1 = t0 + a.span * L < a.T ? t0 + a.span * L : a.T, end = t1 < len ? t1 : len;
-  for (i64 t = end > t0 ? end + tid : t0 + tid; t < t1; t += 1024) store_type(a.dg, (b * a.T + t) * a.H + h, (int)a.type, 0.f);
-  if (end <= t0) return;
-  double x = 0.0;
-  const f4 *ms = (const f4*)(a.marks_s + (bh * spans + s) * a.size), *mx = (const f4*)(a.marks_x + (bh * spans + s) * a.size);
-  for (i64 i = tid; i < a.size / 4; i += 1024) {
-    const f4 u = ms[i], v = mx[i];
-    x += (double)(u[0] * v[0] + u[1] * v[1]) + (double)(u[2] * v[2] + u[3] * v[3]);
-  }
-  x = read_lane(scan64(x), 63);
-  if (lane == 0) part[w] = x;
-  __syncthreads();
-  double carry = 0.0;
-  for (int i = 0; i < 16; i++) carry += part[i];
-  if (end < len) carry *= exp(gate_of(a.g, b, h, end));      // (a mark inside the sequence lacks its own step's decay)
-  __syncthreads();
-  for (i64 hi = end; hi > t0; hi -= 1024) {                   // thread i has token hi - 1 - i
-    const i64 t = hi - 1 - tid;
-    double d = 0.0;
-    if (t >= t0)
-      for (i64 k = 0; k < a.tiles; k++) d += (double)a.dots_q[(k * BH + bh) * a.T + t] - (double)a.dots_k[(k * BH + bh) * a.T + t];
-    d = scan64(d);
-    if (lane == 63) part[w] = d;
-    __syncthreads();
-    double before = carry;
-    for (int i = 0; i < 16; i++) {
-      if (i < w) before += part[i];
-      carry += part[i];
+  __shared__ double sums[32], ends[33];          // a block's; what a border in front of a block (or none: unused) holds
+  const int tid = threadIdx.x, lane = tid & 63, blk = tid / L;
+  const int T = (int)a.T, nall = (T + L - 1) / L, groups = (nall + 31) / 32;
+  const i64 bh = blockIdx.x / groups, b = bh / a.H, h = bh % a.H, BH = a.B * a.H;
+  const int c0 = (int)(blockIdx.x % groups) * 32, c = c0 + blk;
+  const int len = (int)length_of(a.lengths, b, T), nreal = (len + L - 1) / L, parts = 4 * (int)a.tiles;
+  if (tid < 33) {
+    const int at = c0 + tid;
+    double x = 0.0;
+    if (at > 0 && at <= nreal && is_border(at, nreal)) {
+      const double* from = a.inner + (bh * borders_of(nall) + border_at(at, nreal, nall)) * parts;
+      for (int i = 0; i < parts; i++) x += from[i];
+      if (at < nreal) x *= exp(gate_of(a.g, b, h, (i64)at * L));         // (inside the sequence the walk has yet to decay by it)
     }
-    if (t >= t0) store_type(a.dg, (b * a.T + t) * a.H + h, (int)a.type, (float)(before + d));
-    __syncthreads();
+    ends[tid] = x;
   }
+  // half a wave holds a block back to front
+  const int t = c * L + L - 1 - (tid & (L - 1));
+  double d = 0.0;
+  if (t < len)
+    for (i64 k = 0; k < a.tiles; k++) d += (double)a.dots_q[(k * BH + bh) * T + t] - (double)a.dots_k[(k * BH + bh) * T + t];
+  d = scan32(d);
+  if ((lane & (L - 1)) == L - 1) sums[blk] = d;
+  __syncthreads();
+  if (t >= T) return;
+  double x = 0.0;
+  if (t < len) {
+    int at = blk + 1;
+    for (; !is_border(c0 + at, nreal); at++) x += sums[at];              // (32 blocks on is a border)
+    x += ends[at] + d;
+  }
+  store_type(a.dg, (b * a.T + t) * a.H + h, (int)a.type, (float)x);
 }
 #endif
 

@@ -30,12 +30,12 @@ WIDTHS = (64, 128, 256)         # what M and N are padded to
 BLOCK = 32                      # tokens per block
 WORKGROUPS = 512                # two per compute unit: below this a sequence is split into segments
 MAX_SEGMENTS = 16
-MARK_BLOCKS = 32                # blocks between the borders at which the gradient of g starts anew
+BORDER = 8                      # blocks between the borders at which the gradient of g starts anew
 
 # argument blocks (see the structs in the source): Tensor 6 fields, Gate 5, States 6
-_JOB = struct.Struct('<6q6q6q6q6q6q7q4q8q2d')
-_BLOCK = struct.Struct('<5qq7q')
-_GATE = '4q5qqq7q'
+_JOB = struct.Struct('<6q6q6q6q6q6q7q5q8q2d')
+_BLOCK = struct.Struct('<5qq6q')
+_GATE = '3q5qqq5q'
 _STEP = '6q6q6q5q6qq8qd'
 
 
@@ -110,7 +110,7 @@ def _ptr(t):
 
 def _segments(groups: int, blocks: int) -> Tuple[int, int]:
     """(segments, blocks per segment) of a walk over `blocks` blocks by `groups` workgroups side by side."""
-    n = min(-(-WORKGROUPS // max(groups, 1)), blocks // 8, MAX_SEGMENTS)
+    n = min(-(-WORKGROUPS // max(groups, 1)), blocks // 16, MAX_SEGMENTS)
     if n <= 1:
         return 1, blocks
     per = -(-blocks // n)
@@ -130,9 +130,9 @@ class _Role:
         self.fields, self.heads = _tensor(t, True), t.shape[2]
 
 
-def _job(q, k, v, x, width, C, init, fin, out, strides, out_type, back=0, pairs=0, in_scale=1.0, out_scale=1.0, dots=0, marks=0):
+def _job(q, k, v, x, width, C, init, fin, out, strides, out_type, back=0, pairs=0, in_scale=1.0, out_scale=1.0, dots=0, marks=0, inner=0):
     """The fields of struct Job that are known before segments are; `local` and `totals` follow in `_walk`."""
-    return [(*q.fields, *k.fields, *v.fields, *(_NO_TENSOR if x is None else x.fields), *init, *fin, out, *strides, out_type, dots, marks),
+    return [(*q.fields, *k.fields, *v.fields, *(_NO_TENSOR if x is None else x.fields), *init, *fin, out, *strides, out_type, dots, marks, inner),
             (q.heads, k.heads, v.heads, 1 if x is None else x.heads, width, C, back, pairs, in_scale, out_scale),
             C % 4 == 0 and all(r is None or r.fields[5] for r in (q, k, v, x))]
 
@@ -162,7 +162,7 @@ def _walk(dev, dtype, jobs, gate, lengths, B, T, H, dots=0):
         totals = th.empty((len(jobs), size), dtype=th.float64, device=dev)
     blob = b''.join([_JOB.pack(*head, 0 if local is None else local[i].data_ptr(), 0 if totals is None else totals[i].data_ptr(), *tail)
                      for i, (head, tail, _) in enumerate(jobs)] + [_NO_JOB] * (2 - len(jobs))
-                    + [_BLOCK.pack(*gate, _ptr(lengths), B, T, H, nseg, per, tiles, MARK_BLOCKS)])
+                    + [_BLOCK.pack(*gate, _ptr(lengths), B, T, H, nseg, per, tiles)])
     for out in ((0, 1) if nseg > 1 else (1,)):
         k = _block_kernel(dev, dtype, width, out, dots if out else 0, fast, wide if out else 0)
         groups = B * H * (nseg if out else nseg - 1)
@@ -193,20 +193,26 @@ def _backward(q, k, v, g, state, lengths, dy, dstate, scale, need_g, need_state)
     share = H // Hk
     pq, pk, type_ = (dq, dk, DTYPES[dt]) if share == 1 else (*th.empty((2, share, B, T, Hk, N), dtype=th.float32, device=dev), 2)
     strides = (T * Hk * N, Hk * N, N, B * T * Hk * N, share)
-    dots = marks = None
-    tiles, spans = -(-N // 64), -(-T // (BLOCK * MARK_BLOCKS))
-    size = -(-N // 16) * 16 * _width(M)
-    if need_g:
-        dots = th.empty((2, tiles, B * H, T), dtype=th.float32, device=dev)
-        marks = th.empty((2, B * H * spans * size), dtype=th.float32, device=dev)
     rq, rk, rv, ry = (_Role(t) for t in (q, k, v, dy))
-    extra = [dict(dots=dots[i].data_ptr(), marks=marks[i].data_ptr()) if need_g else {} for i in range(2)]
-    none = _states(None)
-    _walk(dev, dt, [_job(ry, rv, rk, rq, M, N, _states_t(state), none, pq.data_ptr(), strides, type_, pairs=1, out_scale=scale, **extra[0]),
-                    _job(rv, ry, rq, rk, M, N, _states_t(dstate), _states_t(ds), pk.data_ptr(), strides, type_, back=1, in_scale=scale, **extra[1])],
-          gate, lengths, B, T, H, dots=int(need_g))
-    _walk(dev, dt, [_job(rk, rq, ry, None, N, M, _states(dstate), none, dv.data_ptr(), (T * H * M, H * M, M, 0, 1), DTYPES[dt], back=1, in_scale=scale)],
-          gate, lengths, B, T, H)
+    none, extra = _states(None), [{}, {}]
+    tiles, blocks = -(-N // 64), -(-T // BLOCK)
+    if need_g:
+        borders = -(-blocks // BORDER) + 2
+        dots = th.empty((2, tiles, B * H, T), dtype=th.float32, device=dev)
+        marks = th.empty(B * H * borders * -(-N // 16) * 16 * _width(M), dtype=th.float32, device=dev)
+        inner = th.empty((B * H * borders, tiles * 4), dtype=th.float64, device=dev)
+        extra = [dict(dots=d.data_ptr(), marks=marks.data_ptr(), inner=inner.data_ptr()) for d in dots]
+    of_q = _job(ry, rv, rk, rq, M, N, _states_t(state), none, pq.data_ptr(), strides, type_, pairs=1, out_scale=scale, **extra[0])
+    of_k = _job(rv, ry, rq, rk, M, N, _states_t(dstate), _states_t(ds), pk.data_ptr(), strides, type_, back=1, in_scale=scale, **extra[1])
+    of_v = _job(rk, rq, ry, None, N, M, _states(dstate), none, dv.data_ptr(), (T * H * M, H * M, M, 0, 1), DTYPES[dt], back=1, in_scale=scale)
+    # dq's walk multiplies with what dk's wrote down, so it comes later.  dv's goes along with dk's, at the price of dk's three
+    # parts of the state, where one kernel serves both and the chip has room for them side by side (B2 T500 H8 64x48 fp32:
+    # 21 us less); by itself it takes two thirds of the time.
+    together = _width(M) == _width(N) and (share == 1 or dt == th.float32) and 2 * B * H * max(tiles, -(-M // 64)) <= WORKGROUPS
+    for jobs, dots_ in (([of_k, of_v] if together else [of_k], 1), ([of_q], 1)) if need_g else (([of_q, of_k], 0),):
+        _walk(dev, dt, jobs, gate, lengths, B, T, H, dots=dots_)
+    if not (need_g and together):
+        _walk(dev, dt, [of_v], gate, lengths, B, T, H)
     if share > 1:
         hw.slice_sums([(pq, dq), (pk, dk)], share)
     dg = None
@@ -214,9 +220,8 @@ def _backward(q, k, v, g, state, lengths, dy, dstate, scale, need_g, need_state)
         per_head = g.ndim == 1
         dg = th.empty(g.shape, dtype=g.dtype, device=dev)
         out = th.empty((B, T, H), dtype=th.float32, device=dev) if per_head else dg
-        hw.launch(hw.kernel(dev, SOURCE, 'la_gate', _GATE_DEFINES), dev, B * H * spans, 1024, _GATE,
-                  dots[0].data_ptr(), dots[1].data_ptr(), marks[0].data_ptr(), marks[1].data_ptr(), *gate, out.data_ptr(), _ptr(lengths),
-                  B, T, H, tiles, MARK_BLOCKS, size, DTYPES[out.dtype])
+        hw.launch(hw.kernel(dev, SOURCE, 'la_gate', _GATE_DEFINES), dev, B * H * -(-blocks // 32), 1024, _GATE,
+                  dots[0].data_ptr(), dots[1].data_ptr(), inner.data_ptr(), *gate, out.data_ptr(), _ptr(lengths), B, T, H, tiles, DTYPES[out.dtype])
         if per_head:
             hw.slice_sums([(out, dg)], B * T)
     return dq, dk, dv, dg, ds
