@@ -1,27 +1,31 @@
-"""Hand-written kernels (flex_rnn_amd/csrc/*.hip): compiled per set of preprocessor constants into the same on-disk cache as
-the generated ones, loaded once per device, launched through the same C-ABI runtime on the current stream.
+"""Hand-written kernels (flex_rnn_amd/csrc/*.hip) and the operators over them (csrc/frnn_ops.cpp).
 
-`kernel()` finds or builds one; `launch()` packs the argument block and launches; `slice_sums()` is the reduction over
-leading slices that the backward passes of `linear.py` and `norm.py` share.
+The operators are C++: they allocate, pack argument blocks and launch through the C ABI of include/frnn_rt.h.  When one needs
+a kernel for the first time on a device it asks `_load` here by number; the kernel is then compiled with its constants into the
+same on-disk cache as the generated ones (or found there) and loaded.
 """
 from __future__ import annotations
 
+import ctypes
 import os
-import struct
+import subprocess
 import threading
 from concurrent.futures import ThreadPoolExecutor
-from typing import Dict, Iterable, Tuple
+from typing import Dict, Tuple
 
 import torch as th
 
 from . import runtime
 
-_CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'csrc')
+_HERE = os.path.dirname(os.path.abspath(__file__))
+_CSRC = os.path.join(_HERE, 'csrc')
+OPS_PATH = os.path.join(_HERE, 'libfrnn_ops.so')
 DTYPES = {th.bfloat16: 0, th.float16: 1, th.float32: 2}      # the kernels' type codes
 
 _lock = threading.Lock()
 _sources: Dict[str, str] = {}
-_kernels: Dict[tuple, runtime.Kernel] = {}
+_modules: list = []             # loaded code objects stay as long as the process
+_lib = None
 
 
 def require(ok, message: str):
@@ -30,7 +34,57 @@ def require(ok, message: str):
         raise AssertionError(message)
 
 
-def build(source: str, name: str, defines: Tuple[Tuple[str, int], ...] = (), force: bool = False) -> str:
+# ------------------------------------------------------------------ kernels by number
+Kernel = Tuple[str, str, Tuple[Tuple[str, int], ...]]        # source, kernel, constants
+
+
+def _block(dtype: int, width: int, out: int, dots: int, fast: int, wide: int) -> Kernel:
+    """The walk of linear attention; see csrc/linear_attention.hip.  Two tiles in LDS where two workgroups per compute unit
+    still fit (bfloat16 up to 128 columns)."""
+    w = (64, 128, 256)[width]
+    return ('linear_attention.hip', 'la_block', (('KERNEL_BLOCK', 1), ('IN', dtype), ('W', w), ('OUT', out), ('DOTS', dots), ('FAST', fast), ('WIDE', wide),
+                                                 ('NBUF', 2 if dtype == 0 and w <= 128 else 1), ('OCC', 2)))
+
+
+def _norm(name: str, backward: int):
+    def kernel(dtype, pieces, threads, lanes_log, wide) -> Kernel:
+        return ('layer_norm.hip', name, (('IN', dtype), ('K', pieces), ('TH', 1024 if threads else 256), ('GL', 1 << lanes_log), ('WIDE', wide),
+                                         ('BACKWARD', backward)))
+    return kernel
+
+
+# kind (as in frnn_ops.cpp) -> number of 6-bit fields, and the kernel they stand for
+_KINDS = {
+    1: (6, _block),
+    2: (0, lambda: ('linear_attention.hip', 'la_gate', (('KERNEL_GATE', 1), ('IN', 0)))),
+    3: (1, lambda dtype: ('linear_attention.hip', 'la_step', (('KERNEL_STEP', 1), ('IN', dtype)))),
+    4: (0, lambda: ('slice_sum.hip', 'slice_sum', ())),
+    5: (5, _norm('ln_fw', 0)),
+    6: (5, _norm('ln_bw', 1)),
+}
+
+
+def decode(key: int) -> Kernel:
+    for kind, (n, kernel) in _KINDS.items():
+        if key >> (6 * n) == kind:
+            return kernel(*[key >> (6 * (n - 1 - i)) & 63 for i in range(n)])
+    raise KeyError(key)
+
+
+def builds():
+    """Every code object that an operator can ask for."""
+    out = [_KINDS[2][1](), _KINDS[4][1]()]
+    for dt in DTYPES.values():
+        out.append(_KINDS[3][1](dt))
+        for w in range(3):
+            out += [_block(dt, w, o, d, fast, 0) for o, d in ((1, 0), (1, 1), (0, 0)) for fast in (0, 1)]
+            out += [_block(dt, w, 1, d, 1, 1) for d in (0, 1) if dt != 2]
+        shapes = [(k, 0, lanes, 0) for k in (1, 2, 4) for lanes in range(7) if k == 1 or lanes == 6] + [((2, 2, 4)[dt], t, 10 if t else 8, 1) for t in (0, 1)]
+        out += [_KINDS[kind][1](dt, *s) for kind in (5, 6) for s in shapes]
+    return out
+
+
+def build(source: str, name: str, defines=(), force: bool = False) -> str:
     """Path of the code object of kernel `name` from csrc/`source`, compiled with `defines` on a cache miss."""
     with _lock:
         if source not in _sources:
@@ -40,97 +94,91 @@ def build(source: str, name: str, defines: Tuple[Tuple[str, int], ...] = (), for
     return runtime.compile_kernel(name, _sources[source], opts=opts, force=force)
 
 
-def build_all(cases: Iterable[tuple], force: bool = False, workers: int = 6) -> int:
-    """Compiles `cases` = (source, name, defines), side by side; returns their number."""
-    cases = list(cases)
+def build_all(force: bool = False, workers: int = 6) -> int:
+    """Compiles every kernel, side by side; returns their number."""
+    cases = builds()
     with ThreadPoolExecutor(max_workers=workers) as pool:
         list(pool.map(lambda c: build(*c, force=force), cases))
     return len(cases)
 
 
-def kernel(device: th.device, source: str, name: str, defines: Tuple[Tuple[str, int], ...] = ()) -> runtime.Kernel:
-    key = (device.index, source, name, defines)
-    k = _kernels.get(key)
-    if k is None:
+def _load(device: int, key: int, message: int, capacity: int) -> int:
+    try:
+        source, name, defines = decode(key)
         with th.cuda.device(device):
             if th.cuda.is_current_stream_capturing():
                 raise runtime.RuntimeError_(f'kernel {name} is not loaded yet and cannot be while a graph is captured: '
-                                            'make one call with these types and head sizes before the capture')
-            k = runtime.Module(build(source, name, defines)).kernel(name)
-        k = _kernels.setdefault(key, k)
-    return k
+                                            'make one call with these types and sizes before the capture')
+            module = runtime.Module(build(source, name, defines))
+            _modules.append(module)
+            return module.kernel(name).handle.value
+    except BaseException as e:  # noqa: B902  (nothing may leave through the C++ caller)
+        text = f'{type(e).__name__}: {e}'.encode()[:capacity - 1] + b'\0'
+        ctypes.memmove(message, text, len(text))
+        return 0
 
 
-class Once(th.autograd.Function):
-    """Calls `op(*args)`, the gradient of an operator; a gradient of that is refused (it would silently miss terms)."""
-
-    @staticmethod
-    def forward(ctx, op, *args):
-        return op(*args)
-
-    @staticmethod
-    def backward(ctx, *grads):
-        raise AssertionError('linear_attention and layer_norm can be differentiated once')
+_LOADER = ctypes.CFUNCTYPE(ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64)
+_loader = _LOADER(_load)
 
 
-def once(op, *args):
-    return Once.apply(op, *args) if th.is_grad_enabled() else op(*args)
+# ------------------------------------------------------------------ the operators' library
+def build_library(verbose: bool = False) -> str:
+    """Compiles csrc/frnn_ops.cpp -> flex_rnn_amd/libfrnn_ops.so (host code only, against PyTorch's headers)."""
+    root = os.path.dirname(th.__file__)
+    tmp = OPS_PATH + f'.tmp{os.getpid()}'
+    rocm = os.environ.get('ROCM_PATH', '/opt/rocm')
+    cmd = ['g++', '-std=c++17', '-O2', '-Wall', '-Wno-unused', '-fPIC', '-shared', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
+           f'-D_GLIBCXX_USE_CXX11_ABI={int(th.compiled_with_cxx11_abi())}', '-I', os.path.join(os.path.dirname(_HERE), 'include'),
+           '-isystem', os.path.join(root, 'include'), '-isystem', os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'),
+           '-isystem', os.path.join(rocm, 'include'), os.path.join(_CSRC, 'frnn_ops.cpp'), '-o', tmp, '-L', os.path.join(root, 'lib'),
+           '-lc10', '-ltorch_cpu', '-ltorch', '-lc10_hip', '-L', _HERE, '-lfrnn_rt', '-Wl,-rpath,$ORIGIN']
+    if verbose:
+        print(' '.join(cmd))
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, OPS_PATH)
+    return OPS_PATH
 
 
-_packers: Dict[str, struct.Struct] = {}
+def load() -> ctypes.CDLL:
+    """Registers the operators with PyTorch (once)."""
+    global _lib
+    if _lib is None:
+        with _lock:
+            if _lib is None:
+                if not os.path.isfile(OPS_PATH):
+                    raise runtime.RuntimeError_(f'{OPS_PATH} is missing: the operators have not been built. '
+                                                'Run `python -c "import __graft_entry__ as g; g.build()"`.')
+                runtime.lib()                       # (the kernels' runtime, which the operators link against)
+                th.ops.load_library(OPS_PATH)
+                lib = ctypes.CDLL(OPS_PATH)
+                lib.frnn_ops_set_loader.argtypes = [_LOADER]
+                lib.frnn_ops_set_loader.restype = None
+                lib.frnn_ops_set_loader(_loader)
+                _lib = lib
+    return _lib
 
 
-def launch(k: runtime.Kernel, device: th.device, grid: int, threads: int, layout: str, *args):
-    """Launches `k` on the current stream of `device`; `layout` names the argument block's 8-byte fields (struct)."""
-    p = _packers.get(layout)
-    if p is None:
-        p = _packers[layout] = struct.Struct('<' + layout)
-    launch_bytes(k, device, grid, 1, threads, p.pack(*args))
+def load_if_built():
+    """At import: traced and compiled code finds the operators registered; without the library the first call says so."""
+    if os.path.isfile(OPS_PATH) and os.path.isfile(runtime.LIB_PATH):
+        load()
 
 
-def launch_bytes(k: runtime.Kernel, device: th.device, grid: int, grid_y: int, threads: int, block: bytes):
-    """The same with a packed argument block."""
-    if grid <= 0:
-        return
-    if grid * threads >= 2 ** 32:
-        require(False, f'{k.name}: a launch of {grid} workgroups is more than the hardware takes; split the batch')
-    index = device.index
-    if th.cuda.current_device() != index:
-        with th.cuda.device(device):
-            k.launch((grid, grid_y, 1), (threads, 1, 1), block, stream=_raw_stream(index))
-    else:
-        k.launch((grid, grid_y, 1), (threads, 1, 1), block, stream=_raw_stream(index))
+def op(name: str):
+    load()
+    return getattr(th.ops.flex_rnn, name).default
 
 
-def _raw_stream(index: int) -> int:
-    return th._C._cuda_getCurrentRawStream(index)
+# ------------------------------------------------------------------ host-side rules, as the operators apply them
+def segments(groups: int, blocks: int) -> Tuple[int, int]:
+    """(segments, blocks per segment) of a walk over `blocks` blocks by `groups` workgroups."""
+    out = (ctypes.c_int64 * 2)()
+    load().frnn_ops_segments(ctypes.c_int64(groups), ctypes.c_int64(blocks), out)
+    return out[0], out[1]
 
 
-def slice_sums(pairs, slices: int):
-    """For one or two `(x, out)` of one size and type: out[...] = the sum of `slices` leading fp32 slices of `x`."""
-    out = pairs[0][1] if pairs else None
-    if not pairs or out.numel() == 0:
-        return
-    X, dev = out.numel(), out.device
-    k = kernel(dev, 'slice_sum.hip', 'slice_sum')
-    # as many columns side by side as leave 256 workgroups (up to a 256-byte row of them); the other threads share the slices
-    cw = 1
-    while cw < 64 and cw < X and X // (2 * cw) * len(pairs) >= 256:
-        cw *= 2
-    groups = -(-X // cw)
-    # many slices over few columns: parts of at least 16 trips per thread, joined by a second launch
-    parts = max(1, min(512 // (groups * len(pairs)), slices // (16 * (256 // cw))))
-    ins, outs = [x for x, _ in pairs], [o for _, o in pairs]
-
-    def run(ins, outs, slices, type_, parts):
-        ptrs = [t.data_ptr() for t in (ins[0], outs[0], ins[-1], outs[-1])]
-        launch_bytes(k, dev, groups * parts, len(pairs), 256, _SUM.pack(*ptrs, slices, X, type_, cw, parts))
-
-    if parts > 1:
-        part = th.empty((len(pairs), parts, X), dtype=th.float32, device=dev)
-        run(ins, list(part), slices, 2, parts)
-        ins, slices = list(part), parts
-    run(ins, outs, slices, DTYPES[out.dtype], 1)
-
-
-_SUM = struct.Struct('<9q')
+def norm_shape(rows: int, heads: int, C: int, size: int) -> Dict[str, int]:
+    out = (ctypes.c_int64 * 5)()
+    load().frnn_ops_norm_shape(ctypes.c_int64(rows), ctypes.c_int64(heads), ctypes.c_int64(C), ctypes.c_int64(size), out)
+    return dict(zip(('wide', 'threads', 'pieces', 'lanes', 'teams'), out))

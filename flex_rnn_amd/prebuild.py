@@ -104,12 +104,6 @@ def example_plans():
     return plans
 
 
-def warm_handwritten(force: bool = False) -> int:
-    """Compiles every hand-written kernel (linear attention, layer norm, sums of slices)."""
-    from . import handwritten, linear, norm
-    return handwritten.build_all(linear.builds() + norm.builds() + [('slice_sum.hip', 'slice_sum', ())], force=force)
-
-
 def warm(cases: Iterable = CASES, verbose: bool = False, force: bool = False, examples: bool = False) -> int:
     """Compiles the kernels of `cases`; with `examples` also those of the example layers (eager adapters and traced
     layers) at `EXAMPLE_ARGS`."""

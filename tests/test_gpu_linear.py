@@ -6,7 +6,7 @@ import pytest
 import torch as th
 
 import flex_rnn_amd as F
-from flex_rnn_amd import examples, linear
+from flex_rnn_amd import examples
 
 import linear_cases as lc
 import warm
@@ -40,7 +40,7 @@ def _bounds(inputs, lens, scale, tokens, dy=None, ds=None):
     B, T, H = v.shape[:3]
     share = H // q.shape[2]
     per_token = sum((x.double().abs() * grads[n]).sum(-1).repeat_interleave(share, 2) for n, x in (('q', q), ('k', k)))
-    span = linear.BLOCK * linear.BORDER
+    span = 32 * 8          # a block's tokens, the blocks between borders
     pad = -T % span
     folded = th.nn.functional.pad(per_token, (0, 0, 0, pad)).reshape(B, -1, span, H).sum(2, keepdim=True).expand(-1, -1, span, -1).reshape(B, -1, H)[:, :T]
     # (the product at a span's border: at most what follows sums to, plus the final state's with its gradient)
@@ -257,7 +257,7 @@ def test_partial_gradients():
         lc.assert_within(got, lc.run64(inputs, None, 1.0, *cot)[2][2], _bounds(inputs, None, 1.0, 40, *cot)[4], f'dv of the {name} alone')
     for f in (lambda: F.linear_attention(q, k, v, g, s)[0], lambda: F.layer_norm(v)):
         d, = th.autograd.grad(f(), v, dy.cuda(), create_graph=True)
-        with pytest.raises(AssertionError, match='differentiated once'):
+        with pytest.raises(RuntimeError, match='differentiated once'):
             d.sum().backward()
 
 

@@ -1,12 +1,22 @@
 """Linear attention and layer norm without a GPU: refusals, the plain loop that the GPU tests compare with (against
 `jit.naive` of the recurrences that it covers, and against differences), metadata, host-side planning."""
+import os
+
 import pytest
 import torch as th
 
 import flex_rnn_amd as F
-from flex_rnn_amd import examples, handwritten, linear, norm, ops, prebuild
+from flex_rnn_amd import examples, handwritten, linear, ops, runtime
 
 import linear_cases as lc
+
+
+@pytest.fixture(scope='module', autouse=True)
+def operators(runtime_lib):
+    """The operators' library; built once if a run finds it missing."""
+    if not os.path.isfile(handwritten.OPS_PATH):
+        handwritten.build_library()
+    return handwritten.load()
 
 
 def _meta(*shape, dtype=th.bfloat16):
@@ -153,44 +163,55 @@ def test_plain_loop_lengths_and_gradients():
 
 def test_segments_cover_the_blocks():
     for groups in (1, 2, 7, 64, 511, 512, 5000):
-        for blocks in (0, 1, 7, 16, 17, 35, 1024, 4097):
-            nseg, per = linear._segments(groups, blocks)
-            assert nseg >= 1 and nseg * per >= blocks and nseg <= linear.MAX_SEGMENTS
+        for blocks in (0, 1, 15, 16, 17, 35, 1024, 4097):
+            nseg, per = handwritten.segments(groups, blocks)
+            assert nseg >= 1 and nseg * per >= blocks and nseg <= 16
             assert nseg == 1 or (nseg - 1) * per < blocks          # no segment without a block
-            assert groups < linear.WORKGROUPS or nseg == 1
+            assert groups < 512 or nseg == 1
 
 
-def test_teams_keep_their_head():
-    for shape, heads in (((8192, 32, 128), 32), ((1, 5, 64), 5), ((37, 1000), 1), ((3, 64, 4096), 64), ((70000, 8), 1), ((2, 300, 512), 300)):
-        for dt in (th.bfloat16, th.float32):
-            x = _meta(*shape, dtype=dt)
-            teams, lanes = norm._teams(x, heads)
-            assert teams % heads == 0 and heads <= teams <= x.numel() // shape[-1]
-            wide, threads, k, gl = norm._shape_rule(shape[-1], dt)
-            assert lanes == gl and gl * k * 16 >= shape[-1] * x.element_size() and (gl <= 64 or wide)
+def test_teams_keep_their_head_and_hold_a_row():
+    for rows, heads, C in ((8192 * 32, 32, 128), (5, 5, 64), (37, 1, 1000), (192, 64, 4096), (70000, 1, 8), (600, 300, 512), (3, 1, 16384), (1, 1, 1)):
+        for size in (2, 4):
+            s = handwritten.norm_shape(rows, heads, C, size)
+            assert s['teams'] % heads == 0 and heads <= s['teams'] <= rows
+            assert s['lanes'] * s['pieces'] * 16 >= C * size and (s['wide'] or s['lanes'] <= 64) and s['lanes'] <= s['threads']
 
 
-def test_rows_fold_or_are_copied():
-    x = th.zeros(4, 6, 3, 8)
-    for view, heads, copied in ((x, False, False), (x, True, False), (x.transpose(0, 1), False, True), (x[:, :, :, ::2], False, True),
-                                (x[:, :3], False, True), (x[:, :, 1:], True, False), (x[:2].transpose(1, 2), True, True), (x[..., 2:6], True, False)):
-        got, so, sh = norm._rows(view, heads)
-        assert th.equal(got, view) and (got.data_ptr() == view.data_ptr()) != copied
-        lead = got.shape[:-2] if heads else got.shape[:-1]
-        flat = got.as_strided((lead.numel(), got.shape[-2] if heads else 1, got.shape[-1]), (so, sh, 1))
-        assert th.equal(flat.reshape(-1), view.reshape(-1))
-
-
-def test_every_code_object_of_the_rules_is_prebuilt(runtime_lib, monkeypatch):
-    built = set(linear.builds()) | set(norm.builds())
-    for dt in handwritten.DTYPES:
-        for n in (1, 16, 64, 65, 128, 129, 256):
-            for out, dots in ((1, 0), (1, 1), (0, 0)):
-                for fast in (0, 1):
-                    assert (linear.SOURCE, 'la_block', linear._block_defines(dt, n, out, dots, fast, 0)) in built
-        for C in (1, 5, 64, 100, 513, 600, 1000, 2047, 2049, 3000, 5000, 16384):
-            for name, back in (('ln_fw', False), ('ln_bw', True)):
-                assert (norm.SOURCE, name, norm._defines(C, dt, back)) in built
+def test_every_kernel_that_an_operator_asks_for_is_prebuilt(monkeypatch):
+    built = handwritten.builds()
+    assert len(set(built)) == len(built)
+    for dt in range(3):
+        for C in (1, 5, 64, 100, 513, 600, 1000, 2047, 2049, 4096, 5000, 9000, 16384):
+            s = handwritten.norm_shape(7, 1, C, 4 if dt == 2 else 2)
+            for kind in (5, 6):
+                fields = (dt, s['pieces'], int(s['threads'] == 1024), s['lanes'].bit_length() - 1, s['wide'])
+                key = kind
+                for f in fields:
+                    key = key << 6 | f
+                assert handwritten.decode(key) in built and dict(handwritten.decode(key)[2])['GL'] == s['lanes']
+    assert handwritten.decode(2)[1] == 'la_gate' and handwritten.decode(4)[1] == 'slice_sum' and handwritten.decode(3 << 6 | 1)[1] == 'la_step'
+    key = 1
+    for f in (0, 1, 1, 1, 1, 0):
+        key = key << 6 | f
+    assert handwritten.decode(key) in built and dict(handwritten.decode(key)[2]) == dict(KERNEL_BLOCK=1, IN=0, W=128, OUT=1, DOTS=1, FAST=1, WIDE=0, NBUF=2, OCC=2)
+    with pytest.raises(KeyError):
+        handwritten.decode(9)
     seen = []
     monkeypatch.setattr(handwritten, 'build', lambda *c, force=False: seen.append(c))
-    assert prebuild.warm_handwritten() == len(seen) == len(built) + 1
+    assert handwritten.build_all() == len(seen) == len(built)
+
+
+def test_a_kernel_that_cannot_be_loaded_is_an_error_not_a_crash():
+    """The loader runs on a C++ frame: whatever goes wrong comes back as a message."""
+    import ctypes
+    text = ctypes.create_string_buffer(256)
+    assert handwritten._load(0, 9, ctypes.addressof(text), 256) == 0 and b'KeyError' in text.value
+    assert handwritten._load(0, 4, ctypes.addressof(text), 16) == 0 and len(text.value) == 15          # (no GPU here: cut to the room there is)
+
+
+def test_missing_library_says_how_to_build_it(monkeypatch):
+    monkeypatch.setattr(handwritten, '_lib', None)
+    monkeypatch.setattr(handwritten, 'OPS_PATH', '/nowhere/libfrnn_ops.so')
+    with pytest.raises(runtime.RuntimeError_, match='have not been built'):
+        handwritten.op('layer_norm')
