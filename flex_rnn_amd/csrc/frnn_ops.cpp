@@ -111,7 +111,7 @@ void slice_sums(i64 device, int n, const Tensor* in, const Tensor* out, i64 S) {
 constexpr i64 TOKENS = 32;            // per block
 constexpr i64 BORDER = 8;             // blocks between the borders at which the gradient of g starts anew
 constexpr i64 WORKGROUPS = 512;       // two per compute unit: below this a sequence is split into segments
-constexpr i64 MAX_SEGMENTS = 16;
+constexpr i64 MAX_SEGMENTS = 32;
 
 struct Operand {                      // struct Tensor of the kernels
   const void* p;
@@ -167,7 +167,7 @@ Tensor near(const Tensor& t) {
 Operand operand(const Tensor& t, bool time) {
   const i64 size = t.element_size(), st = time ? t.stride(1) : 0;
   Operand o = {t.data_ptr(), t.stride(0), st, t.stride(time ? 2 : 1), t.stride(-1), 0};
-  o.vec = o.sn == 1 && t.size(-1) % 8 == 0 && ((i64)o.p | o.sb * size | o.st * size | o.sh * size) % 16 == 0;
+  if (o.sn == 1 && t.size(-1) >= 8) o.vec = t.size(-1) % 8 == 0 && ((i64)o.p | o.sb * size | o.st * size | o.sh * size) % 16 == 0 ? 1 : 2;
   return o;
 }
 Gate gate(const Tensor& g) {
@@ -180,11 +180,12 @@ States states(const optional<Tensor>& s, bool rows_m) {
   return {s->data_ptr(), s->stride(0), s->stride(1), s->stride(rows_m ? 2 : 3), s->stride(rows_m ? 3 : 2), type_of(s->scalar_type())};
 }
 
-// (segments, blocks per segment) of a walk over `blocks` blocks by `groups` workgroups side by side.  A segment costs a
-// second walk over k and v for the state at its start, and a launch: at 16 blocks and more the shorter walk wins.
+// (segments, blocks per segment) of a walk over `blocks` blocks by `groups` workgroups side by side.  Segments cost a second
+// walk over k and v for the state at their starts, about half as long as the first, and a launch, about three blocks long:
+// from 12 blocks on, segments of four and more win (T777, 24 workgroups: 53 us in two, 32 us in six).
 std::pair<i64, i64> segments(i64 groups, i64 blocks) {
-  const i64 n = std::min({up(WORKGROUPS, std::max<i64>(groups, 1)), blocks / 16, MAX_SEGMENTS});
-  if (n <= 1) return {1, blocks};
+  const i64 n = std::min({up(WORKGROUPS, std::max<i64>(groups, 1)), blocks / 4, MAX_SEGMENTS});
+  if (n <= 1 || blocks < 12) return {1, blocks};
   const i64 per = up(blocks, n);
   return {up(blocks, per), per};
 }
@@ -220,7 +221,7 @@ void walk(const Problem& p, std::initializer_list<Job> jobs, bool dots) {
   for (const Job& j : jobs) {
     a.job[n++] = j;
     a.tiles = std::max(a.tiles, up(j.C, 64));
-    fast = fast && j.C % 4 == 0 && j.q.vec && j.k.vec && j.v.vec && j.x.vec;
+    fast = fast && j.C % 4 == 0 && j.q.vec == 1 && j.k.vec == 1 && j.v.vec == 1 && j.x.vec == 1;
   }
   const i64 w = width_of(a.job[0].width);
   a.g = p.g, a.lengths = p.lengths, a.B = p.B, a.T = p.T, a.H = p.H;

@@ -79,9 +79,10 @@ constexpr double NO_DECAY = -200.0;           // exp of less is zero in fp32; ke
 
 enum { BF16 = 0, FP16 = 1, FP32 = 2 };
 
-struct Tensor {      // strides in elements; `vec`: 16-byte loads of 8 (4 of fp32) elements are allowed
+struct Tensor {      // strides in elements
   const char* p;
-  i64 sb, st, sh, sn, vec;
+  i64 sb, st, sh, sn;
+  i64 vec;           // how 8 neighbours are read: 1 in aligned pieces of 16 bytes; 2 in pieces at any address (at least 8 columns next to each other); 0 one by one
 };
 
 struct States {      // element (row, column) of a head's state, of a type; or p = null
@@ -249,6 +250,32 @@ DEV Raw load_apart(Buffer base, u32 at, u32 step, int n) {
   return r;
 }
 
+// 8 elements at any address
+DEV Raw load_any(const char* at) {
+  typedef v4u v4u_any __attribute__((aligned(2)));
+  Raw r;
+  for (int i = 0; i < ESZ / 2; i++) r.d[i] = ((const v4u_any*)at)[i];
+  return r;
+}
+// the last 8 - n of them first, zeros behind
+DEV Raw drop(const Raw& r, int n) {
+  Raw o;
+  if constexpr (ESZ == 4) {
+    u32 x[8];
+    for (int e = 0; e < 8; e++) x[e] = r.d[e / 4][e % 4];
+    for (int b = 4; b > 0; b /= 2)
+      for (int e = 0; e < 8; e++) x[e] = n & b ? (e + b < 8 ? x[e + b < 8 ? e + b : e] : 0u) : x[e];
+    for (int e = 0; e < 8; e++) o.d[e / 4][e % 4] = x[e];
+  } else {
+    u64 lo = (u64)r.d[0][1] << 32 | r.d[0][0], hi = (u64)r.d[0][3] << 32 | r.d[0][2];
+    const int bits = 16 * n;
+    lo = n >= 4 ? hi >> (bits & 63) : n > 0 ? lo >> bits | hi << (64 - bits) : lo;
+    hi = n >= 4 ? 0 : n > 0 ? hi >> bits : hi;
+    o.d[0] = v4u{(u32)lo, (u32)(lo >> 32), (u32)hi, (u32)(hi >> 32)};
+  }
+  return o;
+}
+
 template <int PLANE>
 DEV void store_parts(u16* at, const Raw& r) {
   if constexpr (IN == BF16) {
@@ -274,14 +301,14 @@ struct Staging {
   const char* at;           // the next block's first token
   i64 step;
   int token, dir;           // of the thread's first piece
-  bool vec;
+  int vec;
   int left;                 // columns from the thread's own on
 
   DEV_MEMBER void init(const Tensor& t, const char* first, int cols, bool back, int tid) {
     const int row = tid / (W_ / 8), col = tid % (W_ / 8) * 8;
     const u32 st = (u32)t.st * ESZ;
     sn = (u32)t.sn * ESZ;
-    vec = t.vec != 0;
+    vec = (int)t.vec;
     token = back ? L - 1 - row : row;
     dir = back ? -ROWS : ROWS;
     left = cols - col;
@@ -293,13 +320,21 @@ struct Staging {
   // (with vec, columns come in eights: all of a piece's are inside, or none)
   DEV_MEMBER void load(int tokens) {
     const Buffer from = buffer_at(at);
+    const char* before = at;
     at += step;
-    if (FAST || vec) {
+    if (FAST || vec == 1) {
 #pragma unroll
       for (int i = 0; i < N; i++) {
         const u32 o = token + i * dir < tokens ? off[i] : NOTHING;
 #pragma unroll
         for (int e = 0; e < ESZ / 2; e++) r[i].d[e] = __builtin_amdgcn_raw_buffer_load_b128(from, o + 16 * e, 0, 0);
+      }
+    } else if (vec == 2) {
+      // a row's last piece is read so that it ends with the row, and put right on the way to LDS: nothing waits for it here
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        for (int e = 0; e < ESZ / 2; e++) r[i].d[e] = v4u{0, 0, 0, 0};
+        if (left > 0 && token + i * dir < tokens) r[i] = load_any(before + off[i] - (left < 8 ? (8 - left) * ESZ : 0));
       }
     } else {
 #pragma unroll
@@ -313,7 +348,10 @@ struct Staging {
   DEV_MEMBER void store(u16* tile, int tid) {
     const int row = tid / (W_ / 8), col = tid % (W_ / 8) * 8;
 #pragma unroll
-    for (int i = 0; i < N; i++) store_parts<L * STR>(tile + (row + i * ROWS) * STR + col, r[i]);
+    for (int i = 0; i < N; i++) {
+      if (!FAST && vec == 2 && left < 8) r[i] = drop(r[i], left > 0 ? 8 - left : 0);
+      store_parts<L * STR>(tile + (row + i * ROWS) * STR + col, r[i]);
+    }
   }
 };
 
@@ -598,6 +636,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   }
 #endif
 #if OUT
+#pragma unroll 2
   for (i64 s = 0; s < seg; s++) {                // the state at this segment's start
     const i64 at = bh * (nseg - 1) + s;
     const float e = expf((float)job.totals[at]);

@@ -165,7 +165,7 @@ def test_segments_cover_the_blocks():
     for groups in (1, 2, 7, 64, 511, 512, 5000):
         for blocks in (0, 1, 15, 16, 17, 35, 1024, 4097):
             nseg, per = handwritten.segments(groups, blocks)
-            assert nseg >= 1 and nseg * per >= blocks and nseg <= 16
+            assert nseg >= 1 and nseg * per >= blocks and nseg <= 32
             assert nseg == 1 or (nseg - 1) * per < blocks          # no segment without a block
             assert groups < 512 or nseg == 1
 
