@@ -9,6 +9,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/library.h>
 
 #include <array>
@@ -88,9 +89,12 @@ void slice_sums(i64 device, int n, const Tensor* in, const Tensor* out, i64 S) {
   // as many columns side by side (up to a 256-byte row of them) as leave 256 workgroups; the other threads share the slices
   i64 cw = 1;
   while (cw < 64 && cw < X && X / (2 * cw) * n >= 256) cw *= 2;
+  // few slices of many columns: nothing to share, and 16-byte loads (2 x 4 M columns: 12 us against 74; 32 x 1 M: 22 and 25;
+  // with more slices or fewer columns the two come out alike)
+  if (S <= 32 && X % 4 == 0 && X >= 65536) cw = 1024;
   const i64 groups = up(X, cw);
   // many slices over few columns: parts of at least 16 trips per thread, joined by a second launch
-  const i64 parts = std::max<i64>(1, std::min(512 / (groups * n), S / (16 * (256 / cw))));
+  const i64 parts = std::max<i64>(1, std::min(512 / (groups * n), S / (16 * std::max<i64>(256 / cw, 1))));
   SumArgs a;
   for (int i = 0; i < 2; i++) a.pair[i] = {in[i % n].data_ptr(), out[i % n].data_ptr()};
   a.S = S, a.X = X, a.type = type_of(out[0].scalar_type()), a.cw = cw, a.parts = 1;
@@ -110,8 +114,9 @@ void slice_sums(i64 device, int n, const Tensor* in, const Tensor* out, i64 S) {
 // ------------------------------------------------------------------ linear attention
 constexpr i64 TOKENS = 32;            // per block
 constexpr i64 BORDER = 8;             // blocks between the borders at which the gradient of g starts anew
-constexpr i64 WORKGROUPS = 512;       // two per compute unit: below this a sequence is split into segments
-constexpr i64 MAX_SEGMENTS = 32;
+constexpr i64 UNITS = 256;            // compute units
+constexpr i64 WORKGROUPS = 2 * UNITS; // below this a sequence is split into segments
+constexpr i64 MAX_SEGMENTS = 64;
 
 struct Operand {                      // struct Tensor of the kernels
   const void* p;
@@ -182,9 +187,12 @@ States states(const optional<Tensor>& s, bool rows_m) {
 
 // (segments, blocks per segment) of a walk over `blocks` blocks by `groups` workgroups side by side.  Segments cost a second
 // walk over k and v for the state at their starts, about half as long as the first, and a launch, about three blocks long:
-// from 12 blocks on, segments of four and more win (T777, 24 workgroups: 53 us in two, 32 us in six).
+// from 12 blocks on, segments of four and more win (T777, 24 workgroups: 53 us in two, 32 us in six).  Two workgroups per unit
+// are worth up to 16 segments (T8192 H16 128x128: 97 us, 108 with one per unit); more, whose states each segment adds up, only
+// reach for one (T16384 H4: 68 us in 32 segments, 84 in 64; T65536 H2: 91 in 64, 137 in 32).
 std::pair<i64, i64> segments(i64 groups, i64 blocks) {
-  const i64 n = std::min({up(WORKGROUPS, std::max<i64>(groups, 1)), blocks / 4, MAX_SEGMENTS});
+  groups = std::max<i64>(groups, 1);
+  const i64 n = std::min(std::max(std::min<i64>(up(WORKGROUPS, groups), 16), std::min(up(UNITS, groups), MAX_SEGMENTS)), blocks / 4);
   if (n <= 1 || blocks < 12) return {1, blocks};
   const i64 per = up(blocks, n);
   return {up(blocks, per), per};
@@ -242,11 +250,14 @@ void walk(const Problem& p, std::initializer_list<Job> jobs, bool dots) {
   launch(p.device, key_of(BLOCK, {in, wc, 1, dots, fast, wide}), up(p.B * p.H * a.nseg, 8) * 8 * a.tiles, n, 256, &a, sizeof a);
 }
 
+// Offsets of results within a block of tokens are 31 bits, too.
+constexpr i64 MAX_ROW = (1ll << 31) / (TOKENS * 4) - 1;
+
 // What the kernels rely on; flex_rnn_amd/linear.py says what is wrong in words.
 void check(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const optional<Tensor>& state, const optional<Tensor>& lengths, int lead) {
   const i64 B = q.size(0), Hk = q.size(-2), N = q.size(-1), H = v.size(-2), M = v.size(-1);
   bool ok = q.dim() == lead + 2 && q.sizes() == k.sizes() && v.dim() == lead + 2 && q.sizes().slice(0, lead) == v.sizes().slice(0, lead);
-  ok = ok && Hk >= 1 && H >= 1 && H % Hk == 0 && N >= 1 && N <= 256 && M >= 1 && M <= 256 && (lead == 1 || q.size(1) < (1ll << 31) - 64);
+  ok = ok && Hk >= 1 && H >= 1 && H % Hk == 0 && N >= 1 && N <= 256 && M >= 1 && M <= 256 && (lead == 1 || (q.size(1) < (1ll << 31) - 64 && H * M <= MAX_ROW && Hk * N <= MAX_ROW));
   ok = ok && q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type();
   ok = ok && (g.dim() == 1 || (g.dim() == lead + 1 && g.sizes().slice(0, lead) == q.sizes().slice(0, lead))) && g.size(-1) == H;
   if (state) ok = ok && state->sizes() == at::IntArrayRef({B, H, M, N});
@@ -349,6 +360,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward(const Tens
   return {dq, dk, dv, dg, ds};
 }
 
+// Autograd finds that a tensor it has kept was written to.
+void changed(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& state, double scale) {
   check(q, k, v, g, state, {}, 1);
   const c10::DeviceGuard guard(q.device());
@@ -360,6 +376,7 @@ Tensor attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const T
   while (a.gl < 64 && a.gl * (a.vec ? ve : 1) < N) a.gl *= 2;
   a.rows = std::min<i64>(M, 256 / a.gl * 4);
   launch(q.device().index(), key_of(STEP, {in}), B * H * up(M, a.rows), 1, 256, &a, sizeof a);
+  changed(state);
   return y;
 }
 
@@ -497,6 +514,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward_meta(const
           need_g ? at::empty_symint(g.sym_sizes(), g.options()) : at::empty({0}, g.options()), need_state ? at::empty_like(*state) : at::empty({0}, q.options())};
 }
 Tensor attention_step_meta(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& state, double scale) {
+  changed(state);
   return at::empty_symint(v.sym_sizes(), v.options());
 }
 Tensor norm_meta(const Tensor& x, const optional<Tensor>& w, const optional<Tensor>& b, double eps) { return at::empty_symint(x.sym_sizes(), x.options()); }
@@ -533,6 +551,25 @@ Tensor asking(std::initializer_list<optional<Tensor>> inputs) {
   return Tensor();
 }
 
+bool captured(const c10::hip::HIPStream& s) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  return s.stream() && hipStreamIsCapturing(s.stream(), &status) == hipSuccess && status == hipStreamCaptureStatusActive;
+}
+// In a backward pass that is being captured, a gradient for a node on a stream outside the capture - a leaf's, which belongs to
+// the stream of an earlier graph that is still alive - makes autograd wait across the capture's border, on a thread where the
+// error that this gives ends the process.  An error here does not.
+void refuse_nodes_outside_capture(const Tensor& t) {
+  if (!t.is_cuda() || !captured(c10::hip::getCurrentHIPStream(t.device().index()))) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (const auto& e : node->next_edges()) {
+    const auto s = e.is_valid() ? e.function->stream() : std::nullopt;
+    TORCH_CHECK(!s || captured(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *s)),
+                "flex_rnn: a captured backward pass would wait for a stream outside the capture: an input has an autograd graph from before it. "
+                "Delete that graph's results first, or run it on the stream of the capture");
+  }
+}
+
 struct Attention : torch::autograd::Function<Attention> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const optional<Tensor>& state,
                                const optional<Tensor>& lengths, double scale) {
@@ -548,6 +585,7 @@ struct Attention : torch::autograd::Function<Attention> {
     const variable_list s = ctx->get_saved_variables();
     variable_list out(7);
     if (!grads[0].defined() && !grads[1].defined()) return out;
+    refuse_nodes_outside_capture(s[0]);
     const Tensor dy = grads[0].defined() ? grads[0] : at::zeros_like(s[2], at::MemoryFormat::Contiguous);
     const bool need_state = s[4].defined() && ctx->needs_input_grad(4);
     static const auto call = op<decltype(attention_backward)>("flex_rnn::linear_attention_backward");
@@ -597,6 +635,7 @@ struct Norm : torch::autograd::Function<Norm> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
+    refuse_nodes_outside_capture(s[0]);
     const bool need_w = s[1].defined() && ctx->needs_input_grad(1), need_b = s[2].defined() && ctx->needs_input_grad(s[1].defined() ? 2 : 1);
     static const auto call = op<decltype(norm_backward)>("flex_rnn::layer_norm_backward");
     auto [dx, dw, db] = call.call(s[0], maybe(s[1]), maybe(s[2]), grads[0], ctx->saved_data["eps"].toDouble(), need_w, need_b);

@@ -635,7 +635,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   }
 #endif
 #if OUT
-#pragma unroll 2
+#pragma unroll 4
   for (i64 s = 0; s < seg; s++) {                // the state at this segment's start
     const i64 at = bh * (nseg - 1) + s;
     const float e = expf((float)job.totals[at]);

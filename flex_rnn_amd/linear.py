@@ -24,13 +24,14 @@ from .handwritten import DTYPES, require
 
 MAX_HEAD = 256                  # largest M and N
 MAX_TOKENS = 2 ** 31 - 65       # longest sequence (positions are 32 bits, rounded up to blocks)
+MAX_ROW = 2 ** 24 - 1           # a token's elements over all heads (offsets within a block of 32 tokens are 31 bits)
 
 
 def _check(q, k, v, g, state, lead, what, types=True):
     """Argument checks shared by the prompt and the single-token form; `lead`: the dimensions in front of the heads."""
     n, sq, sv, dt = len(lead), q.shape, v.shape, q.dtype
     if len(sq) == len(sv) == n + 2 and sq == k.shape and sq[:n] == sv[:n] and sq[n] >= 1 and sv[n] >= 1 and sv[n] % sq[n] == 0 \
-            and 1 <= sq[-1] <= MAX_HEAD and 1 <= sv[-1] <= MAX_HEAD and (n == 1 or sq[1] <= MAX_TOKENS) \
+            and 1 <= sq[-1] <= MAX_HEAD and 1 <= sv[-1] <= MAX_HEAD and (n == 1 or sq[1] <= MAX_TOKENS and sv[2] * sv[3] <= MAX_ROW and sq[2] * sq[3] <= MAX_ROW) \
             and dt in DTYPES and k.dtype == dt and v.dtype == dt and g.dtype in (dt, th.float32) and g.shape in (sv[n:n + 1], sv[:n + 1]) \
             and (state is None or (state.shape == (sq[0], sv[n], sv[-1], sq[-1]) and state.dtype in (dt, th.float32))):
         return
@@ -43,6 +44,7 @@ def _check(q, k, v, g, state, lead, what, types=True):
     require(Hk >= 1 and H >= 1 and H % Hk == 0, f'{what}: {H} heads of v do not divide into {Hk} heads of q and k')
     require(1 <= N <= MAX_HEAD and 1 <= M <= MAX_HEAD, f'{what}: head sizes from 1 to {MAX_HEAD} (q and k have {N}, v has {M})')
     require(n == 1 or q.shape[1] <= MAX_TOKENS, f'{what}: sequences of up to {MAX_TOKENS} tokens')
+    require(n == 1 or H * M <= MAX_ROW and Hk * N <= MAX_ROW, f'{what}: a token has up to {MAX_ROW} elements over all heads (v has {H * M}, q and k {Hk * N})')
     require(not types or dt in DTYPES and dt == k.dtype == v.dtype, f'{what}: q, k and v are of one type, bfloat16, float16 or float32 (got {dt}, {k.dtype}, {v.dtype})')
     require(not types or g.dtype in (dt, th.float32), f'{what}: g is float32 or of the type of q (got {g.dtype})')
     require(tuple(g.shape) in ((H,), (*v.shape[:n], H)), f'{what}: g is [H] or {names}H] with H = {H} (got {list(g.shape)})')

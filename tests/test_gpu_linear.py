@@ -76,6 +76,7 @@ FORWARD = [
     (FP32, 1, 97, 3, 1, 48, 200, dict(lengths=(1,))),
     (FP32, 1, 1030, 1, 1, 128, 64, dict(resets=0.02)),
     (FP32, 1, 40, 2, 2, 256, 256, {}),
+    (FP16, 1, 8230, 1, 1, 16, 16, dict(resets=0.01)),          # as many segments as there are
 ]
 
 
@@ -107,6 +108,7 @@ GRADIENT = [
     (FP32, 1, 97, 3, 1, 48, 100, dict(lengths=(64,))),
     (FP32, 1, 1030, 2, 2, 16, 32, dict(resets=0.02)),
     (FP32, 1, 33, 1, 1, 256, 256, {}),
+    (BF16, 2, 300, 4, 2, 16, 64, {}),                          # shares of many elements
 ]
 
 
@@ -431,6 +433,31 @@ def test_captured_training_step():
         graph.replay()
         th.cuda.synchronize()
         assert all(th.equal(a, b) for a, b in zip([y, s, *grads], want))
+
+
+def test_captured_gradients_for_an_earlier_graph_are_refused():
+    """A leaf whose eager graph is alive belongs to that graph's stream; a captured backward pass may not wait for it."""
+    print('case capture beside an eager graph', flush=True)
+    inputs, _ = lc.make(BF16, 1, 40, 2, 2, 64, 64)
+    dy, ds = [t.cuda() for t in lc.cotangents(inputs)]
+    leaves = [x.requires_grad_() for x in _gpu(inputs)]
+    for f in (lambda: F.linear_attention(*leaves)[0], lambda: F.layer_norm(leaves[2])):
+        want = th.autograd.grad(f(), leaves[2], dy)[0]
+        alive = f()
+        th.cuda.synchronize()
+        with pytest.raises(RuntimeError, match='a stream outside the capture'):
+            with th.cuda.graph(th.cuda.CUDAGraph()):
+                th.autograd.grad(f(), leaves[2], dy)
+        th.cuda.synchronize()
+        del alive
+        graph = th.cuda.CUDAGraph()
+        with th.cuda.graph(graph):
+            got = th.autograd.grad(f(), leaves[2], dy)[0]
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            th.cuda.synchronize()
+            assert th.equal(got, want)
 
 
 def test_compiles_without_a_break():
