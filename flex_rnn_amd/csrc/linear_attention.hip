@@ -25,7 +25,7 @@
 //   OUT    0: the state alone (what a segment of a sequence leaves behind)
 //   DOTS   1: also what the gradient of g is made of
 //   FAST   1: every operand allows 16-byte loads and rows of y are a multiple of four long.  Without the branches and the
-//          second set of loads and stores that any other layout needs, a block takes a fifth less time
+//          second set of loads and stores that any other layout needs, a block takes a tenth less time
 //   WIDE   with FAST, the type of y: 0 the operands', 1 float32
 //   NBUF   operand tiles in LDS: 2 lets a block's operands arrive while the one before is read, 1 saves LDS
 //   OCC    waves per SIMD to compile for
@@ -35,10 +35,12 @@
 // 8 bits of what is left), and a product of two such factors is the sum of the products of their parts, less those below the
 // last bit that counts.  The bfloat16 exponent is that of float32, so nothing overflows on the way that would not in float32.
 //   - factors read from memory are exact;
-//   - the decayed products P = exp(G_i - G_j) q_i.k_j are rounded to RP parts: one rounding to the inputs' own precision,
-//     as large as the one of the result that they are summed into;
-//   - the state, where it is a factor, is rounded to RP parts too; to three where the product is part of g's gradient, whose
-//     type may be float32 with 16-bit inputs;
+//   - the decayed products P = exp(G_i - G_j) q_i.k_j are rounded to RP parts, and to two with bfloat16: each stands for a whole
+//     row of v, so its rounding would not average out (the second part is 2.5 % of a block's time, and y as far from the exact
+//     result as its own rounding, 1.7e-3 of its norm, where a fast decay leaves little of the state);
+//   - the state, where it is a factor, is rounded to RP parts: one rounding of independent numbers to the inputs' own precision,
+//     as large as the one of the result that they are summed into (2.3e-3 where the state dominates; a second part in bfloat16
+//     takes 5 to 10 % longer); to three where the product is part of g's gradient, whose type may be float32 with 16-bit inputs;
 //   - the decayed v that enters the state has three parts: the state is an fp32 result even where the inputs are not.
 // The state itself stays in fp32 accumulators for the whole sequence.
 //
@@ -172,6 +174,7 @@ DEV void mul_each(const Frag<PA>* a, const Frag<PB>& b, f4* c) {
 }
 constexpr int RAW = RP == 1 ? 0 : 2;           // both factors exact
 constexpr int CALC = RP - 1;                   // one factor rounded to RP parts
+constexpr int PP = RP == 1 ? 2 : RP;           // parts of the decayed products
 
 // ------------------------------------------------------------------ LDS tiles
 constexpr int stride_down(int w) { return w + 16; }       // for tiles read down their columns
@@ -198,12 +201,12 @@ DEV Frag<RP> down(const u16* tile, int r0, int c0, int lane) {
 }
 
 // lane (p, g) gets row r, columns c0 + {4g..4g+3, 16+4g..16+4g+3}
-template <int STR>
-DEV Frag<RP> along(const u16* tile, int r, int c0, int g) {
+template <int STR, int NP = RP>
+DEV Frag<NP> along(const u16* tile, int r, int c0, int g) {
   const u16* at = tile + r * STR + c0 + 4 * g;
-  Frag<RP> f;
+  Frag<NP> f;
 #pragma unroll
-  for (int i = 0; i < RP; i++) {
+  for (int i = 0; i < NP; i++) {
     const v2u a = *(const v2u*)(at + i * L * STR), b = *(const v2u*)(at + i * L * STR + 16);
     f.d[i] = v4u{a[0], a[1], b[0], b[1]};
   }
@@ -596,7 +599,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   __shared__ __attribute__((aligned(16))) u16 stage[NBUF][STAGE];
   __shared__ Decays decays[16];
 #if OUT
-  __shared__ __attribute__((aligned(16))) u16 P[NBUF][RP * L * SP];
+  __shared__ __attribute__((aligned(16))) u16 P[NBUF][PP * L * SP];
 #endif
 #if !OUT
   __shared__ double totals[4];
@@ -642,7 +645,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     const f4* from = (const f4*)job.local + ((at * ntiles + tile) * 4 + w) * (NT * 64) + lane;
     for (int nt = 0; nt < NT; nt++) S[nt] = S[nt] * e + from[nt * 64];
   }
-  for (int i = tid; i < NBUF * RP * L * SP / 8; i += 256) *(v4u*)(&P[0][0] + 8 * i) = v4u{0, 0, 0, 0};     // (stays zero above the diagonal)
+  for (int i = tid; i < NBUF * PP * L * SP / 8; i += 256) *(v4u*)(&P[0][0] + 8 * i) = v4u{0, 0, 0, 0};     // (stays zero above the diagonal)
 #endif
 #if DOTS
   if (tid < NBUF * LT * L) (&of_rows[0][0][0])[tid] = (&of_cols[0][0][0])[tid] = 0.0;
@@ -801,12 +804,12 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   const auto pair_end = [&](Pair& x, f4 c, const u16* tiles, int o) {
 #pragma unroll
     for (int r = 0; r < 4; r++) c[r] = pj + r <= pi ? c[r] * (__builtin_amdgcn_exp2f(x.apart[r]) * in_scale) : 0.f;
-    u32 d[RP * 2];
-    split2<RP>(c[0], c[1], d, 2);
-    split2<RP>(c[2], c[3], d + 1, 2);
+    u32 d[PP * 2];
+    split2<PP>(c[0], c[1], d, 2);
+    split2<PP>(c[2], c[3], d + 1, 2);
     if (w < 3) {
 #pragma unroll
-      for (int q = 0; q < RP; q++) *(v2u*)(P[o % NBUF] + (q * L + pi) * SP + pj) = v2u{d[2 * q], d[2 * q + 1]};
+      for (int q = 0; q < PP; q++) *(v2u*)(P[o % NBUF] + (q * L + pi) * SP + pj) = v2u{d[2 * q], d[2 * q + 1]};
     }
 #if DOTS
     if (job.pairs && w < 3) {
@@ -944,9 +947,9 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     if constexpr (NBUF == 1) __syncthreads();
     {
       const u16* own = P[n % NBUF];
-      const Frag<RP> p0 = along<SP>(own, p, 0, g), p1 = along<SP>(own, 16 + p, 0, g);
-      y[0] = mul<CALC>(vf, p0, y[0]);
-      y[1] = mul<CALC>(vf, p1, y[1]);
+      const Frag<PP> p0 = along<SP, PP>(own, p, 0, g), p1 = along<SP, PP>(own, 16 + p, 0, g);
+      y[0] = mul<PP - 1>(vf, p0, y[0]);
+      y[1] = mul<PP - 1>(vf, p1, y[1]);
     }
 #endif
     if ((n & 7) == 6) {
