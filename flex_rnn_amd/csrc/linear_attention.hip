@@ -605,7 +605,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   __shared__ double totals[4];
 #endif
 #if DOTS
-  __shared__ double of_rows[NBUF][LT][L], of_cols[NBUF][LT][L], of_state[4][L];
+  __shared__ double of_rows[NBUF][LT][L], of_cols[NBUF][LT][L], of_state[NBUF][4][L];
 #endif
   const Job& job = args.job[blockIdx.y];
   const int tid = threadIdx.x, lane = tid & 63, p = lane & 15, g = lane >> 4;
@@ -830,20 +830,38 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     }
 #endif
   };
-  if constexpr (NBUF == 2) {
-    Pair x;
-    pair_begin(x, stage[0], decays[0]);
-    pair_end(x, pair_product(x, stage[0]), stage[0], 0);
-    __syncthreads();
-  }
+  f4 y[LT];                                      // column i = 16 it + p, rows cw + 4 g + r
+  Frag<RP> vf = {};
+  const auto own_share = [&](int n) {            // of block n, whose P lies in LDS
+    const u16* own = P[n % NBUF];
+    const Frag<PP> p0 = along<SP, PP>(own, p, 0, g), p1 = along<SP, PP>(own, 16 + p, 0, g);
+    y[0] = mul<PP - 1>(vf, p0, y[0]);
+    y[1] = mul<PP - 1>(vf, p1, y[1]);
+  };
+  const auto write = [&](int o, bool any) {
+    const Buffer into = buffer_at(to);
+    if (any) to += to_step;
+#pragma unroll
+    for (int it = 0; it < LT; it++) {
+      const int i = back ? L - 1 - (16 * it + p) : 16 * it + p;
+      const int t0 = block_of(o) * L;
+      const f4 z = t0 + i < len ? y[it] * out_scale : f4{0.f, 0.f, 0.f, 0.f};
+      const u32 off = any && t0 + i < T ? to_off[it] : NOTHING;
+      if (wide) store_wide(into, off, z, C - cw - 4 * g, whole);
+      else store_in(into, off, z, C - cw - 4 * g, whole);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < LT; i++) y[i] = f4{0.f, 0.f, 0.f, 0.f};
 #endif
 #if DOTS
   if (back && first < last && block_of(first) == nreal - 1) mark_down(nreal);
 #endif
   for (int o = first; o < last; o++) {
-    // With two tiles in LDS, P of the block behind this one is formed here, so that nothing waits for it; with one, this
-    // block's.
-    const int n = o - first, pn = NBUF == 2 ? n + 1 : n;
+    // With two tiles in LDS, the block's own share of y is added a block later: one barrier a block stands between P's writers
+    // and its readers, and between a tile's readers and its next writers.  (P a block ahead,
+    // which needs two, is 2 to 5 % slower.)
+    const int n = o - first;
     const u16* tiles = stage[n % NBUF];
     const u16 *K = tiles + AT_K, *V = tiles + AT_V;
     const Decays& D = decays[n & 15];
@@ -856,12 +874,16 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     // fences that kept this one made a block 5 % slower.)
     const float all = D.from_start[L - 1];
     const f4 to0 = *(const f4*)(D.to_end + 4 * g), to1 = *(const f4*)(D.to_end + 16 + 4 * g);
-    const Frag<RP> vf = down<SV>(V, 0, 16 * w, lane);
 #if OUT
+    if constexpr (NBUF == 2) {
+      own_share(n + 1);                          // (the one before: two are kept)
+      write(o - 1, n > 0);
+    }
+    vf = down<SV>(V, 0, 16 * w, lane);
     const u16* Q = tiles;
     const float from[LT] = {D.from_start[p], D.from_start[16 + p]};
     Pair pair;
-    pair_begin(pair, stage[pn % NBUF], decays[pn & 15]);
+    pair_begin(pair, tiles, D);
     Frag<RP> qf[QB][LT];
 #pragma unroll
     for (int x = 0; x < QB; x++)
@@ -874,6 +896,8 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) S[nt] *= all;
     }
+#else
+    const Frag<RP> vf = down<SV>(V, 0, 16 * w, lane);
 #endif
     float vx[8];
     frag_values(vf, vx);
@@ -884,10 +908,9 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     }
     const Frag<3> vd = make_frag<3>(vx);
 #if OUT
-    f4 y[LT];                                    // column i = 16 it + p, rows cw + 4 g + r
 #pragma unroll
     for (int i = 0; i < LT; i++) y[i] = f4{0.f, 0.f, 0.f, 0.f};
-    const f4 product = pair_product(pair, stage[pn % NBUF]);
+    const f4 product = pair_product(pair, tiles);
 #endif
     Frag<RP> kf[KB];
 #pragma unroll
@@ -908,7 +931,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
           for (int i = 0; i < LT; i++) qf[x][i] = along<SQ>(Q, 16 * i + p, 32 * (k0 + QB + x), g);
       }
     }
-    pair_end(pair, product, stage[pn % NBUF], pn);
+    pair_end(pair, product, tiles, n);
 #pragma unroll
     for (int i = 0; i < LT; i++) y[i] *= from[i];
 #if DOTS
@@ -922,7 +945,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
         s += (double)y[i][2] * (double)as_f(x[1] << 16) + (double)y[i][3] * (double)as_f(x[1] & 0xffff0000u);
       }
       s = over_rows(s);
-      if (g == 3) of_state[w][16 * i + p] = s;
+      if (g == 3) of_state[n % NBUF][w][16 * i + p] = s;
     }
 #endif
 #endif
@@ -944,12 +967,9 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
       }
     }
 #if OUT
-    if constexpr (NBUF == 1) __syncthreads();
-    {
-      const u16* own = P[n % NBUF];
-      const Frag<PP> p0 = along<SP, PP>(own, p, 0, g), p1 = along<SP, PP>(own, 16 + p, 0, g);
-      y[0] = mul<PP - 1>(vf, p0, y[0]);
-      y[1] = mul<PP - 1>(vf, p1, y[1]);
+    if constexpr (NBUF == 1) {
+      __syncthreads();
+      own_share(n);
     }
 #endif
     if ((n & 7) == 6) {
@@ -961,7 +981,8 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 #if DOTS
     if (w == 3 && lane < L) {
       const int t = block_of(o) * L + (back ? L - 1 - lane : lane);
-      double s = of_state[0][lane] + of_state[1][lane] + (of_state[2][lane] + of_state[3][lane]);
+      const auto& of = of_state[n % NBUF];
+      double s = of[0][lane] + of[1][lane] + (of[2][lane] + of[3][lane]);
       if (job.pairs) s += (of_rows[n % NBUF][0][lane] + of_rows[n % NBUF][1][lane]) - (of_cols[n % NBUF][0][lane] + of_cols[n % NBUF][1][lane]);
       if (job.dots && t < T) job.dots[((i64)tile * args.B * args.H + bh) * T + t] = (float)(s * job.out_scale);
     }
@@ -969,21 +990,17 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     else mark_product(o + 1);
 #endif
 #if OUT
-    const Buffer into = buffer_at(to);
-    to += to_step;
-#pragma unroll
-    for (int it = 0; it < LT; it++) {
-      const int i = back ? L - 1 - (16 * it + p) : 16 * it + p;
-      const int t0 = block_of(o) * L;
-      const f4 z = t0 + i < len ? y[it] * out_scale : f4{0.f, 0.f, 0.f, 0.f};
-      const u32 off = t0 + i < T ? to_off[it] : NOTHING;
-      if (wide) store_wide(into, off, z, C - cw - 4 * g, whole);
-      else store_in(into, off, z, C - cw - 4 * g, whole);
-    }
+    if constexpr (NBUF == 1) write(o, true);
 #endif
-    __syncthreads();
+    if constexpr (NBUF == 1) __syncthreads();
   }
 #if OUT
+  if constexpr (NBUF == 2) {
+    if (first < last) {
+      own_share(last - 1 - first);
+      write(last - 1, true);
+    }
+  }
   for (int o = s0; o < s1; o++) {                // blocks without a token
     if (o >= first && o < last) continue;
     for (int u = tid; u < L * 16; u += 256) {
