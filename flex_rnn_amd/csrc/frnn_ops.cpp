@@ -395,7 +395,7 @@ struct NormArgs {
 struct Shape {
   int wide, threads, pieces, lanes;         // pieces: of 16 bytes, per lane
 };
-// A row stays in the registers of up to 64 lanes with four pieces each; wider rows take a workgroup of 256, then 1024 threads.
+// A row stays in the registers of up to 64 lanes with four pieces each; wider rows take a workgroup of 256, 512 or 1024 threads.
 Shape shape_of(i64 C, i64 size) {
   const i64 pieces = up(C * size, 16);
   for (int k : {1, 2, 4})
@@ -405,11 +405,16 @@ Shape shape_of(i64 C, i64 size) {
       return {0, 256, k, lanes};
     }
   const int k = size == 4 ? 4 : 2;
-  return pieces <= 256 * k ? Shape{1, 256, k, 256} : Shape{1, 1024, k, 1024};
+  int threads = 256;
+  while (threads * k < pieces) threads *= 2;
+  return {1, threads, k, threads};
 }
 
-// as many rows side by side as keep the chip busy, a multiple of `heads` (a team of lanes keeps its head)
-i64 teams_of(i64 rows, i64 heads, i64 lanes) { return std::min(rows / heads, std::max<i64>(1, THREADS / (lanes * heads))) * heads; }
+// as many rows side by side as keep the chip busy, a multiple of `heads` (a team of lanes keeps its head); of workgroups with 1024
+// threads one per compute unit (128 of them: 54 us against 39 for 2048 rows of 16384 bfloat16; 512: 54)
+i64 teams_of(i64 rows, i64 heads, i64 lanes) {
+  return std::min(rows / heads, std::max<i64>(1, (lanes == 1024 ? 2 : 1) * THREADS / (lanes * heads))) * heads;
+}
 
 struct Rows {
   Tensor t;
@@ -449,10 +454,10 @@ void norm_launch(Kind kind, const Rows& x, const Rows& dy, const Tensor& out, co
   const Shape s = shape_of(C, size);
   NormArgs a = {x.t.data_ptr(), dy.t.defined() ? dy.t.data_ptr() : nullptr, out.data_ptr(), ptr(w), ptr(b), dw, db, out.numel() / C, heads, C,
                 x.outer, x.head, dy.outer, dy.head, w ? type_of(w->scalar_type()) : 2, b ? type_of(b->scalar_type()) : 2, 0, teams, eps};
-  a.vec = C * size % 16 == 0 && ((i64)a.x | (i64)a.dy | (x.outer | x.head | dy.outer | dy.head) * size) % 16 == 0;
+  a.vec = C * size >= 16;
   int lanes_log = 0;
   while (1 << lanes_log < s.lanes) lanes_log++;
-  launch(device, key_of(kind, {type_of(out.scalar_type()), s.pieces, s.threads == 1024, lanes_log, s.wide}), s.wide ? teams : up(teams * s.lanes, s.threads), 1,
+  launch(device, key_of(kind, {type_of(out.scalar_type()), s.pieces, lanes_log, s.wide}), s.wide ? teams : up(teams * s.lanes, s.threads), 1,
          s.threads, &a, sizeof a);
 }
 

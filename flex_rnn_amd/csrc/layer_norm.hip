@@ -13,9 +13,14 @@
 // issued before the current row is worked on.  Shares of dw and db meet in two steps in a fixed order (per team in fp32,
 // between teams by the kernel that sums slices in 64 bits), never in atomics.
 //
+// Measured against the 5.1 TB/s of a large copy, per-column w and b in fp32: forward 8192 x 4096 bfloat16 32 us (4.2 TB/s),
+// 262144 x 128 27 us (5.0), 2048 x 16384 39 us (3.4), 4096 x 8192 float32 46 us (5.8, part of it from the last-level cache);
+// forward and backward together 95, 97, 151 and 148 us (five passes of 67 or 134 MB: 3.5, 3.5, 2.2 and 4.5 TB/s).  Backward, the
+// registers for w, dw and db leave fewer rows in flight, and 1024 threads (over 8192 columns) spill some of them.
+//
 // Sums over a row are fp32 and two passes over registers (mean first, then squares of what is left): no cancellation.
 //
-// Compiled by flex_rnn_amd/norm.py with IN (0 bfloat16, 1 float16, 2 float32), K, TH (threads), GL, WIDE and BACKWARD.
+// Compiled by flex_rnn_amd/handwritten.py with IN (0 bfloat16, 1 float16, 2 float32), K, TH (threads), GL, WIDE and BACKWARD.
 #include <hip/hip_runtime.h>
 
 typedef unsigned int u32;
@@ -58,16 +63,22 @@ struct Piece {               // 16 bytes of a row as they are in memory
   v4u d;
 };
 
-DEV Piece load_piece(const char* row, int n, int C, bool vec) {
+// 16 bytes at any address of the element type
+typedef v4u v4u_any __attribute__((aligned(2)));
+
+// Columns start .. start + VE - 1 of a row.  A row's last piece is moved back so that it ends with the row: its first `skip`
+// columns belong to the piece before it too, are left out of sums, and come out the same twice.  (Whole pieces at any address:
+// 33588 rows of 999 bfloat16 take 30 us, 91 one element at a time.)  Of a row shorter than a piece, `start` is negative.
+DEV Piece load_piece(const char* row, int start, int skip, bool vec) {
   Piece r;
   r.d = v4u{0, 0, 0, 0};
   if (vec) {
-    if (n < C) r.d = *(const v4u*)(row + (i64)n * ESZ);     // (C is a multiple of VE here)
+    if (skip < VE) r.d = *(const v4u_any*)(row + (i64)start * ESZ);
   } else {
     for (int e = 0; e < VE; e++)
-      if (n + e < C) {
-        if constexpr (IN == FP32) r.d[e] = ((const u32*)row)[n + e];
-        else r.d[e / 2] |= (u32)((const u16*)row)[n + e] << (e % 2 * 16);
+      if (e >= skip) {
+        if constexpr (IN == FP32) r.d[e] = ((const u32*)row)[start + e];
+        else r.d[e / 2] |= (u32)((const u16*)row)[start + e] << (e % 2 * 16);
       }
   }
   return r;
@@ -79,7 +90,7 @@ DEV void values(const Piece& r, float* x) {
     else x[e] = e % 2 ? as_f(r.d[e / 2] & 0xffff0000u) : as_f(r.d[e / 2] << 16);
   }
 }
-DEV void store_piece(char* row, int n, int C, bool vec, const float* x) {
+DEV void store_piece(char* row, int start, int skip, bool vec, const float* x) {
   v4u d;
   for (int e = 0; e < 4; e++) {
     if constexpr (IN == FP32) d[e] = __float_as_uint(x[e]);
@@ -87,12 +98,12 @@ DEV void store_piece(char* row, int n, int C, bool vec, const float* x) {
     else d[e] = (u32)__builtin_bit_cast(u16, (_Float16)x[2 * e]) | (u32)__builtin_bit_cast(u16, (_Float16)x[2 * e + 1]) << 16;
   }
   if (vec) {
-    if (n < C) *(v4u*)(row + (i64)n * ESZ) = d;
+    if (skip < VE) *(v4u_any*)(row + (i64)start * ESZ) = d;
   } else {
     for (int e = 0; e < VE; e++)
-      if (n + e < C) {
-        if constexpr (IN == FP32) ((u32*)row)[n + e] = d[e];
-        else ((u16*)row)[n + e] = (u16)(d[e / 2] >> (e % 2 * 16));
+      if (e >= skip) {
+        if constexpr (IN == FP32) ((u32*)row)[start + e] = d[e];
+        else ((u16*)row)[start + e] = (u16)(d[e / 2] >> (e % 2 * 16));
       }
   }
 }
@@ -166,16 +177,24 @@ ln_fw(Args a) {
   const i64 head = live ? team % a.heads : 0;
   const float inv = 1.f / (float)C, eps = (float)a.eps;
 
+  int start[K], skip[K];
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const int n = (sub + k * lanes) * VE;
+    start[k] = n < C - VE ? n : C - VE;
+    skip[k] = n - start[k] < VE ? n - start[k] : VE;
+  }
   float w[K * VE];
 #if !BACKWARD
   float b[K * VE];
 #endif
   for (int k = 0; k < K; k++)
     for (int e = 0; e < VE; e++) {
-      const int n = (sub + k * lanes) * VE + e;
-      w[k * VE + e] = a.w && n < C ? load_type(a.w, head * C + n, (int)a.w_type) : 1.f;
+      const int n = start[k] + e;
+      const bool in = n >= 0 && skip[k] < VE;
+      w[k * VE + e] = a.w && in ? load_type(a.w, head * C + n, (int)a.w_type) : 1.f;
 #if !BACKWARD
-      b[k * VE + e] = a.b && n < C ? load_type(a.b, head * C + n, (int)a.b_type) : 0.f;
+      b[k * VE + e] = a.b && in ? load_type(a.b, head * C + n, (int)a.b_type) : 0.f;
 #endif
     }
 #if BACKWARD
@@ -189,9 +208,9 @@ ln_fw(Args a) {
   const auto fetch = [&](i64 o) {
 #pragma unroll
     for (int k = 0; k < K; k++) {
-      nx[k] = load_piece(a.x + (o * a.sx + head * a.hx) * ESZ, (sub + k * lanes) * VE, C, vec);
+      nx[k] = load_piece(a.x + (o * a.sx + head * a.hx) * ESZ, start[k], skip[k], vec);
 #if BACKWARD
-      ny[k] = load_piece(a.dy + (o * a.sy + head * a.hy) * ESZ, (sub + k * lanes) * VE, C, vec);
+      ny[k] = load_piece(a.dy + (o * a.sy + head * a.hy) * ESZ, start[k], skip[k], vec);
 #endif
     }
   };
@@ -209,15 +228,15 @@ ln_fw(Args a) {
 #endif
     if (o + step < outers) fetch(o + step);
     float s = 0.f;
-    for (int i = 0; i < K * VE; i++) s += x[i];
+    for (int i = 0; i < K * VE; i++) s += i % VE >= skip[i / VE] ? x[i] : 0.f;
     const float mean = team_sum(f2{s, 0.f}, gl, lds, tid)[0] * inv;
     s = 0.f;
 #pragma unroll
     for (int k = 0; k < K; k++)
       for (int e = 0; e < VE; e++) {
         const int i = k * VE + e;
-        x[i] = (sub + k * lanes) * VE + e < C ? x[i] - mean : 0.f;
-        s += x[i] * x[i];
+        x[i] -= mean;
+        s += e >= skip[k] ? x[i] * x[i] : 0.f;
       }
     const float rstd = 1.f / sqrtf(team_sum(f2{s, 0.f}, gl, lds, tid)[0] * inv + eps);
     char* to = a.y + (o * a.heads + head) * C * (i64)ESZ;
@@ -228,8 +247,9 @@ ln_fw(Args a) {
       dw[i] += d[i] * x[i];
       db[i] += d[i];
       d[i] *= w[i];
-      m[0] += d[i];
-      m[1] += d[i] * x[i];
+      const bool in = i % VE >= skip[i / VE];
+      m[0] += in ? d[i] : 0.f;
+      m[1] += in ? d[i] * x[i] : 0.f;
     }
     m = team_sum(m, gl, lds, tid) * inv;
     for (int i = 0; i < K * VE; i++) x[i] = rstd * (d[i] - m[0] - x[i] * m[1]);
@@ -237,14 +257,14 @@ ln_fw(Args a) {
     for (int i = 0; i < K * VE; i++) x[i] = x[i] * rstd * w[i] + b[i];
 #endif
 #pragma unroll
-    for (int k = 0; k < K; k++) store_piece(to, (sub + k * lanes) * VE, C, vec, x + k * VE);
+    for (int k = 0; k < K; k++) store_piece(to, start[k], skip[k], vec, x + k * VE);
   }
 #if BACKWARD
   if (live)
     for (int k = 0; k < K; k++)
       for (int e = 0; e < VE; e++) {
-        const int n = (sub + k * lanes) * VE + e;
-        if (n < C) {
+        const int n = start[k] + e;
+        if (e >= skip[k]) {
           if (a.dw) a.dw[team * C + n] = dw[k * VE + e];
           if (a.db) a.db[team * C + n] = db[k * VE + e];
         }

@@ -18,7 +18,7 @@
 // so one kernel, la_block, computes y and all three; backwards, a sequence is read from its end and the decay of a position
 // is the one of the token behind it.
 //
-// Compiled per set of constants by flex_rnn_amd/linear.py, which passes
+// Compiled per set of constants by flex_rnn_amd/handwritten.py, which passes
 //   KERNEL_BLOCK / KERNEL_GATE / KERNEL_STEP   which kernel this code object holds
 //   IN     element type of q, k, v, dy: 0 bfloat16, 1 float16, 2 float32
 //   W      padded width (64, 128 or 256) of q and k

@@ -47,8 +47,8 @@ def _block(dtype: int, width: int, out: int, dots: int, fast: int, wide: int) ->
 
 
 def _norm(name: str, backward: int):
-    def kernel(dtype, pieces, threads, lanes_log, wide) -> Kernel:
-        return ('layer_norm.hip', name, (('IN', dtype), ('K', pieces), ('TH', 1024 if threads else 256), ('GL', 1 << lanes_log), ('WIDE', wide),
+    def kernel(dtype, pieces, lanes_log, wide) -> Kernel:
+        return ('layer_norm.hip', name, (('IN', dtype), ('K', pieces), ('TH', max(256, 1 << lanes_log)), ('GL', 1 << lanes_log), ('WIDE', wide),
                                          ('BACKWARD', backward)))
     return kernel
 
@@ -59,8 +59,8 @@ _KINDS = {
     2: (0, lambda: ('linear_attention.hip', 'la_gate', (('KERNEL_GATE', 1), ('IN', 0)))),
     3: (1, lambda dtype: ('linear_attention.hip', 'la_step', (('KERNEL_STEP', 1), ('IN', dtype)))),
     4: (0, lambda: ('slice_sum.hip', 'slice_sum', ())),
-    5: (5, _norm('ln_fw', 0)),
-    6: (5, _norm('ln_bw', 1)),
+    5: (4, _norm('ln_fw', 0)),
+    6: (4, _norm('ln_bw', 1)),
 }
 
 
@@ -79,7 +79,7 @@ def builds():
         for w in range(3):
             out += [_block(dt, w, o, d, fast, 0) for o, d in ((1, 0), (1, 1), (0, 0)) for fast in (0, 1)]
             out += [_block(dt, w, 1, d, 1, 1) for d in (0, 1) if dt != 2]
-        shapes = [(k, 0, lanes, 0) for k in (1, 2, 4) for lanes in range(7) if k == 1 or lanes == 6] + [((2, 2, 4)[dt], t, 10 if t else 8, 1) for t in (0, 1)]
+        shapes = [(k, lanes, 0) for k in (1, 2, 4) for lanes in range(7) if k == 1 or lanes == 6] + [(4 if dt == 2 else 2, lanes, 1) for lanes in (8, 9, 10)]
         out += [_KINDS[kind][1](dt, *s) for kind in (5, 6) for s in shapes]
     return out
 

@@ -197,10 +197,10 @@ def test_every_kernel_that_an_operator_asks_for_is_prebuilt(monkeypatch):
     built = handwritten.builds()
     assert len(set(built)) == len(built)
     for dt in range(3):
-        for C in (1, 5, 64, 100, 513, 600, 1000, 2047, 2049, 4096, 5000, 9000, 16384):
+        for C in (1, 5, 64, 100, 513, 600, 1000, 2047, 2049, 4096, 5000, 8192, 9000, 16384):
             s = handwritten.norm_shape(7, 1, C, 4 if dt == 2 else 2)
             for kind in (5, 6):
-                fields = (dt, s['pieces'], int(s['threads'] == 1024), s['lanes'].bit_length() - 1, s['wide'])
+                fields = (dt, s['pieces'], s['lanes'].bit_length() - 1, s['wide'])
                 key = kind
                 for f in fields:
                     key = key << 6 | f
