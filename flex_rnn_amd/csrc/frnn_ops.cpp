@@ -94,7 +94,7 @@ void slice_sums(i64 device, int n, const Tensor* in, const Tensor* out, i64 S) {
   if (S <= 32 && X % 4 == 0 && X >= 65536) cw = 1024;
   const i64 groups = up(X, cw);
   // many slices over few columns: parts of at least 16 trips per thread, joined by a second launch
-  const i64 parts = std::max<i64>(1, std::min(512 / (groups * n), S / (16 * std::max<i64>(256 / cw, 1))));
+  const i64 parts = cw > 256 ? 1 : std::max<i64>(1, std::min(512 / (groups * n), S / (16 * (256 / cw))));
   SumArgs a;
   for (int i = 0; i < 2; i++) a.pair[i] = {in[i % n].data_ptr(), out[i % n].data_ptr()};
   a.S = S, a.X = X, a.type = type_of(out[0].scalar_type()), a.cw = cw, a.parts = 1;

@@ -489,7 +489,7 @@ NORM = [
     (FP16, (33, 4, 64), 'heads', FP16), (FP16, (9, 1111), 'columns', FP32), (FP16, (40, 5000), 'bias', FP16),
     (FP32, (70, 2, 24), 'heads', FP32), (FP32, (5, 4095), 'columns', FP32), (FP32, (3, 9000), 'weight', FP32), (FP32, (64,), 'columns', FP32),
     (BF16, (700, 5), 'columns', FP32), (BF16, (20, 8), 'columns', BF16), (FP16, (6, 3, 9), 'heads', FP32), (FP16, (5, 8191), 'columns', FP16), (FP32, (9, 3), 'columns', FP32),
-    (FP32, (700, 5), 'columns', FP32), (FP32, (3, 6001), 'columns', FP32), (FP32, (2, 16383), 'bias', FP32), (BF16, (300, 16381), 'columns', BF16),
+    (BF16, (40, 64, 1024), 'heads', FP32), (FP32, (700, 5), 'columns', FP32), (FP32, (3, 6001), 'columns', FP32), (FP32, (2, 16383), 'bias', FP32), (BF16, (300, 16381), 'columns', BF16),
 ]
 
 
