@@ -560,18 +560,18 @@ bool captured(const c10::hip::HIPStream& s) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   return s.stream() && hipStreamIsCapturing(s.stream(), &status) == hipSuccess && status == hipStreamCaptureStatusActive;
 }
-// In a backward pass that is being captured, a gradient for a node on a stream outside the capture - a leaf's, which belongs to
-// the stream of an earlier graph that is still alive - makes autograd wait across the capture's border, on a thread where the
-// error that this gives ends the process.  An error here does not.
+// In a backward pass that is being captured, a gradient for a node on the default stream - a leaf's, which belongs to the stream
+// of an earlier graph that is still alive - makes autograd let that stream wait for the capture, which it cannot, on a thread
+// where the error ends the process.  An error here does not.  (Any other stream joins the capture by waiting for it.)
 void refuse_nodes_outside_capture(const Tensor& t) {
   if (!t.is_cuda() || !captured(c10::hip::getCurrentHIPStream(t.device().index()))) return;
   const auto node = torch::autograd::get_current_node();
   if (!node) return;
   for (const auto& e : node->next_edges()) {
     const auto s = e.is_valid() ? e.function->stream() : std::nullopt;
-    TORCH_CHECK(!s || captured(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *s)),
-                "flex_rnn: a captured backward pass would wait for a stream outside the capture: an input has an autograd graph from before it. "
-                "Delete that graph's results first, or run it on the stream of the capture");
+    TORCH_CHECK(!s || c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *s).stream(),
+                "flex_rnn: a captured backward pass would make the default stream, a stream outside the capture, wait for it: an input has an autograd "
+                "graph from before. Delete that graph's results first, or compute it on another stream");
   }
 }
 

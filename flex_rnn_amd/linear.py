@@ -9,9 +9,11 @@ Recurrences whose decay differs along the state's columns, or that read the stat
     y, state = linear_attention(q, k, v, g, state)              # a prompt, or training (differentiable)
     y = linear_attention_step(q, k, v, g, state)                # one token; `state` is updated in place
 
-The kernels are in csrc/linear_attention.hip, their launches and gradients in csrc/frnn_ops.cpp.  Like the compiled operators they run on the GPU only, on the current stream of
-the tensors' device, without synchronising, and can be captured into a HIP graph after a first call with the same types
-and head sizes; `linear_attention.naive` and `linear_attention.naive_fp64` are the per-token loop in plain PyTorch.
+The kernels are in csrc/linear_attention.hip, their launches and gradients in csrc/frnn_ops.cpp.  Like the compiled operators
+they run on the GPU only, on the current stream of the tensors' device, without synchronising, and can be captured into a HIP
+graph after a first call with the same types, sizes and layouts (a captured backward pass: while no graph of the same leaves
+from the default stream is alive; it says so).  `linear_attention.naive` and `linear_attention.naive_fp64` are the per-token loop
+in plain PyTorch.
 """
 from __future__ import annotations
 
@@ -87,7 +89,7 @@ def linear_attention_step(q: th.Tensor, k: th.Tensor, v: th.Tensor, g: th.Tensor
     """One token of `linear_attention` for decoding: `state` [B,H,M,N] is updated in place, y [B,H,M] is returned.
 
     q, k [B,Hk,N], v [B,H,M], g [B,H] or [H]; types as there.  Any strides, except that no two elements of the state may
-    share memory.  Not differentiable: with T = 1, `linear_attention` is.
+    share memory, nor may one with another argument.  Not differentiable: with T = 1, `linear_attention` is.
     """
     _check(q, k, v, g, state, ('B',), 'linear_attention_step')
     _check_device('linear_attention_step', q, k, v, g, state)
