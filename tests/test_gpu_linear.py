@@ -236,6 +236,57 @@ def test_strides_and_broadcast_inputs():
     assert th.empty_like(s.mT).stride() == F.linear_attention(q, k, v, g, s.mT)[1].stride()
 
 
+def test_offsets_beyond_32_bits():
+    """Batches, tokens, rows and states that lie gigabytes apart, as in a pool, against the same numbers side by side."""
+    print('case far apart', flush=True)
+    B, T, H, M, N = 2, 33, 2, 64, 64
+    inputs, _ = lc.make(BF16, B, T, H, H, M, N, state=BF16)
+    dy, ds = [t.cuda() for t in lc.cotangents(inputs)]
+    xs = _gpu(inputs)
+    want = _gradients(xs, None, 1.0, dy, ds)
+    pool = th.empty(2 ** 31 + 2 ** 27, dtype=BF16, device='cuda')
+    far_batch = pool.as_strided((B, T, H, N), (2 ** 31, H * N, N, 1))
+    far_token = pool.as_strided((B, T, H, N), (H * N, 2 ** 26, N, 1), 2 ** 20)
+    far_state = pool.as_strided((B, H, M, N), (2 ** 31, M * N, N, 1), 2 ** 19)
+    for at in (far_batch, far_token):
+        at.copy_(xs[1])
+        far_state.copy_(xs[4])
+        got = _gradients([xs[0], at, xs[2], xs[3], far_state], None, 1.0, dy, ds)
+        assert all(th.equal(a, b) for a, b in zip(got, want))
+    state = xs[4].clone()
+    y = F.linear_attention_step(xs[0][:, 0], xs[1][:, 0], xs[2][:, 0], xs[3][:, 0], state)
+    assert th.equal(y, F.linear_attention_step(xs[0][:, 0], xs[1][:, 0], xs[2][:, 0], xs[3][:, 0], far_state)) and th.equal(state, far_state)
+    rows = pool.as_strided((3, 100), (2 ** 30, 1), 2 ** 18)
+    rows.copy_(th.randn(3, 100, device='cuda'))
+    assert th.equal(F.layer_norm(rows), F.layer_norm(rows.contiguous()))
+
+
+def test_threads_on_streams_of_their_own():
+    print('case threads', flush=True)
+    import threading
+    inputs, _ = lc.make(FP16, 1, 450, 2, 1, 24, 40)
+    dy, ds = [t.cuda() for t in lc.cotangents(inputs)]
+    xs = _gpu(inputs)
+    th.cuda.synchronize()
+    results = [None] * 4
+
+    def run(i):
+        stream = th.cuda.Stream()
+        with th.cuda.stream(stream):
+            out = [_gradients(xs, None, 1.0, dy, ds) + [F.layer_norm(xs[2])] for _ in range(5)]
+        stream.synchronize()
+        results[i] = out
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    want = _gradients(xs, None, 1.0, dy, ds) + [F.layer_norm(xs[2])]
+    for r in results:
+        assert all(th.equal(a, b) for out in r for a, b in zip(out, want))
+
+
 def test_partial_gradients():
     print('case partial gradients', flush=True)
     inputs, _ = lc.make(BF16, 1, 40, 2, 2, 64, 64)
