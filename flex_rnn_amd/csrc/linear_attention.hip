@@ -1096,8 +1096,8 @@ extern "C" __global__ void __launch_bounds__(1024) la_gate(GateArgs a) {
 
 // ================================================================== one token
 #ifdef KERNEL_STEP
-// S = exp(g) S + v k^T in place, y = scale S q.  Bound by reading and writing the state once: 124 us for 128 sequences x
-// 32 heads of 128x128 in fp32 (4.4 TB/s of the 5.1 that a large copy reaches), 8 us for one sequence, which is the call.  A group of `gl` lanes owns
+// S = exp(g) S + v k^T in place, y = scale S q.  Bound by reading and writing the state once: 110 us for 128 sequences x
+// 32 heads of 128x128 in fp32 (4.9 TB/s of the 5.1 that a large copy reaches), 8 us for one sequence, which is the call.  A group of `gl` lanes owns
 // rows of the state, a lane VE neighbouring columns (16 bytes) of each, whose q and k it holds; R rows are in flight at a
 // time.  States that do not allow 16-byte accesses go column by column.
 struct StepArgs {
