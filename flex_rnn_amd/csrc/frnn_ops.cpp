@@ -374,9 +374,10 @@ Tensor attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const T
   StepArgs a = {operand(q, false), operand(k, false), operand(v, false), gate(g), states(state, true), y.data_ptr(), B, H, Hk, M, N, 0, 1, 0, scale};
   a.vec = a.s.sc == 1 && N % ve == 0 && ((i64)a.s.p | a.s.sb * size | a.s.sh * size | a.s.sr * size) % 16 == 0;
   while (a.gl < 64 && a.gl * (a.vec ? ve : 1) < N) a.gl *= 2;
-  // eight rows per thread, four in flight (128 sequences x 32 heads of 128x128: 110 us; with four rows 124, twelve 134, sixteen 115)
-  a.rows = std::min<i64>(M, 256 / a.gl * 8);
-  launch(q.device().index(), key_of(STEP, {in}), B * H * up(M, a.rows), 1, 256, &a, sizeof a);
+  // eight rows per lane, four in flight (128 sequences x 32 heads of 128x128: 111 us; with four rows 125, twelve 116, sixteen 112 but
+  // 12 instead of 8 for four sequences)
+  a.rows = std::min<i64>(M, 64 / a.gl * 8);
+  launch(q.device().index(), key_of(STEP, {in}), up(B * H * up(M, a.rows), 4), 1, 256, &a, sizeof a);
   changed(state);
   return y;
 }

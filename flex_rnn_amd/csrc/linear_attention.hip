@@ -1096,16 +1096,18 @@ extern "C" __global__ void __launch_bounds__(1024) la_gate(GateArgs a) {
 
 // ================================================================== one token
 #ifdef KERNEL_STEP
-// S = exp(g) S + v k^T in place, y = scale S q.  Bound by reading and writing the state once: 110 us for 128 sequences x
-// 32 heads of 128x128 in fp32 (4.9 TB/s of the 5.1 that a large copy reaches), 8 us for one sequence, which is the call.  A group of `gl` lanes owns
-// rows of the state, a lane VE neighbouring columns (16 bytes) of each, whose q and k it holds; R rows are in flight at a
-// time.  States that do not allow 16-byte accesses go column by column.
+// S = exp(g) S + v k^T in place, y = scale S q.  Bound by reading and writing the state once: 111 us for 128 sequences x
+// 32 heads of 128x128 in fp32 and 27 us for 256 x 32 heads of 64x64 in bfloat16 (4.9 and 5.0 TB/s of the 5.1 that a large copy
+// reaches), 8 us for one sequence, which is the call.  A wave takes some rows of one head, so that small heads fill a workgroup
+// too (a workgroup per head: 37 us in the second case).  A group of `gl` lanes owns rows of the state, a lane VE neighbouring
+// columns (16 bytes) of each, whose q and k it holds; R rows are in flight at a time.  States that do not allow 16-byte accesses
+// go column by column.
 struct StepArgs {
   Tensor q, k, v;           // st unused
   Gate g;
   States s;
   char* y;                  // [B,H,M]
-  i64 B, H, Hk, M, N, vec, gl, rows;      // rows of the state per workgroup
+  i64 B, H, Hk, M, N, vec, gl, rows;      // rows of the state per wave
   double scale;
 };
 DEV float load_in(const char* p, i64 i) { return load_type(p, i, IN); }
@@ -1139,9 +1141,9 @@ struct Token {              // one head's operands
 };
 
 template <int TYPE>
-DEV void step_rows(const StepArgs& a, const Token& t, int r0, int end, int tid) {
+DEV void step_rows(const StepArgs& a, const Token& t, int r0, int end, int lane) {
   constexpr int VE = TYPE == FP32 ? 4 : 8, SZ = 16 / VE, R = 4;
-  const int gl = (int)a.gl, sub = tid % gl, grp = tid / gl, groups = 256 / gl, N = (int)a.N, n = sub * VE;
+  const int gl = (int)a.gl, sub = lane % gl, grp = lane / gl, groups = 64 / gl, N = (int)a.N, n = sub * VE;
   float q[VE], k[VE];
   for (int i = 0; i < VE; i++) {
     q[i] = n < N ? load_in(t.q, (n + i) * a.q.sn) * t.scale : 0.f;
@@ -1174,8 +1176,8 @@ DEV void step_rows(const StepArgs& a, const Token& t, int r0, int end, int tid) 
   }
 }
 
-DEV void step_columns(const StepArgs& a, const Token& t, int r0, int end, int tid) {
-  const int gl = (int)a.gl, sub = tid % gl, grp = tid / gl, groups = 256 / gl, type = (int)a.s.type;
+DEV void step_columns(const StepArgs& a, const Token& t, int r0, int end, int lane) {
+  const int gl = (int)a.gl, sub = lane % gl, grp = lane / gl, groups = 64 / gl, type = (int)a.s.type;
   for (int m0 = r0; m0 < end; m0 += groups) {
     const int m = m0 + grp;
     float acc = 0.f;
@@ -1194,19 +1196,21 @@ DEV void step_columns(const StepArgs& a, const Token& t, int r0, int end, int ti
 }
 
 extern "C" __global__ void __launch_bounds__(256) la_step(StepArgs a) {
-  const i64 per = (a.M + a.rows - 1) / a.rows, bh = blockIdx.x / per, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hk);
-  const int r0 = (int)(blockIdx.x % per * a.rows), end = r0 + (int)a.rows < a.M ? r0 + (int)a.rows : (int)a.M, tid = threadIdx.x;
+  const u32 unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = (u32)((a.M + a.rows - 1) / a.rows), bh = unit / per;
+  if (bh >= a.B * a.H) return;
+  const i64 b = bh / (u32)a.H, h = bh % (u32)a.H, hk = h / (a.H / a.Hk);
+  const int r0 = (int)(unit % per * a.rows), end = r0 + (int)a.rows < a.M ? r0 + (int)a.rows : (int)a.M, lane = threadIdx.x & 63;
   Token t;
   t.q = a.q.p + (b * a.q.sb + hk * a.q.sh) * ESZ;
   t.k = a.k.p + (b * a.k.sb + hk * a.k.sh) * ESZ;
   t.v = a.v.p + (b * a.v.sb + h * a.v.sh) * ESZ;
   t.s = a.s.p + (b * a.s.sb + h * a.s.sh) * (a.s.type == FP32 ? 4 : 2);
-  t.y = a.y + bh * a.M * ESZ;
+  t.y = a.y + (i64)bh * a.M * ESZ;
   t.e = expf((float)gate_of(a.g, b, h, 0));
   t.scale = (float)a.scale;
-  if (!a.vec) step_columns(a, t, r0, end, tid);
-  else if (a.s.type == FP32) step_rows<FP32>(a, t, r0, end, tid);
-  else if (a.s.type == BF16) step_rows<BF16>(a, t, r0, end, tid);
-  else step_rows<FP16>(a, t, r0, end, tid);
+  if (!a.vec) step_columns(a, t, r0, end, lane);
+  else if (a.s.type == FP32) step_rows<FP32>(a, t, r0, end, lane);
+  else if (a.s.type == BF16) step_rows<BF16>(a, t, r0, end, lane);
+  else step_rows<FP16>(a, t, r0, end, lane);
 }
 #endif
