@@ -150,7 +150,7 @@ struct GateArgs {
   Gate g;
   void* dg;
   const void* lengths;
-  i64 B, T, H, tiles, type;
+  i64 B, T, H, tiles, type, init;
 };
 struct StepArgs {
   Operand q, k, v;
@@ -351,7 +351,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward(const Tens
     dg = at::empty(g.sizes(), g.options());
     const bool per_head = g.dim() == 1;
     const Tensor out = per_head ? at::empty({p.B, p.T, p.H}, p.bytes) : dg;
-    const GateArgs a = {dots.data_ptr(), of_k.dots, inner.data_ptr(), p.g, out.data_ptr(), p.lengths, p.B, p.T, p.H, tiles, type_of(out.scalar_type())};
+    const GateArgs a = {dots.data_ptr(), of_k.dots, inner.data_ptr(), p.g, out.data_ptr(), p.lengths, p.B, p.T, p.H, tiles, type_of(out.scalar_type()), state.has_value()};
     launch(p.device, key_of(GATE, {}), p.B * p.H * up(blocks, 32), 1, 1024, &a, sizeof a);
     if (per_head) slice_sums(p.device, 1, &out, &dg, p.B * p.T);
   } else {

@@ -674,7 +674,8 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) mark[nt] = at[nt * 64];
   };
-  const auto mark_product = [&](int c) {
+  // before the block in front of the border adds what is its own to the state, which it decays by `all`
+  const auto mark_product = [&](int c, float all) {
     if (!counts(c)) return;
     if (!EARLY) mark_ahead(c);
     double s = 0.0;
@@ -683,7 +684,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
       for (int nt = 0; nt < NT; nt++)
         s += (double)(mark[nt][0] * S[nt][0] + mark[nt][1] * S[nt][1]) + (double)(mark[nt][2] * S[nt][2] + mark[nt][3] * S[nt][3]);
     }
-    s = read_lane(scan64(s), 63);
+    s = read_lane(scan64(s), 63) * all;
     if (lane == 0) job.inner[((bh * borders + border_at(c, nreal, nall)) * ntiles + tile) * 4 + w] = s;
   };
 #endif
@@ -956,6 +957,9 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     }
 #endif
 #endif
+#if DOTS
+    if (!back) mark_product(o + 1, all);
+#endif
 #pragma unroll
     for (int n0 = 0; n0 < NT; n0 += KB) {
       Frag<RP> next[KB];
@@ -994,7 +998,6 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
       if (job.dots && t < T) job.dots[((i64)tile * args.B * args.H + bh) * T + t] = (float)(s * job.out_scale);
     }
     if (back) mark_down(block_of(o));
-    else mark_product(o + 1);
 #endif
 #if OUT
     if constexpr (NBUF == 1) write(o, true);
@@ -1040,8 +1043,11 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 
 // ================================================================== gradient of the decays
 #ifdef KERNEL_GATE
-// The gradient of g_t is what token t's step carries over, <X, exp(g_t) S>: at a border between blocks the product that the
-// walks left there, and from one token to the one before it
+// The gradient of g_t is what token t's step carries over, <X, exp(g_t) S>.  For the tokens of a block that ends at a border the
+// walks left the product of X behind it with the state in front of it, decayed through the block; that and
+//     sum over i >= t of q_i.dq_i  +  sum over j < t of k_j.dk_j                (i, j in the block)
+// is the result, sums of terms that exp(g_t) is part of: with a fast decay, or an empty state, nothing larger has to cancel.
+// From the first token of a block to the block before, and from one token to the one before it in blocks without a border,
 //     <X, S> + q_t.dq_t - k_t.dk_t.
 // Summed backwards in 64 bits from the nearest border (at most BORDER blocks away), never over a whole sequence, where what
 // is left of a fast decay would drown in the rounding of what came before.  The block's own share of q.dq and k.dk is the same
@@ -1055,11 +1061,11 @@ struct GateArgs {
   Gate g;
   char* dg;                 // [B,T,H]
   const i64* lengths;
-  i64 B, T, H, tiles, type;
+  i64 B, T, H, tiles, type, init;     // init: whether there is a state in front of the first token
 };
 
 extern "C" __global__ void __launch_bounds__(1024) la_gate(GateArgs a) {
-  __shared__ double sums[32], ends[33];          // a block's; what a border in front of a block (or none: unused) holds
+  __shared__ double sums_q[32], sums_k[32], ends[33];     // a block's; what a border in front of a block (or none: unused) holds
   const int tid = threadIdx.x, lane = tid & 63, blk = tid / L;
   const int T = (int)a.T, nall = (T + L - 1) / L, groups = (nall + 31) / 32;
   const i64 bh = blockIdx.x / groups, b = bh / a.H, h = bh % a.H, BH = a.B * a.H;
@@ -1077,18 +1083,31 @@ extern "C" __global__ void __launch_bounds__(1024) la_gate(GateArgs a) {
   }
   // half a wave holds a block back to front
   const int t = c * L + L - 1 - (tid & (L - 1));
-  double d = 0.0;
+  double dq = 0.0, dk = 0.0;
   if (t < len)
-    for (i64 k = 0; k < a.tiles; k++) d += (double)a.dots_q[(k * BH + bh) * T + t] - (double)a.dots_k[(k * BH + bh) * T + t];
-  d = scan32(d);
-  if ((lane & (L - 1)) == L - 1) sums[blk] = d;
+    for (i64 k = 0; k < a.tiles; k++) {
+      dq += (double)a.dots_q[(k * BH + bh) * T + t];
+      dk += (double)a.dots_k[(k * BH + bh) * T + t];
+    }
+  dq = scan32(dq);
+  dk = scan32(dk);
+  if ((lane & (L - 1)) == L - 1) {
+    sums_q[blk] = dq;
+    sums_k[blk] = dk;
+  }
   __syncthreads();
   if (t >= T) return;
   double x = 0.0;
-  if (t < len) {
+  if (t < len && (t > 0 || a.init)) {
+    x = dq;
     int at = blk + 1;
-    for (; !is_border(c0 + at, nreal); at++) x += sums[at];              // (32 blocks on is a border)
-    x += ends[at] + d;
+    if (is_border(c0 + at, nreal)) x += sums_k[blk] - dk;
+    else {
+      x -= dk;
+      for (; !is_border(c0 + at + 1, nreal); at++) x += sums_q[at] - sums_k[at];       // (32 blocks on is a border)
+      x += sums_q[at++];
+    }
+    x += ends[at];
   }
   store_type(a.dg, (b * a.T + t) * a.H + h, (int)a.type, (float)x);
 }

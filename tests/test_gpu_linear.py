@@ -199,6 +199,24 @@ def test_decays_at_their_ends(value):
         lc.assert_within(x, w, b, f'gate {value}')
 
 
+@pytest.mark.parametrize('dtype', [BF16, FP16, FP32], ids=str)
+@pytest.mark.parametrize('T', [1, 33, 300])
+def test_gradient_of_decays_that_leave_little(dtype, T):
+    """With g near -20, g's gradient is e^-20 of the products that it is made of, and zero for the first token after an empty
+    state.  Every term that is summed has that factor, so the result keeps fp32's precision relative to itself: 2^-24 for each
+    of at most M + N + 64 terms in a chain of sums, M = N = 32, in the 2-norm (below 2e-5)."""
+    print(f'case fast decays {dtype} {T}', flush=True)
+    for state in (FP32, None):
+        inputs, _ = lc.make(dtype, 2, T, 2, 1, 32, 32, state=state)
+        inputs[3] = inputs[3] - 20
+        dy, ds = lc.cotangents(inputs)
+        want = lc.run64(inputs, None, 1.0, dy, ds)[2][3]
+        got = _gradients(_gpu(inputs), None, 1.0, dy.cuda(), ds.cuda())[5].cpu().double()
+        assert float((got - want).norm()) <= 128 * 2.0 ** -24 * 2 * float(want.norm()), state
+        if state is None:
+            assert bool((got[:, 0] == 0).all())
+
+
 def test_strides_and_broadcast_inputs():
     print('case strides', flush=True)
     B, T, H, M, N = 2, 75, 2, 64, 64
