@@ -38,9 +38,9 @@
 //   - the decayed products P = exp(G_i - G_j) q_i.k_j are rounded to RP parts, and to two with bfloat16: each stands for a whole
 //     row of v, so its rounding would not average out (the second part is 2.5 % of a block's time, and y as far from the exact
 //     result as its own rounding, 1.7e-3 of its norm, where a fast decay leaves little of the state);
-//   - the state, where it is a factor, is rounded to RP parts: one rounding of independent numbers to the inputs' own precision,
-//     as large as the one of the result that they are summed into (2.3e-3 where the state dominates; a second part in bfloat16
-//     takes 5 to 10 % longer); to three where the product is part of g's gradient, whose type may be float32 with 16-bit inputs;
+//   - the state, where it is a factor, is rounded to as many parts as P: with one part in bfloat16 an element of y whose terms
+//     cancel was off by up to ten times its own rounding (2.2e-3 of y's norm for a long document, against 1.7e-3, for 2.5 to 6.5 %
+//     of the time); to three where the product is part of g's gradient, whose type may be float32 with 16-bit inputs;
 //   - the decayed v that enters the state has three parts: the state is an fp32 result even where the inputs are not.
 // The state itself stays in fp32 accumulators for the whole sequence.
 //
@@ -173,8 +173,7 @@ DEV void mul_each(const Frag<PA>* a, const Frag<PB>& b, f4* c) {
     }
 }
 constexpr int RAW = RP == 1 ? 0 : 2;           // both factors exact
-constexpr int CALC = RP - 1;                   // one factor rounded to RP parts
-constexpr int PP = RP == 1 ? 2 : RP;           // parts of the decayed products
+constexpr int PP = RP == 1 ? 2 : RP;           // parts of the decayed products, and of the state as a factor
 
 // ------------------------------------------------------------------ LDS tiles
 constexpr int stride_down(int w) { return w + 16; }       // for tiles read down their columns
@@ -567,11 +566,10 @@ struct BlockArgs {
 };
 
 constexpr int NT = W / 16, LT = 2;
-constexpr int SPARTS = DOTS ? 3 : RP, SLIM = DOTS ? 2 : CALC;
+constexpr int SPARTS = DOTS ? 3 : PP, SLIM = SPARTS - 1;
 constexpr int QB = RP == 1 ? (W < 128 ? W / 32 : 4) : RP == 2 ? 2 : 1;       // operands read ahead: what 32 registers hold
 constexpr int KB = RP == 1 ? 4 : RP == 2 ? 2 : 2;
 constexpr bool EARLY = RP == 1 && W <= 128;                                  // registers for what dots need, ahead of its use
-constexpr bool AHEAD = OUT && RP == 1 && SPARTS == 1 && W <= 128;            // the state as a factor: what 16 registers hold
 constexpr int SQ = stride_along(W), SK = stride_down(W), SV = stride_down(64), SX = stride_along(64), SP = stride_along(L);
 constexpr int AT_K = OUT ? RP * L * SQ : 0, AT_V = AT_K + RP * L * SK, AT_X = AT_V + RP * L * SV, STAGE = AT_X + (DOTS ? RP * L * SX : 0);
 
@@ -877,9 +875,8 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 #if DOTS
     if (EARLY && !back) mark_ahead(o + 1);
 #endif
-    // What a block needs is read from LDS well ahead of its use, and what can be computed without it - the state as a
-    // factor, the decayed state, the parts of the decayed v - fills the wait.  (The compiler's own order within that: scheduling
-    // fences that kept this one made a block 5 % slower.)
+    // What a block needs is read from LDS well ahead of its use, and the parts of the decayed v fill the wait.  (The
+    // compiler's own order within that: scheduling fences that kept this one made a block 5 % slower.)
     const float all = D.from_start[L - 1];
     const f4 to0 = *(const f4*)(D.to_end + 4 * g), to1 = *(const f4*)(D.to_end + 16 + 4 * g);
 #if OUT
@@ -897,13 +894,6 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     for (int x = 0; x < QB; x++)
 #pragma unroll
       for (int i = 0; i < LT; i++) qf[x][i] = along<SQ>(Q, 16 * i + p, 32 * x, g);
-    Frag<SPARTS> sf[AHEAD ? NT / 2 : 1];
-    if constexpr (AHEAD) {
-#pragma unroll
-      for (int x = 0; x < NT / 2; x++) sf[x] = state_frag(S, x);
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) S[nt] *= all;
-    }
 #else
     const Frag<RP> vf = down<SV>(V, 0, 16 * w, lane);
 #endif
@@ -928,7 +918,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
     for (int k0 = 0; k0 < W / 32; k0 += QB) {
 #pragma unroll
       for (int ks = 0; ks < QB; ks++) {
-        const Frag<SPARTS> s = AHEAD ? sf[AHEAD ? k0 + ks : 0] : state_frag(S, k0 + ks);
+        const Frag<SPARTS> s = state_frag(S, k0 + ks);
 #pragma unroll
         for (int i = 0; i < LT; i++) y[i] = mul<SLIM>(s, qf[ks][i], y[i]);
       }
@@ -967,10 +957,8 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 #pragma unroll
         for (int x = 0; x < KB; x++) next[x] = down<SK>(K, 0, 16 * (n0 + KB + x), lane);
       }
-      if constexpr (!AHEAD) {
 #pragma unroll
-        for (int x = 0; x < KB; x++) S[n0 + x] *= all;
-      }
+      for (int x = 0; x < KB; x++) S[n0 + x] *= all;
       mul_each<KB, 2>(kf, vd, S + n0);
       if (n0 + KB < NT) {
 #pragma unroll

@@ -645,3 +645,37 @@ def test_examples_command(op):
     a = warm.EXAMPLE_ARGS
     examples.main(['--op', op, '--chunked', '--head-norm', '--check-flex', '--batchsz', str(a['B']), '--seqlen', str(a['T']),
                    '--modeldim', str(a['D']), '--headsz', str(a['C'])])
+
+
+# ------------------------------------------------------------------ linear attention: precision and borders
+# What a result's own rounding (u = half a step of its type) does not explain: the decayed products and the state as a factor
+# keep 2^-15 of themselves (two bfloat16 parts: what truncation to 8 bits leaves is at most 2^-7, its rounding 2^-8 of that),
+# and with float16 a product leaves out that of the two lower parts (at most 2^-7 each, 2^-14); the exponentials and the three
+# parts of what enters the state 2^-20 in all; sums as in linear_cases.
+REST = {BF16: 2.0 ** -15, FP16: 2.0 ** -13}
+
+
+@pytest.mark.parametrize('case', [
+    (BF16, 1, 300, 2, 2, 128, 128, dict(g='head')),
+    (BF16, 1, 300, 2, 2, 128, 128, {}),
+    (BF16, 2, 200, 4, 1, 64, 64, dict(g='head')),
+    (BF16, 1, 130, 1, 1, 256, 256, dict(g='head')),
+    (BF16, 1, 200, 2, 1, 33, 100, dict(g='head')),
+    (FP16, 1, 300, 2, 2, 64, 128, dict(g='head')),
+], ids=str)
+def test_nothing_but_the_result_is_rounded_to_the_inputs_type(case):
+    *shape, opts = case
+    print(f'case rounding {case}', flush=True)
+    dtype = shape[0]
+    inputs, _ = lc.make(*shape, **opts)
+    dy, ds = lc.cotangents(inputs)
+    y, _, grads = lc.run64(inputs, None, 0.7, dy, ds)
+    ay, _, agrads = lc.run64(lc.absolute(inputs), None, 0.7, dy.abs(), ds.abs())
+    u, rest = lc.HALF_STEP[dtype], REST[dtype] + 2.0 ** -20 + (shape[2] + shape[5] + shape[6]) * 2.0 ** -24
+    got = _gradients(_gpu(inputs), None, 0.7, dy.cuda(), ds.cuda())
+    q, k, v, g, s = _gpu(inputs)
+    v.requires_grad_()
+    dv, = th.autograd.grad(F.linear_attention(q, k, v, g, s, scale=0.7), v, (dy.cuda(), ds.cuda()))
+    for name, x, w, a in (('y', got[0], y, ay), ('dq', got[2], grads[0], agrads[0]), ('dk', got[3], grads[1], agrads[1]),
+                          ('dv', got[4], grads[2], agrads[2]), ('dv alone', dv, grads[2], agrads[2])):
+        lc.assert_within(x, w, u * w.abs() + (1 + u) * rest * a, name)
