@@ -553,6 +553,14 @@ struct Once : torch::autograd::Function<Once> {
     TORCH_CHECK(false, "linear_attention and layer_norm can be differentiated once");
   }
 };
+// A forward-mode derivative of an input would be lost without a word.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const optional<Tensor>& t) { return t && has_tangent(*t); }
+template <class... Inputs>
+void refuse_tangents(const char* what, const Inputs&... inputs) {
+  TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !(has_tangent(inputs) || ...), what,
+              " has no forward-mode derivative (an input has a tangent)");
+}
 // the first of `inputs` that asks for a gradient
 Tensor asking(std::initializer_list<optional<Tensor>> inputs) {
   if (at::GradMode::is_enabled())
@@ -612,6 +620,7 @@ struct Attention : torch::autograd::Function<Attention> {
 
 std::tuple<Tensor, Tensor> attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const optional<Tensor>& state,
                                               const optional<Tensor>& lengths, double scale) {
+  refuse_tangents("linear_attention", q, k, v, g, state);
   if (at::GradMode::is_enabled() && (wanted(q) || wanted(k) || wanted(v) || wanted(g) || wanted(state))) {
     const auto r = Attention::apply(q, k, v, g, state, lengths, scale);
     return {r[0], r[1]};
@@ -624,6 +633,7 @@ std::tuple<Tensor, Tensor> attention_autograd(const Tensor& q, const Tensor& k, 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
                                                                                const optional<Tensor>& state, const optional<Tensor>& lengths, const Tensor& dy,
                                                                                const optional<Tensor>& dstate, double scale, bool need_g, bool need_state) {
+  refuse_tangents("linear_attention's gradient", q, k, v, g, state, dy, dstate);
   static const auto call = op<decltype(attention_backward)>("flex_rnn::linear_attention_backward");
   std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> r;
   {
@@ -633,6 +643,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward_autograd(c
   const Tensor t = asking({q, k, v, g, state, dy, dstate});
   if (!t.defined()) return r;
   return {Once::apply(std::get<0>(r), t), Once::apply(std::get<1>(r), t), Once::apply(std::get<2>(r), t), Once::apply(std::get<3>(r), t), Once::apply(std::get<4>(r), t)};
+}
+
+Tensor attention_step_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& state, double scale) {
+  refuse_tangents("linear_attention_step", q, k, v, g, state);
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(wanted(q) || wanted(k) || wanted(v) || wanted(g) || wanted(state)), "linear_attention_step updates the state in place and cannot be differentiated");
+  at::AutoDispatchBelowAutograd below;
+  static const auto call = op<decltype(attention_step)>("flex_rnn::linear_attention_step");
+  return call.call(q, k, v, g, state, scale);
 }
 
 struct Norm : torch::autograd::Function<Norm> {
@@ -658,6 +676,7 @@ struct Norm : torch::autograd::Function<Norm> {
 };
 
 Tensor norm_autograd(const Tensor& x, const optional<Tensor>& w, const optional<Tensor>& b, double eps) {
+  refuse_tangents("layer_norm", x, w, b);
   if (at::GradMode::is_enabled() && (wanted(x) || wanted(w) || wanted(b))) return Norm::apply(x, w, b, eps);
   at::AutoDispatchBelowAutograd below;
   static const auto call = op<decltype(norm)>("flex_rnn::layer_norm");
@@ -666,6 +685,7 @@ Tensor norm_autograd(const Tensor& x, const optional<Tensor>& w, const optional<
 
 std::tuple<Tensor, Tensor, Tensor> norm_backward_autograd(const Tensor& x, const optional<Tensor>& w, const optional<Tensor>& b, const Tensor& dy, double eps,
                                                           bool need_w, bool need_b) {
+  refuse_tangents("layer_norm's gradient", x, w, b, dy);
   static const auto call = op<decltype(norm_backward)>("flex_rnn::layer_norm_backward");
   std::tuple<Tensor, Tensor, Tensor> r;
   {
@@ -705,6 +725,7 @@ TORCH_LIBRARY_IMPL(flex_rnn, Meta, m) {
 TORCH_LIBRARY_IMPL(flex_rnn, Autograd, m) {
   m.impl("linear_attention", attention_autograd);
   m.impl("linear_attention_backward", attention_backward_autograd);
+  m.impl("linear_attention_step", attention_step_autograd);
   m.impl("layer_norm", norm_autograd);
   m.impl("layer_norm_backward", norm_backward_autograd);
 }

@@ -74,7 +74,8 @@ def linear_attention(q: th.Tensor, k: th.Tensor, v: th.Tensor, g: th.Tensor, sta
     lengths [B], int64 or int32: sequence b ends after `lengths[b]` tokens (clamped to 0..T); what is behind is not
             looked at, its `y` and gradients are zero, and the final state is the one after the last real token
 
-    Any strides.  Sums and the state are fp32.  Differentiable once in q, k, v, g and state; gradients are deterministic.
+    Any strides.  Sums and the state are fp32.  Differentiable once, backwards, in q, k, v, g and state (a forward-mode tangent is
+    refused); gradients are deterministic.
     """
     _check(q, k, v, g, state, ('B', 'T'), 'linear_attention')
     _check_device('linear_attention', q, k, v, g, state, lengths)
@@ -89,7 +90,8 @@ def linear_attention_step(q: th.Tensor, k: th.Tensor, v: th.Tensor, g: th.Tensor
     """One token of `linear_attention` for decoding: `state` [B,H,M,N] is updated in place, y [B,H,M] is returned.
 
     q, k [B,Hk,N], v [B,H,M], g [B,H] or [H]; types as there.  Any strides, except that no two elements of the state may
-    share memory, nor may one with another argument.  Not differentiable: with T = 1, `linear_attention` is.
+    share memory, nor may one with another argument.  Not differentiable (inputs that want gradients or have a
+    tangent are refused): with T = 1, `linear_attention` is.
     """
     _check(q, k, v, g, state, ('B',), 'linear_attention_step')
     _check_device('linear_attention_step', q, k, v, g, state)

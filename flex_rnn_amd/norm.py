@@ -46,8 +46,8 @@ def layer_norm(x: th.Tensor, weight: Optional[th.Tensor] = None, bias: Optional[
             fold into one, or whose columns are not next to each other, is copied first)
     weight, bias  [C], or [H,C] with x [..., H, C]; float32 or the type of x; None: one, zero
 
-    Sums are fp32 (mean first, then squares of the differences).  Differentiable once in x, weight and bias; gradients are
-    deterministic.
+    Sums are fp32 (mean first, then squares of the differences).  Differentiable once, backwards, in x, weight and
+    bias (a forward-mode tangent is refused); gradients are deterministic.
     """
     _check(x, weight, bias)
     weight, bias = (p if p is None or p.is_contiguous() else p.contiguous() for p in (weight, bias))

@@ -230,3 +230,48 @@ def test_missing_library_says_how_to_build_it(monkeypatch):
     monkeypatch.setattr(handwritten, 'OPS_PATH', '/nowhere/libfrnn_ops.so')
     with pytest.raises(runtime.RuntimeError_, match='have not been built'):
         handwritten.op('layer_norm')
+
+
+def _tangent_calls():
+    m, s, g, c = _meta(1, 4, 2, 8, dtype=th.float32), _meta(1, 2, 8, 8, dtype=th.float32), _meta(2, dtype=th.float32), _meta(8, dtype=th.float32)
+    t = m[:, 0]
+    o = th.ops.flex_rnn
+    return {
+        'linear_attention': (lambda q, k, v, g, s: F.linear_attention(q, k, v, g, s), [m, m, m, g, s]),
+        'linear_attention_step': (lambda q, k, v, g, s: F.linear_attention_step(q, k, v, g, s), [t, t, t, g, s]),
+        'layer_norm': (lambda x, w, b: F.layer_norm(x, w, b), [m, c, c]),
+        'linear_attention backward': (lambda q, k, v, g, s, d, e: o.linear_attention_backward(q, k, v, g, s, None, d, e, 1.0, True, True), [m, m, m, g, s, m, s]),
+        'layer_norm backward': (lambda x, w, b, d: o.layer_norm_backward(x, w, b, d, 1e-5, True, True), [m, c, c, m]),
+    }
+
+
+@pytest.mark.parametrize('name', list(_tangent_calls()))
+def test_forward_mode_derivatives_are_refused(name):
+    """A tangent of any argument would be lost without a word: it is an error, with and without a graph being recorded."""
+    import torch.autograd.forward_ad as fw
+    f, args = _tangent_calls()[name]
+    for i in range(len(args)):
+        for record in (True, False):
+            with fw.dual_level(), th.set_grad_enabled(record):
+                xs = [a.clone() for a in args]
+                xs[i] = fw.make_dual(xs[i], th.ones_like(xs[i]))
+                with pytest.raises(RuntimeError, match='forward-mode'):
+                    f(*xs)
+    with fw.dual_level():
+        f(*[a.clone() for a in args])
+        xs = [fw.make_dual(a.clone(), th.ones_like(a)) for a in args]
+        with fw._set_fwd_grad_enabled(False):
+            f(*xs)
+    xs = tuple(a.clone() for a in args)
+    with pytest.raises(RuntimeError, match='forward-mode'):
+        th.func.jvp(f, xs, tuple(th.ones_like(x) for x in xs))
+
+
+def test_a_step_of_inputs_that_want_gradients_is_refused_below_the_public_function_too():
+    t, s, g = _meta(1, 2, 8, dtype=th.float32), _meta(1, 2, 8, 8, dtype=th.float32), _meta(2, dtype=th.float32)
+    call = th.ops.flex_rnn.linear_attention_step
+    with pytest.raises(RuntimeError, match='cannot be differentiated'):
+        call(t.clone().requires_grad_(), t, t, g, s, 1.0)
+    with th.no_grad():
+        call(t.clone().requires_grad_(), t, t, g, s, 1.0)
+    call(t, t, t, g, s, 1.0)
