@@ -3,10 +3,15 @@
 The operators are C++: they allocate, pack argument blocks and launch through the C ABI of include/frnn_rt.h.  When one needs
 a kernel for the first time on a device it asks `_load` here by number; the kernel is then compiled with its constants into the
 same on-disk cache as the generated ones (or found there) and loaded.
+
+Operators and kernels share argument blocks, so they have to come from the same sources: these are read once, at import, the
+library's file name holds their hash (and PyTorch's version, whose C++ interface it uses), and another library is not looked at.
 """
 from __future__ import annotations
 
 import ctypes
+import glob
+import hashlib
 import os
 import subprocess
 import threading
@@ -19,11 +24,9 @@ from . import runtime
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _CSRC = os.path.join(_HERE, 'csrc')
-OPS_PATH = os.path.join(_HERE, 'libfrnn_ops.so')
 DTYPES = {th.bfloat16: 0, th.float16: 1, th.float32: 2}      # the kernels' type codes
 
 _lock = threading.Lock()
-_sources: Dict[str, str] = {}
 _modules: list = []             # loaded code objects stay as long as the process
 _lib = None
 
@@ -32,6 +35,28 @@ def require(ok, message: str):
     """Argument checks raise what the compiled operators' own checks raise (and also do so under `python -O`)."""
     if not ok:
         raise AssertionError(message)
+
+
+def sources() -> Dict[str, str]:
+    """File name -> text of everything that operators and kernels are made of."""
+    out = {}
+    for path in sorted([os.path.join(_CSRC, 'frnn_ops.cpp'), os.path.join(os.path.dirname(_HERE), 'include', 'frnn_rt.h'), os.path.abspath(__file__),
+                        *(os.path.join(_CSRC, f'{n}.hip') for n in ('layer_norm', 'linear_attention', 'slice_sum'))]):
+        if os.path.isfile(path):
+            with open(path) as f:
+                out[os.path.basename(path)] = f.read()
+    return out
+
+
+def library_name(texts: Dict[str, str], torch_version: str) -> str:
+    h = hashlib.sha256(torch_version.encode())
+    for name in sorted(texts):
+        h.update(f'\0{name}\0'.encode() + texts[name].encode())
+    return f'libfrnn_ops.{h.hexdigest()[:16]}.so'
+
+
+_sources = sources()
+OPS_PATH = os.path.join(_HERE, library_name(_sources, th.__version__))
 
 
 # ------------------------------------------------------------------ kernels by number
@@ -86,10 +111,6 @@ def builds():
 
 def build(source: str, name: str, defines=(), force: bool = False) -> str:
     """Path of the code object of kernel `name` from csrc/`source`, compiled with `defines` on a cache miss."""
-    with _lock:
-        if source not in _sources:
-            with open(os.path.join(_CSRC, source)) as f:
-                _sources[source] = f.read()
     opts = ' '.join([runtime.EMITTER_OPTS] + [f'-D{k}={v}' for k, v in defines])
     return runtime.compile_kernel(name, _sources[source], opts=opts, force=force)
 
@@ -124,7 +145,8 @@ _loader = _LOADER(_load)
 
 # ------------------------------------------------------------------ the operators' library
 def build_library(verbose: bool = False) -> str:
-    """Compiles csrc/frnn_ops.cpp -> flex_rnn_amd/libfrnn_ops.so (host code only, against PyTorch's headers)."""
+    """Compiles csrc/frnn_ops.cpp -> flex_rnn_amd/libfrnn_ops.<hash>.so (host code only, against PyTorch's headers) and removes
+    those of other sources."""
     root = os.path.dirname(th.__file__)
     tmp = OPS_PATH + f'.tmp{os.getpid()}'
     rocm = os.environ.get('ROCM_PATH', '/opt/rocm')
@@ -137,6 +159,9 @@ def build_library(verbose: bool = False) -> str:
         print(' '.join(cmd))
     subprocess.run(cmd, check=True)
     os.replace(tmp, OPS_PATH)
+    for old in glob.glob(os.path.join(_HERE, 'libfrnn_ops*.so')):
+        if old != OPS_PATH:
+            os.remove(old)
     return OPS_PATH
 
 
@@ -146,23 +171,30 @@ def load() -> ctypes.CDLL:
     if _lib is None:
         with _lock:
             if _lib is None:
+                how = 'Run `python -c "import __graft_entry__ as g; g.build()"`.'
                 if not os.path.isfile(OPS_PATH):
-                    raise runtime.RuntimeError_(f'{OPS_PATH} is missing: the operators have not been built. '
-                                                'Run `python -c "import __graft_entry__ as g; g.build()"`.')
-                runtime.lib()                       # (the kernels' runtime, which the operators link against)
-                th.ops.load_library(OPS_PATH)
-                lib = ctypes.CDLL(OPS_PATH)
-                lib.frnn_ops_set_loader.argtypes = [_LOADER]
-                lib.frnn_ops_set_loader.restype = None
-                lib.frnn_ops_set_loader(_loader)
+                    raise runtime.RuntimeError_(f'{OPS_PATH} is missing: the operators have not been built from these sources. {how}')
+                try:
+                    runtime.lib()                   # (the kernels' runtime, which the operators link against)
+                    th.ops.load_library(OPS_PATH)
+                    lib = ctypes.CDLL(OPS_PATH)
+                    lib.frnn_ops_set_loader.argtypes = [_LOADER]
+                    lib.frnn_ops_set_loader.restype = None
+                    lib.frnn_ops_set_loader(_loader)
+                except (OSError, AttributeError) as e:
+                    raise runtime.RuntimeError_(f'{OPS_PATH} cannot be loaded ({e}). {how}') from e
                 _lib = lib
     return _lib
 
 
 def load_if_built():
-    """At import: traced and compiled code finds the operators registered; without the library the first call says so."""
+    """At import: traced and compiled code finds the operators registered.  Without the library, or with one that cannot be loaded,
+    the rest of the package works, and the first call says what to do."""
     if os.path.isfile(OPS_PATH) and os.path.isfile(runtime.LIB_PATH):
-        load()
+        try:
+            load()
+        except runtime.RuntimeError_:
+            pass
 
 
 def op(name: str):

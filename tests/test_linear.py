@@ -275,3 +275,31 @@ def test_a_step_of_inputs_that_want_gradients_is_refused_below_the_public_functi
     with th.no_grad():
         call(t.clone().requires_grad_(), t, t, g, s, 1.0)
     call(t, t, t, g, s, 1.0)
+
+
+def test_a_library_that_cannot_be_loaded_leaves_the_package_usable(monkeypatch, tmp_path):
+    """A truncated file, or one linked against another PyTorch: the import goes on, the first call says what to do."""
+    bad = tmp_path / 'libfrnn_ops.so'
+    bad.write_bytes(b'\x7fELF not a library')
+    monkeypatch.setattr(handwritten, '_lib', None)
+    monkeypatch.setattr(handwritten, 'OPS_PATH', str(bad))
+    handwritten.load_if_built()
+    assert handwritten._lib is None
+    with pytest.raises(runtime.RuntimeError_, match=r'cannot be loaded.*build\(\)'):
+        F.layer_norm(_meta(2, 8))
+
+
+def test_a_library_from_other_sources_is_not_taken():
+    """The host code shares argument blocks with the kernels: its file's name stands for both, and for PyTorch."""
+    name = handwritten.library_name
+    sources = handwritten.sources()
+    csrc = os.path.join(os.path.dirname(handwritten.__file__), 'csrc')
+    used = {s for s, _, _ in handwritten.builds()} | {'frnn_ops.cpp'}
+    for f in used:
+        with open(os.path.join(csrc, f)) as h:
+            assert sources[f] == h.read()
+    assert 'frnn_rt.h' in sources and 'handwritten.py' in sources
+    assert handwritten.OPS_PATH == os.path.join(os.path.dirname(handwritten.__file__), name(sources, th.__version__))
+    assert name(sources, 'another PyTorch') != name(sources, th.__version__)
+    for f in sources:
+        assert name({**sources, f: sources[f] + ' '}, th.__version__) != name(sources, th.__version__)
