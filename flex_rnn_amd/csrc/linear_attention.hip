@@ -838,11 +838,36 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
   };
   f4 y[LT];                                      // column i = 16 it + p, rows cw + 4 g + r
   Frag<RP> vf = {};
+  bool odd = false;                              // whether a lane of this wave has an infinity or a NaN in it
   const auto own_share = [&](int n) {            // of block n, whose P lies in LDS
     const u16* own = P[n % NBUF];
     const Frag<PP> p0 = along<SP, PP>(own, p, 0, g), p1 = along<SP, PP>(own, 16 + p, 0, g);
+    int from = L;                                // row of the first infinity or NaN in column cw + p
+    if (odd) {
+      // The zeros of P above its diagonal must not meet them (an earlier token would be NaN): they come out of the factor, and
+      // their column is NaN from the first of them on, as the state is from the next block on.  Looking for them takes 1 to 2 %
+      // of the time; all of this stands here because a branch in the middle of a block cost 50 registers.
+      float x[8];
+      frag_values(vf, x);
+      for (int e = 0; e < 8; e++) {
+        if (__builtin_isfinite(x[e])) continue;
+        const int row = (e / 4) * 16 + 4 * g + e % 4;
+        from = row < from ? row : from;
+        for (int q = 0; q < RP; q++) vf.d[q][e / 2] &= e % 2 ? 0xffffu : 0xffff0000u;
+      }
+      for (int far = 16; far < 64; far *= 2) {
+        const int other = __shfl_xor(from, far);
+        from = other < from ? other : from;
+      }
+    }
     y[0] = mul<PP - 1>(vf, p0, y[0]);
     y[1] = mul<PP - 1>(vf, p1, y[1]);
+    if (odd) {
+      for (int r = 0; r < 4; r++) {
+        const int row = __shfl(from, 4 * g + r);
+        for (int i = 0; i < LT; i++) y[i][r] = 16 * i + p < row ? y[i][r] : __builtin_nanf("");
+      }
+    }
   };
   const auto write = [&](int o, bool any) {
     const Buffer into = buffer_at(to);
@@ -899,6 +924,10 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 #endif
     float vx[8];
     frag_values(vf, vx);
+#if OUT
+    const float sum = (fabsf(vx[0]) + fabsf(vx[1])) + (fabsf(vx[2]) + fabsf(vx[3])) + ((fabsf(vx[4]) + fabsf(vx[5])) + (fabsf(vx[6]) + fabsf(vx[7])));
+    odd = __any(!__builtin_isfinite(sum));
+#endif
 #pragma unroll
     for (int r = 0; r < 4; r++) {
       vx[r] *= to0[r];

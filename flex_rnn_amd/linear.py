@@ -75,7 +75,8 @@ def linear_attention(q: th.Tensor, k: th.Tensor, v: th.Tensor, g: th.Tensor, sta
             looked at, its `y` and gradients are zero, and the final state is the one after the last real token
 
     Any strides.  Sums and the state are fp32.  Differentiable once, backwards, in q, k, v, g and state (a forward-mode tangent is
-    refused); gradients are deterministic.
+    refused); gradients are deterministic.  An infinity or NaN in q, k, v or a result's gradient leaves NaN in what it is a factor
+    of, and nothing else (but in the gradient of g: up to 255 tokens in front of it, too).
     """
     _check(q, k, v, g, state, ('B', 'T'), 'linear_attention')
     _check_device('linear_attention', q, k, v, g, state, lengths)

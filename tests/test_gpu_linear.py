@@ -679,3 +679,62 @@ def test_nothing_but_the_result_is_rounded_to_the_inputs_type(case):
     for name, x, w, a in (('y', got[0], y, ay), ('dq', got[2], grads[0], agrads[0]), ('dk', got[3], grads[1], agrads[1]),
                           ('dv', got[4], grads[2], agrads[2]), ('dv alone', dv, grads[2], agrads[2])):
         lc.assert_within(x, w, u * w.abs() + (1 + u) * rest * a, name)
+
+
+@pytest.mark.parametrize('shape', [(BF16, 2, 70, 4, 2, 64, 64), (BF16, 1, 100, 2, 2, 128, 128), (BF16, 1, 70, 2, 2, 256, 200), (FP16, 1, 70, 2, 1, 72, 33),
+                                   (FP32, 1, 70, 2, 2, 40, 64), (FP32, 1, 40, 2, 2, 128, 128)], ids=str)
+@pytest.mark.parametrize('bad', [math.nan, math.inf, -math.inf])
+def test_a_number_that_is_not_finite_reaches_no_earlier_token(shape, bad):
+    """One element of one token, in the middle of a block: where the definition does not read it, every bit is as without it, and
+    where it does the result is not finite.  (g's gradient sums over tokens on both sides of it, and is left out.)"""
+    print(f'case not finite {shape} {bad}', flush=True)
+    T, H, Hk = shape[2], shape[3], shape[4]
+    inputs, _ = lc.make(*shape)
+    dy, ds = lc.cotangents(inputs)
+    clean = [x.cpu() for x in _gradients(_gpu(inputs), None, 1.0, dy.cuda(), ds.cuda())]
+    names = ('y', 'state', 'dq', 'dk', 'dv')
+    at, group = min(45, T - 2), H // Hk
+    share = slice(0, group)                       # the heads of v that read the first head of q and k
+    for which in ('q', 'k', 'v', 'dy'):
+        xs, d = [x.clone() for x in inputs], dy.clone()
+        (d if which == 'dy' else xs['qkv'.index(which)])[0, at, 0, 3] = bad
+        got = dict(zip(names, [x.cpu() for x in _gradients(_gpu(xs), None, 1.0, d.cuda(), ds.cuda())]))
+        # what reads the element (batch 0): all of these are sums with it as a factor of one term or more
+        reach = {n: th.zeros_like(x, dtype=th.bool) for n, x in zip(names, clean)}
+        after, before, heads = slice(at, T), slice(0, at + 1), share if which in 'qk' else slice(0, 1)
+        if which == 'q':
+            reach['y'][0, at, heads] = True
+            reach['dk'][0, before, 0, 3] = True
+            reach['dv'][0, before, heads] = True
+        elif which == 'k':
+            reach['y'][0, after, heads] = True
+            reach['state'][0, heads, :, 3] = True
+            reach['dq'][0, after, 0, 3] = True
+            reach['dv'][0, at, heads] = True
+        elif which == 'v':
+            reach['y'][0, after, 0, 3] = True
+            reach['state'][0, 0, 3] = True
+            reach['dq'][0, after, 0] = True
+            reach['dk'][0, at, 0] = True
+        else:
+            reach['dq'][0, at, 0] = True
+            reach['dk'][0, before, 0] = True
+            reach['dv'][0, before, 0, 3] = True
+        for n, x in zip(names, clean):
+            keep = ~reach[n]
+            assert th.equal(got[n][keep], x[keep]), (which, n)
+            assert not bool(th.isfinite(got[n][reach[n]]).any()), (which, n)
+
+
+def test_how_far_a_number_that_is_not_finite_reaches_in_the_gradient_of_the_decays():
+    """g's gradient is summed between borders, 256 tokens at most: in front of a spoiled v (or k) that far, behind a spoiled dy
+    (or q) not at all; other heads not at all."""
+    print('case not finite, gradient of g', flush=True)
+    inputs, _ = lc.make(BF16, 1, 600, 2, 2, 64, 64)
+    dy, ds = lc.cotangents(inputs)
+    clean = _gradients(_gpu(inputs), None, 1.0, dy.cuda(), ds.cuda())[5]
+    for which, keep in (('k', slice(0, 500 - 255)), ('v', slice(0, 500 - 255)), ('q', slice(501, 600)), ('dy', slice(501, 600))):
+        xs, d = [x.clone() for x in inputs], dy.clone()
+        (d if which == 'dy' else xs['qkv'.index(which)])[0, 500, 0, 3] = math.nan
+        got = _gradients(_gpu(xs), None, 1.0, d.cuda(), ds.cuda())[5]
+        assert th.equal(got[:, keep, 0], clean[:, keep, 0]) and th.equal(got[:, :, 1], clean[:, :, 1]), which
