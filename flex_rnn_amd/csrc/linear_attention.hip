@@ -826,7 +826,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
       double row = 0.0;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const double s = (double)(c[r] * a[r]);
+        const double s = pj + r <= pi ? (double)(c[r] * a[r]) : 0.0;       // (a need not be finite where c is zero)
         row += s;
         const double col = row_of_16(s);
         if (p == 15) of_cols[o % NBUF][it][pj + r] = col;
