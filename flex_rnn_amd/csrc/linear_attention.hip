@@ -76,7 +76,8 @@ constexpr int ESZ = IN == 2 ? 4 : 2;          // bytes per element of q, k, v, d
 constexpr int RP = IN + 1;                    // bfloat16 parts of such an element
 constexpr int L = 32;                         // tokens per block
 constexpr double LOG2E = 1.4426950408889634;
-constexpr double NO_DECAY = -200.0;           // exp of less is zero in fp32; keeps the sums of logarithms finite
+constexpr double NO_DECAY = -200.0;           // keeps the sums of logarithms finite
+constexpr double ZERO_DECAY = -104.0;         // exp of it and less is zero in fp32
 
 enum { BF16 = 0, FP16 = 1, FP32 = 2 };
 
@@ -1115,7 +1116,8 @@ extern "C" __global__ void __launch_bounds__(1024) la_gate(GateArgs a) {
   __syncthreads();
   if (t >= T) return;
   double x = 0.0;
-  if (t < len && (t > 0 || a.init)) {
+  // (a decay of zero carries nothing over: what the sums around it leave is rounding)
+  if (t < len && (t > 0 || a.init) && !(gate_of(a.g, b, h, t) <= ZERO_DECAY)) {
     x = dq;
     int at = blk + 1;
     if (is_border(c0 + at, nreal)) x += sums_k[blk] - dk;

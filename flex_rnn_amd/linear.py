@@ -70,6 +70,7 @@ def linear_attention(q: th.Tensor, k: th.Tensor, v: th.Tensor, g: th.Tensor, sta
     q, k    [B,T,Hk,N]; Hk divides H (heads h * Hk // H share a query and key)
     v       [B,T,H,M], of the same type (bfloat16, float16, float32); M and N from 1 to 256, T from 0
     g       the decay's logarithm, [B,T,H] or [H], float32 or the type of q; -inf forgets everything before the token
+            (and its gradient is zero, as wherever exp(g) is)
     state   [B,H,M,N], float32 or the type of q; None: zero, and the final state is float32
     lengths [B], int64 or int32: sequence b ends after `lengths[b]` tokens (clamped to 0..T); what is behind is not
             looked at, its `y` and gradients are zero, and the final state is the one after the last real token

@@ -738,3 +738,18 @@ def test_how_far_a_number_that_is_not_finite_reaches_in_the_gradient_of_the_deca
         (d if which == 'dy' else xs['qkv'.index(which)])[0, 500, 0, 3] = math.nan
         got = _gradients(_gpu(xs), None, 1.0, d.cuda(), ds.cuda())[5]
         assert th.equal(got[:, keep, 0], clean[:, keep, 0]) and th.equal(got[:, :, 1], clean[:, :, 1]), which
+
+
+@pytest.mark.parametrize('dtype,T,g', [(BF16, 300, 'token'), (FP16, 70, 'token'), (FP32, 600, 'token'), (BF16, 90, 'head')], ids=str)
+@pytest.mark.parametrize('value', [-math.inf, -3e38, -104.0])
+def test_gradient_of_a_decay_that_is_zero_is_zero(dtype, T, g, value):
+    """exp(-104) rounds to zero in 32 bits (its least number is exp(-103.3)): such a token carries nothing over, whatever the
+    sums around it round to."""
+    print(f'case zero decays {dtype} {T} {g} {value}', flush=True)
+    inputs, _ = lc.make(dtype, 2, T, 2, 1, 64, 32, g=g)
+    gen = th.Generator().manual_seed(2)
+    hit = th.rand(inputs[3].shape, generator=gen) < 0.1 if g == 'token' else th.tensor([True, False])
+    inputs[3] = th.where(hit, value, inputs[3])
+    dy, ds = lc.cotangents(inputs)
+    got = _gradients(_gpu(inputs), None, 1.0, dy.cuda(), ds.cuda())[5].cpu()
+    assert bool((got[hit] == 0).all()) and bool((got[~hit] != 0).any())
