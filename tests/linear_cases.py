@@ -71,3 +71,26 @@ def assert_within(got, want, bound, what):
         worst = int(over.argmax())
         assert bool((over <= 0).all()), \
             f'{what}: element {worst} is {float(got.flatten()[worst])}, expected {float(want.flatten()[worst])} within {float(bound.flatten()[worst])}'
+
+
+def bound_of_dg(inputs, lengths, absolute_grads, absolute_state, ds, size):
+    """Bound of the gradient of g [B,T,H], `size` relative to what is summed for a token: q.dq and k.dk of the tokens from its block's
+    start to the next border (blocks of 32; borders in front of every 8th, in front of the last and behind it), and the product of
+    state and gradient there, all of absolute values - the products behind the border are no part of it.  In the |.|-run that
+    product is the gradient of g at the border's own token; behind the last token it is the final state times its gradient."""
+    q, k, v, g, s = inputs
+    B, T, H = v.shape[:3]
+    share = H // q.shape[2]
+    dots = sum((x.double().abs() * absolute_grads[i]).sum(-1).repeat_interleave(share, 2) for i, x in ((0, q), (1, k)))       # [B,T,Hk]: over all its heads
+    upto = th.cat([th.zeros(B, 1, H, dtype=th.float64), dots.cumsum(1)], 1)
+    end = (absolute_state * ds.double().abs()).sum((-1, -2))
+    out = th.zeros(B, T, H, dtype=th.float64)
+    for b in range(B):
+        n = T if lengths is None else max(0, min(T, int(lengths[b])))
+        blocks = (n + 31) // 32
+        for c in range(blocks):
+            at = next(x for x in range(c + 1, blocks + 1) if x % 8 == 0 or x + 1 >= blocks)
+            stop = min(32 * at, n)
+            border = end[b] if stop == n else absolute_grads[3][b, stop]
+            out[b, 32 * c:min(32 * c + 32, n)] = upto[b, stop] - upto[b, 32 * c] + border
+    return out * size

@@ -753,3 +753,89 @@ def test_gradient_of_a_decay_that_is_zero_is_zero(dtype, T, g, value):
     dy, ds = lc.cotangents(inputs)
     got = _gradients(_gpu(inputs), None, 1.0, dy.cuda(), ds.cuda())[5].cpu()
     assert bool((got[hit] == 0).all()) and bool((got[~hit] != 0).any())
+
+
+# every build of the walk that serves g's gradient, over enough blocks for borders and segments
+GRADIENT_BUILDS = [
+    (BF16, 1, 450, 2, 2, 64, 64, {}),
+    (BF16, 1, 450, 2, 1, 64, 64, {}),
+    (BF16, 1, 450, 2, 1, 60, 64, {}),
+    (BF16, 1, 610, 2, 2, 128, 128, {}),
+    (BF16, 1, 450, 4, 2, 128, 96, dict(lengths=(413,))),
+    (BF16, 2, 450, 2, 2, 100, 128, dict(lengths=(450, 390))),
+    (BF16, 1, 400, 1, 1, 256, 256, {}),
+    (BF16, 1, 400, 2, 1, 192, 64, {}),
+    (BF16, 1, 400, 1, 1, 203, 130, {}),
+    (FP16, 1, 450, 2, 2, 64, 64, {}),
+    (FP16, 1, 450, 2, 1, 64, 128, {}),
+    (FP16, 1, 450, 2, 1, 61, 64, {}),
+    (FP16, 1, 610, 2, 2, 128, 128, {}),
+    (FP16, 1, 450, 4, 2, 96, 64, {}),
+    (FP16, 1, 450, 2, 1, 100, 70, dict(resets=0.02)),
+    (FP16, 1, 400, 1, 1, 256, 64, {}),
+    (FP16, 1, 400, 2, 1, 192, 192, {}),
+    (FP16, 1, 400, 1, 1, 201, 64, {}),
+    (FP32, 1, 450, 2, 1, 64, 64, {}),
+    (FP32, 1, 450, 2, 1, 63, 64, {}),
+    (FP32, 1, 450, 2, 2, 128, 128, {}),
+    (FP32, 1, 450, 2, 1, 128, 96, dict(resets=0.02)),
+    (FP32, 1, 450, 2, 2, 101, 100, {}),
+    (FP32, 1, 400, 1, 1, 256, 256, {}),
+    (FP32, 1, 400, 1, 1, 131, 256, {}),
+]
+
+
+def _assert_gradients_within(inputs, lens, scale, dy, ds, got):
+    """Every result of a training step against the 64-bit loop, as close as what stands at `REST` and in `bound_of_dg` says."""
+    q, k, v, g, s = inputs
+    u = lc.HALF_STEP[q.dtype]
+    exact = 2.0 ** -20 + (v.shape[1] + v.shape[3] + q.shape[3]) * 2.0 ** -24
+    rest = exact + REST.get(q.dtype, 0.0)
+    y, sT, grads = lc.run64(inputs, lens, scale, dy, ds)
+    ay, aT, agrads = lc.run64(lc.absolute(inputs), lens, abs(scale), dy.abs(), ds.abs())
+    of_state = lc.HALF_STEP[s.dtype]
+    for name, x, w, a in (('y', got[0], y, ay), ('dq', got[2], grads[0], agrads[0]), ('dk', got[3], grads[1], agrads[1]), ('dv', got[4], grads[2], agrads[2])):
+        lc.assert_within(x, w, u * w.abs() + (1 + u) * rest * a, name)
+    for name, x, w, a in (('state', got[1], sT, aT), ('dstate', got[6], grads[4], agrads[4])):
+        lc.assert_within(x, w, of_state * w.abs() + (1 + of_state) * exact * a, name)
+    lc.assert_within(got[5], grads[3], lc.HALF_STEP[g.dtype] * grads[3].abs() + lc.bound_of_dg(inputs, lens, agrads, aT, ds, exact), 'dg')
+
+
+@pytest.mark.parametrize('case', GRADIENT_BUILDS, ids=str)
+def test_gradients_of_every_build(case):
+    *shape, opts = case
+    print(f'case gradient build {case}', flush=True)
+    inputs, lens = lc.make(*shape, **opts)
+    dy, ds = lc.cotangents(inputs)
+    got = _gradients(_gpu(inputs), None if lens is None else lens.cuda(), 0.7, dy.cuda(), ds.cuda())
+    _assert_gradients_within(inputs, lens, 0.7, dy, ds, got)
+
+
+@pytest.mark.parametrize('dtype', [BF16, FP32], ids=str)
+def test_gradient_of_fast_decays_in_front_of_slow_ones(dtype):
+    from test_linear import fast_then_slow
+    print(f'case fast then slow {dtype}', flush=True)
+    inputs, dy, ds = fast_then_slow(dtype)
+    got = _gradients(_gpu(inputs), None, 1.0, dy.cuda(), ds.cuda())
+    _assert_gradients_within(inputs, None, 1.0, dy, ds, got)
+    # early tokens relative to themselves: a token's products are O(1) numbers of which e^-9 is left, so fp32's 2^-24 of each
+    # of up to 256 + 64 terms is at most 320 2^-24 e^9 of the result
+    want = lc.run64(inputs, None, 1.0, dy, ds)[2][3][:, :256]
+    assert float((got[5].cpu().double()[:, :256] - want).norm()) <= 320 * 2.0 ** -24 * math.exp(9) * float(want.norm())
+
+
+@pytest.mark.parametrize('dtype,M,N', [(BF16, 128, 128), (BF16, 256, 64), (FP16, 128, 256), (FP32, 256, 128)], ids=str)
+def test_layouts_of_wide_heads(dtype, M, N):
+    """Columns far apart, rows at odd addresses and cut out of wider ones give the bits of the plain layout, at every width."""
+    print(f'case layouts {dtype} {M} {N}', flush=True)
+    B, T, H = 1, 400, 2
+    inputs, _ = lc.make(dtype, B, T, H, H, M, N)
+    dy, ds = [t.cuda() for t in lc.cotangents(inputs)]
+    xs = _gpu(inputs)
+    want = _gradients(xs, None, 1.0, dy, ds)
+    columns_apart = lambda x: x.transpose(2, 3).contiguous().transpose(2, 3)       # noqa: E731
+    cut = lambda x: th.cat([x[..., :1], x, x[..., :2]], -1)[..., 1:-2]             # noqa: E731
+    for name, f in (('apart', columns_apart), ('cut', cut)):
+        got = _gradients([f(x) for x in xs[:3]] + xs[3:], None, 1.0, f(dy), ds)
+        for what, a, b in zip(('y', 'state', 'dq', 'dk', 'dv', 'dg', 'dstate'), got, want):
+            assert th.equal(a, b), (name, what)

@@ -303,3 +303,54 @@ def test_a_library_from_other_sources_is_not_taken():
     assert name(sources, 'another PyTorch') != name(sources, th.__version__)
     for f in sources:
         assert name({**sources, f: sources[f] + ' '}, th.__version__) != name(sources, th.__version__)
+
+
+def fast_then_slow(dtype):
+    """Decays that leave e^-9 a token and then hardly any, with cotangents 2^26 times as large behind: what early tokens carry
+    over is nothing against what late ones sum to."""
+    inputs, _ = lc.make(dtype, 1, 700, 2, 1, 32, 32)
+    dy, ds = lc.cotangents(inputs)
+    early = th.arange(700) < 400
+    inputs[3] = th.where(early[None, :, None], -9 + 0.1 * inputs[3], 0.02 * inputs[3])
+    dy = (dy.float() * th.where(early, 1.0, 2.0 ** 26)[None, :, None, None]).to(dtype)
+    return inputs, dy, ds
+
+
+def test_the_bound_of_the_gradient_of_g_refuses_sums_over_a_whole_sequence():
+    """What the borders are for: products rounded to 32 bits, summed from the sequence's end, miss the bound that the GPU's result
+    has to keep; summed from the next border they keep it."""
+    inputs, dy, ds = fast_then_slow(th.float32)
+    y, s, grads = lc.run64(inputs, None, 1.0, dy, ds)
+    ay, a_s, agrads = lc.run64(lc.absolute(inputs), None, 1.0, dy.abs(), ds.abs())
+    bound = lc.bound_of_dg(inputs, None, agrads, a_s, ds, 2.0 ** -20 + (32 + 32 + 700) * 2.0 ** -24)
+    q, k = (x.double().repeat_interleave(2, 2) for x in inputs[:2])
+    v, gate = inputs[2].double(), inputs[3].double()
+    # each head's own dq and dk, by giving it a query and key of its own
+    own = [q, k, v, gate, inputs[4].double()]
+    _, _, each = lc.run64(own, None, 1.0, dy, ds)
+    rounded = [(x * d).sum(-1).float().double() for x, d in ((q, each[0]), (k, each[1]))]
+    exact = [(x * d).sum(-1) for x, d in ((q, each[0]), (k, each[1]))]
+    whole = (rounded[0] - rounded[1]).flip(1).cumsum(1).flip(1) + (s * ds.double()).sum((-1, -2))[:, None]
+    assert bool(((whole - grads[3]).abs() > 10 * bound)[:, :256].any())
+    fine = (exact[0] - exact[1]).flip(1).cumsum(1).flip(1) + (s * ds.double()).sum((-1, -2))[:, None]
+    assert float((fine - grads[3]).abs().max()) < 1e-6 * float(grads[3].abs().max())        # (the formula itself, in 64 bits)
+    spans = th.empty_like(whole)
+    for t0, t1 in ((0, 256), (256, 512), (512, 672), (672, 700)):
+        d = rounded[0][:, t0:t1] - rounded[1][:, t0:t1]
+        border = grads[3][:, t1:t1 + 1] if t1 < 700 else (s * ds.double()).sum((-1, -2))[:, None]
+        spans[:, t0:t1] = d.flip(1).cumsum(1).flip(1) + border
+    assert bool(((spans - grads[3]).abs() <= bound).all())
+
+
+def test_gpu_gradient_cases_reach_every_build_that_serves_the_gradient_of_g():
+    """Each is a code object of its own: the widths of what is staged, the operands' layout, and shared heads choose it."""
+    import test_gpu_linear as t
+    names = {th.bfloat16: 0, th.float16: 1, th.float32: 2}
+    reached = set()
+    for case in t.GRADIENT_BUILDS:
+        dtype, B, T, H, Hk, M, N, opts = case
+        fast = int(M % 8 == 0 and N % 8 == 0)
+        if T > 12 * 32:
+            reached.add((names[dtype], next(w for w in (64, 128, 256) if M <= w), fast, int(bool(fast and H > Hk and dtype != th.float32))))
+    built = {(d['IN'], d['W'], d['FAST'], d['WIDE']) for d in (dict(b[2]) for b in handwritten.builds()) if d.get('DOTS')}
+    assert reached == built
