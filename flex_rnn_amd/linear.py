@@ -12,7 +12,8 @@ Recurrences whose decay differs along the state's columns, or that read the stat
 The kernels are in csrc/linear_attention.hip, their launches and gradients in csrc/frnn_ops.cpp.  Like the compiled operators
 they run on the GPU only, on the current stream of the tensors' device, without synchronising, and can be captured into a HIP
 graph after a first call with the same types, sizes and layouts (a captured backward pass: while no graph of the same leaves
-from the default stream is alive; it says so).  `linear_attention.naive` and `linear_attention.naive_fp64` are the per-token loop
+from the default stream is alive; it says so).  `torch.func.vmap` runs them once per element; a step under vmap and
+`torch.func.grad` are errors.  `linear_attention.naive` and `linear_attention.naive_fp64` are the per-token loop
 in plain PyTorch.
 """
 from __future__ import annotations
@@ -76,8 +77,9 @@ def linear_attention(q: th.Tensor, k: th.Tensor, v: th.Tensor, g: th.Tensor, sta
             looked at, its `y` and gradients are zero, and the final state is the one after the last real token
 
     Any strides.  Sums and the state are fp32.  Differentiable once, backwards, in q, k, v, g and state (a forward-mode tangent is
-    refused); gradients are deterministic.  An infinity or NaN in q, k, v or a result's gradient leaves NaN in what it is a factor
-    of, and nothing else (but in the gradient of g: up to 255 tokens in front of it, too).
+    refused); gradients are deterministic (which of them are asked for may change the last bit of the others).  An infinity or
+    NaN in q, k, v or a result's gradient leaves NaN in what it is a factor of, and nothing else (but in the gradient of g: up to
+    255 tokens in front of it, too).
     """
     _check(q, k, v, g, state, ('B', 'T'), 'linear_attention')
     _check_device('linear_attention', q, k, v, g, state, lengths)

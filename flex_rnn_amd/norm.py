@@ -4,7 +4,7 @@
 
 `weight` and `bias` [C] are the usual norm of a model's width; [H,C] norm each head's output of a recurrence by itself, on
 `[B,T,H,C]` tensors as the operators of this package return them.  The kernels are in csrc/layer_norm.hip; what is said in
-`linear.py` on streams, graphs and devices holds here too.
+`linear.py` on streams, graphs, transforms and devices holds here too.
 """
 from __future__ import annotations
 

@@ -839,3 +839,37 @@ def test_layouts_of_wide_heads(dtype, M, N):
         got = _gradients([f(x) for x in xs[:3]] + xs[3:], None, 1.0, f(dy), ds)
         for what, a, b in zip(('y', 'state', 'dq', 'dk', 'dv', 'dg', 'dstate'), got, want):
             assert th.equal(a, b), (name, what)
+
+
+def test_transforms_of_torch_func():
+    """vmap runs the operators once per element; a step under vmap and func.grad are errors, nothing comes out wrong."""
+    print('case torch.func', flush=True)
+    made = [_gpu(lc.make(FP32, 2, 40, 2, 1, 16, 24, seed=i)[0]) for i in range(3)]
+    q, k, v, g, s = (th.stack(x) for x in zip(*made))
+    y, state = th.func.vmap(F.linear_attention)(q, k, v, g, s)
+    norm = th.func.vmap(F.layer_norm)(v)
+    for i, xs in enumerate(made):
+        want = F.linear_attention(*xs)
+        assert th.equal(y[i], want[0]) and th.equal(state[i], want[1]) and th.equal(norm[i], F.layer_norm(xs[2]))
+    for dims, at in ((0, s), (None, s[0])):
+        with pytest.raises(RuntimeError, match='(?i)batching rule'):
+            th.func.vmap(F.linear_attention_step, in_dims=(0, 0, 0, 0, dims))(q[:, :, 0], k[:, :, 0], v[:, :, 0], g[:, :, 0], at)
+    for f in (lambda x: F.layer_norm(x).sum(), lambda x: F.linear_attention(*made[0][:2], x, *made[0][3:])[0].sum()):
+        with pytest.raises(RuntimeError, match='functorch'):
+            th.func.grad(f)(v[0])
+
+
+def test_a_step_compiles_without_a_break():
+    print('case torch.compile of a step', flush=True)
+    inputs, _ = lc.make(BF16, 2, 1, 4, 2, 64, 64)
+    q, k, v, g = (x[:, 0] for x in _gpu(inputs[:4]))
+    s1 = inputs[4].cuda()
+    s2 = s1.clone()
+
+    def f(q, k, v, g, s):
+        return F.layer_norm(F.linear_attention_step(q, k, v, g, s, scale=0.5))
+
+    compiled = th.compile(f, backend='aot_eager', fullgraph=True)
+    with th.no_grad():
+        for _ in range(3):
+            assert th.equal(compiled(q, k, v, g, s2), f(q, k, v, g, s1)) and th.equal(s1, s2)
