@@ -102,13 +102,18 @@ DEV u32 pack_rne(float a, float b) {           // two floats to bfloat16, to nea
 }
 DEV u32 pack_top(float a, float b) { return __builtin_amdgcn_perm(as_u(b), as_u(a), 0x07060302u); }
 
-// NP parts of the two floats a, b: parts [0, NP-1) by truncation (what is left is exact), the last one to nearest.
+// NP parts of the two floats a, b: the first by truncation (which never overflows), the last to nearest; what is left is exact.
+// With factors of two and three parts, products leave out those of low parts: there the second part is to nearest, too.
+// Truncated, it has the number's sign, and so has what is left out: every product of float32 was 4e-8 too small.  (bfloat16
+// leaves nothing out, and truncation frees its registers earlier.)
 // With INF an infinity is a part by itself; without, it leaves a NaN behind (as its products with zeros would).
 template <int NP, bool INF = false>
 DEV void split2(float a, float b, u32* out, int stride) {
   for (int i = 0; i < NP - 1; i++) {
-    const float ta = as_f(as_u(a) & 0xffff0000u), tb = as_f(as_u(b) & 0xffff0000u);
-    out[i * stride] = pack_top(a, b);
+    const bool cut = i == 0 || RP == 1;
+    const u32 d = cut ? pack_top(a, b) : pack_rne(a, b);
+    const float ta = as_f(cut ? as_u(a) & 0xffff0000u : d << 16), tb = as_f((cut ? as_u(b) : d) & 0xffff0000u);
+    out[i * stride] = d;
     a = INF && a == ta ? 0.f : a - ta;
     b = INF && b == tb ? 0.f : b - tb;
   }
