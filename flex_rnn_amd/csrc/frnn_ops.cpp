@@ -113,7 +113,6 @@ void slice_sums(i64 device, int n, const Tensor* in, const Tensor* out, i64 S) {
 
 // ------------------------------------------------------------------ linear attention
 constexpr i64 TOKENS = 32;            // per block
-constexpr i64 BORDER = 8;             // blocks between the borders at which the gradient of g starts anew
 constexpr i64 UNITS = 256;            // compute units
 constexpr i64 WORKGROUPS = 2 * UNITS; // below this a sequence is split into segments
 constexpr i64 MAX_SEGMENTS = 64;
@@ -143,14 +142,14 @@ struct BlockArgs {
   Job job[2];
   Gate g;
   const void* lengths;
-  i64 B, T, H, nseg, per, tiles;
+  i64 B, T, H, nseg, per, tiles, every;
 };
 struct GateArgs {
   const void *dots_q, *dots_k, *inner;
   Gate g;
   void* dg;
   const void* lengths;
-  i64 B, T, H, tiles, type, init;
+  i64 B, T, H, tiles, type, init, every;
 };
 struct StepArgs {
   Operand q, k, v;
@@ -202,6 +201,7 @@ struct Problem {
   i64 device, B, T, H, Hk, M, N;
   int in;
   Gate g;
+  i64 every;                          // borders at which the gradient of g starts anew: every 2^every blocks
   const void* lengths;
   at::TensorOptions bytes;            // float32 on the device: workspaces
 };
@@ -232,7 +232,7 @@ void walk(const Problem& p, std::initializer_list<Job> jobs, bool dots) {
     fast = fast && j.C % 4 == 0 && j.q.vec == 1 && j.k.vec == 1 && j.v.vec == 1 && j.x.vec == 1;
   }
   const i64 w = width_of(a.job[0].width);
-  a.g = p.g, a.lengths = p.lengths, a.B = p.B, a.T = p.T, a.H = p.H;
+  a.g = p.g, a.lengths = p.lengths, a.B = p.B, a.T = p.T, a.H = p.H, a.every = p.every;
   std::tie(a.nseg, a.per) = segments(n * p.B * p.H * a.tiles, up(p.T, TOKENS));
   const int in = p.in, wc = width_code(w);
   Tensor local, totals;
@@ -269,8 +269,10 @@ void check(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, c
 }
 
 Problem problem(const Tensor& q, const Tensor& v, const Tensor& g, const optional<Tensor>& lengths) {
-  return {q.device().index(), q.size(0), q.size(1), v.size(2), q.size(2), v.size(3), q.size(3), type_of(q.scalar_type()), gate(g), ptr(lengths),
-          q.options().dtype(at::kFloat)};
+  const Gate of_g = gate(g);
+  return {q.device().index(), q.size(0), q.size(1), v.size(2), q.size(2), v.size(3), q.size(3), type_of(q.scalar_type()), of_g,
+          of_g.st == 0 ? 1 : 3,       // (a decay that all tokens share: see la_gate)
+          ptr(lengths), q.options().dtype(at::kFloat)};
 }
 
 Tensor state_like(const Tensor& v, i64 N, const optional<Tensor>& state) {
@@ -301,7 +303,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward(const Tens
   const c10::DeviceGuard guard(q_.device());
   const Tensor q = near(q_), k = near(k_), v = near(v_), dy = near(dy_);
   const Problem p = problem(q, v, g, lengths);
-  const i64 share = p.H / p.Hk, tiles = up(p.N, 64), blocks = up(p.T, TOKENS), borders = up(blocks, BORDER) + 2;
+  const i64 share = p.H / p.Hk, tiles = up(p.N, 64), blocks = up(p.T, TOKENS), borders = up(blocks, 1ll << p.every) + 2;
   Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
   Tensor ds = need_state ? at::empty_like(*state) : at::empty({0}, q.options()), dg;
   // heads that share a query and key each have their own share of its gradient
@@ -325,12 +327,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward(const Tens
   of_v.back = 1, of_v.in_scale = scale;
   Tensor dots, marks, inner;
   if (need_g) {
-    dots = at::empty({2, tiles, p.B * p.H, p.T}, p.bytes);
+    dots = at::empty({2, tiles, p.B * p.H, p.T}, p.bytes.dtype(at::kDouble));
     marks = at::empty({p.B * p.H * borders * up(p.N, 16) * 16 * width_of(p.M)}, p.bytes);
     inner = at::empty({p.B * p.H * borders, tiles * 4}, p.bytes.dtype(at::kDouble));
     for (Job* j : {&of_q, &of_k}) j->marks = marks.data_ptr(), j->inner = inner.data_ptr();
     of_q.pairs = 1, of_q.x = oq, of_q.Hx = p.Hk, of_q.dots = dots.data_ptr();
-    of_k.x = ok, of_k.Hx = p.Hk, of_k.dots = (float*)dots.data_ptr() + dots.numel() / 2;
+    of_k.x = ok, of_k.Hx = p.Hk, of_k.dots = (double*)dots.data_ptr() + dots.numel() / 2;
     // dq's walk multiplies with what dk's wrote down, so it comes later.  dv's goes along with dk's, at the price of dk's
     // three parts of the state, where one kernel serves both and the chip has room for them side by side (B2 T500 H8 64x48
     // fp32: 21 us less); by itself it takes two thirds of the time.
@@ -351,7 +353,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> attention_backward(const Tens
     dg = at::empty(g.sizes(), g.options());
     const bool per_head = g.dim() == 1;
     const Tensor out = per_head ? at::empty({p.B, p.T, p.H}, p.bytes) : dg;
-    const GateArgs a = {dots.data_ptr(), of_k.dots, inner.data_ptr(), p.g, out.data_ptr(), p.lengths, p.B, p.T, p.H, tiles, type_of(out.scalar_type()), state.has_value()};
+    const GateArgs a = {dots.data_ptr(), of_k.dots, inner.data_ptr(), p.g, out.data_ptr(), p.lengths, p.B, p.T, p.H, tiles, type_of(out.scalar_type()), state.has_value(), p.every};
     launch(p.device, key_of(GATE, {}), p.B * p.H * up(blocks, 32), 1, 1024, &a, sizeof a);
     if (per_head) slice_sums(p.device, 1, &out, &dg, p.B * p.T);
   } else {

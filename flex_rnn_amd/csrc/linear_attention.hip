@@ -520,14 +520,13 @@ DEV void store_in(Buffer to, u32 off, f4 x, int n, bool whole) {
   }
 }
 
-// Borders: in front of every BORDER-th block, where the last block begins (the gradient that comes in behind a sequence may be
-// far larger than what is left of it a block earlier) and behind it.
-constexpr int BORDER = 8;
-DEV i64 borders_of(int nall) { return (nall + BORDER - 1) / BORDER + 2; }
-DEV bool is_border(int c, int nreal) { return c % BORDER == 0 || c + 1 >= nreal; }
-DEV i64 border_at(int c, int nreal, int nall) {
-  const int n = (nall + BORDER - 1) / BORDER;
-  return c == nreal ? n : c + 1 == nreal ? n + 1 : c / BORDER;
+// Borders: in front of every (1 << every)-th block, where the last block begins (the gradient that comes in behind a sequence may
+// be far larger than what is left of it a block earlier) and behind it.
+DEV i64 borders_of(int nall, int every) { return ((nall - 1) >> every) + 3; }
+DEV bool is_border(int c, int nreal, int every) { return (c & ((1 << every) - 1)) == 0 || c + 1 >= nreal; }
+DEV i64 border_at(int c, int nreal, int nall, int every) {
+  const int n = ((nall - 1) >> every) + 1;
+  return c == nreal ? n : c + 1 == nreal ? n + 1 : c >> every;
 }
 
 // ================================================================== the walk over a sequence's blocks
@@ -555,7 +554,7 @@ struct Job {
   States init, fin;
   char* out;                // element (b, t, h, column): b * ob + t * ot + h / share * og + h % share * os + column
   i64 ob, ot, og, os, share, out_type;
-  float* dots;              // [column tiles][B*H][T], or null: this job only goes along with one that has them
+  double* dots;             // [column tiles][B*H][T], or null: this job only goes along with one that has them
   float* marks;             // [B*H][borders][ceil(C/16)][W/16][64][4]: written backwards, read forwards
   double* inner;            // [B*H][borders][column tiles][4]: written forwards
   float* local;             // [B*H][nseg-1][column tiles][4][W/16][64][4]: states that segments leave behind, from zero
@@ -568,7 +567,7 @@ struct BlockArgs {
   Job job[2];
   Gate g;
   const i64* lengths;
-  i64 B, T, H, nseg, per, tiles;          // per: blocks per segment; tiles: most column tiles of a job
+  i64 B, T, H, nseg, per, tiles, every;   // per: blocks per segment; tiles: most column tiles of a job; every: of borders
 };
 
 constexpr int NT = W / 16, LT = 2;
@@ -661,10 +660,11 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 #if DOTS
   if (tid < NBUF * LT * L) (&of_rows[0][0][0])[tid] = (&of_cols[0][0][0])[tid] = 0.0;
   // the border in front of block c (behind the last one: c = nreal), of those that count
-  const i64 borders = borders_of(nall);
-  const auto counts = [&](int c) { return job.dots && c > 0 && c <= nreal && is_border(c, nreal); };
+  const int every = (int)args.every;
+  const i64 borders = borders_of(nall, every);
+  const auto counts = [&](int c) { return job.dots && c > 0 && c <= nreal && is_border(c, nreal, every); };
   const auto mark_of = [&](int c) {
-    return (f4*)job.marks + ((bh * borders + border_at(c, nreal, nall)) * ((C + 15) / 16) + cw / 16) * (NT * 64) + lane;
+    return (f4*)job.marks + ((bh * borders + border_at(c, nreal, nall, every)) * ((C + 15) / 16) + cw / 16) * (NT * 64) + lane;
   };
   f4 mark[NT];              // the backward walk's at this block's end, on its way while the block is worked on
   const auto mark_down = [&](int c) {
@@ -689,7 +689,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
         s += (double)(mark[nt][0] * S[nt][0] + mark[nt][1] * S[nt][1]) + (double)(mark[nt][2] * S[nt][2] + mark[nt][3] * S[nt][3]);
     }
     s = read_lane(scan64(s), 63) * all;
-    if (lane == 0) job.inner[((bh * borders + border_at(c, nreal, nall)) * ntiles + tile) * 4 + w] = s;
+    if (lane == 0) job.inner[((bh * borders + border_at(c, nreal, nall, every)) * ntiles + tile) * 4 + w] = s;
   };
 #endif
 
@@ -1018,7 +1018,7 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
       const auto& of = of_state[n % NBUF];
       double s = of[0][lane] + of[1][lane] + (of[2][lane] + of[3][lane]);
       if (job.pairs) s += (of_rows[n % NBUF][0][lane] + of_rows[n % NBUF][1][lane]) - (of_cols[n % NBUF][0][lane] + of_cols[n % NBUF][1][lane]);
-      if (job.dots && t < T) job.dots[((i64)tile * args.B * args.H + bh) * T + t] = (float)(s * job.out_scale);
+      if (job.dots && t < T) job.dots[((i64)tile * args.B * args.H + bh) * T + t] = s * job.out_scale;
     }
     if (back) mark_down(block_of(o));
 #endif
@@ -1072,19 +1072,22 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 // is the result, sums of terms that exp(g_t) is part of: with a fast decay, or an empty state, nothing larger has to cancel.
 // From the first token of a block to the block before, and from one token to the one before it in blocks without a border,
 //     <X, S> + q_t.dq_t - k_t.dk_t.
-// Summed backwards in 64 bits from the nearest border (at most BORDER blocks away), never over a whole sequence, where what
-// is left of a fast decay would drown in the rounding of what came before.  The block's own share of q.dq and k.dk is the same
-// numbers once by rows and once by columns, so it cancels where it should.
+// Summed backwards in 64 bits from the nearest border, never over a whole sequence, where what is left of a fast decay would drown
+// in the rounding of what came before.  Borders stand every eight blocks; every two where all tokens share a decay, whose gradient
+// counts a token's error once for each token in front of it in the span (3 x 4877 tokens, one head, float32, terms that cancel to 1/300:
+// 6e-6 off instead of 3e-5; 8 x 1024 tokens x 32 heads of 128x128 take 531 us instead of 489).  The tokens' products come in 64 bits,
+// too: their rounding to 32 was the largest error of all.  The block's own share of q.dq and k.dk is the same numbers once by rows
+// and once by columns, so it cancels where it should.
 // One workgroup per (batch, head, 32 blocks), a token per thread, a block per half wave.  Bound by waiting for its few loads: 8 us
 // for 8 x 1024 tokens x 32 heads (10 MB).
 struct GateArgs {
-  const float* dots_q;      // [tiles][B*H][T]
-  const float* dots_k;
+  const double* dots_q;     // [tiles][B*H][T]
+  const double* dots_k;
   const double* inner;      // [B*H][borders][parts]
   Gate g;
   char* dg;                 // [B,T,H]
   const i64* lengths;
-  i64 B, T, H, tiles, type, init;     // init: whether there is a state in front of the first token
+  i64 B, T, H, tiles, type, init, every;      // init: whether there is a state in front of the first token
 };
 
 extern "C" __global__ void __launch_bounds__(1024) la_gate(GateArgs a) {
@@ -1093,12 +1096,12 @@ extern "C" __global__ void __launch_bounds__(1024) la_gate(GateArgs a) {
   const int T = (int)a.T, nall = (T + L - 1) / L, groups = (nall + 31) / 32;
   const i64 bh = blockIdx.x / groups, b = bh / a.H, h = bh % a.H, BH = a.B * a.H;
   const int c0 = (int)(blockIdx.x % groups) * 32, c = c0 + blk;
-  const int len = (int)length_of(a.lengths, b, T), nreal = (len + L - 1) / L, parts = 4 * (int)a.tiles;
+  const int len = (int)length_of(a.lengths, b, T), nreal = (len + L - 1) / L, parts = 4 * (int)a.tiles, every = (int)a.every;
   if (tid < 33) {
     const int at = c0 + tid;
     double x = 0.0;
-    if (at > 0 && at <= nreal && is_border(at, nreal)) {
-      const double* from = a.inner + (bh * borders_of(nall) + border_at(at, nreal, nall)) * parts;
+    if (at > 0 && at <= nreal && is_border(at, nreal, every)) {
+      const double* from = a.inner + (bh * borders_of(nall, every) + border_at(at, nreal, nall, every)) * parts;
       for (int i = 0; i < parts; i++) x += from[i];
       if (at < nreal) x *= exp(gate_of(a.g, b, h, (i64)at * L));         // (inside the sequence the walk has yet to decay by it)
     }
@@ -1109,8 +1112,8 @@ extern "C" __global__ void __launch_bounds__(1024) la_gate(GateArgs a) {
   double dq = 0.0, dk = 0.0;
   if (t < len)
     for (i64 k = 0; k < a.tiles; k++) {
-      dq += (double)a.dots_q[(k * BH + bh) * T + t];
-      dk += (double)a.dots_k[(k * BH + bh) * T + t];
+      dq += a.dots_q[(k * BH + bh) * T + t];
+      dk += a.dots_k[(k * BH + bh) * T + t];
     }
   dq = scan32(dq);
   dk = scan32(dk);
@@ -1125,10 +1128,10 @@ extern "C" __global__ void __launch_bounds__(1024) la_gate(GateArgs a) {
   if (t < len && (t > 0 || a.init) && !(gate_of(a.g, b, h, t) <= ZERO_DECAY)) {
     x = dq;
     int at = blk + 1;
-    if (is_border(c0 + at, nreal)) x += sums_k[blk] - dk;
+    if (is_border(c0 + at, nreal, every)) x += sums_k[blk] - dk;
     else {
       x -= dk;
-      for (; !is_border(c0 + at + 1, nreal); at++) x += sums_q[at] - sums_k[at];       // (32 blocks on is a border)
+      for (; !is_border(c0 + at + 1, nreal, every); at++) x += sums_q[at] - sums_k[at];       // (32 blocks on is a border)
       x += sums_q[at++];
     }
     x += ends[at];
