@@ -271,7 +271,7 @@ void check(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, c
 Problem problem(const Tensor& q, const Tensor& v, const Tensor& g, const optional<Tensor>& lengths) {
   const Gate of_g = gate(g);
   return {q.device().index(), q.size(0), q.size(1), v.size(2), q.size(2), v.size(3), q.size(3), type_of(q.scalar_type()), of_g,
-          of_g.st == 0 ? 1 : 3,       // (a decay that all tokens share: see la_gate)
+          of_g.st == 0 ? 0 : 3,       // (a decay that all tokens share: see la_gate)
           ptr(lengths), q.options().dtype(at::kFloat)};
 }
 

@@ -1073,9 +1073,9 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 // From the first token of a block to the block before, and from one token to the one before it in blocks without a border,
 //     <X, S> + q_t.dq_t - k_t.dk_t.
 // Summed backwards in 64 bits from the nearest border, never over a whole sequence, where what is left of a fast decay would drown
-// in the rounding of what came before.  Borders stand every eight blocks; every two where all tokens share a decay, whose gradient
+// in the rounding of what came before.  Borders stand every eight blocks; at every block where all tokens share a decay, whose gradient
 // counts a token's error once for each token in front of it in the span (3 x 4877 tokens, one head, float32, terms that cancel to 1/300:
-// 6e-6 off instead of 3e-5; 8 x 1024 tokens x 32 heads of 128x128 take 531 us instead of 489).  The tokens' products come in 64 bits,
+// 3e-5 off with eight blocks, 6e-6 with two, 1e-6 with one; 8 x 1024 tokens x 32 heads of 128x128 take 489, 531 and 620 us).  The tokens' products come in 64 bits,
 // too: their rounding to 32 was the largest error of all.  The block's own share of q.dq and k.dk is the same numbers once by rows
 // and once by columns, so it cancels where it should.
 // One workgroup per (batch, head, 32 blocks), a token per thread, a block per half wave.  Bound by waiting for its few loads: 8 us
