@@ -197,11 +197,19 @@ std::pair<i64, i64> segments(i64 groups, i64 blocks) {
   return {up(blocks, per), per};
 }
 
+// Borders at which the gradient of g starts anew, every 2^n blocks (see la_gate): at each for a decay that all tokens share, as long as
+// the states that are written down there (a state of N rounded up to 16 by M rounded up to 64, 128 or 256, in fp32) take 8 GiB at most.
+i64 every_of(i64 B, i64 T, i64 H, i64 M, i64 N, bool shared) {
+  i64 n = shared ? 0 : 3;
+  while (n < 3 && B * H * up(up(T, TOKENS), 1ll << n) > (1ll << 31) / (up(N, 16) * 16 * width_of(M))) n++;
+  return n;
+}
+
 struct Problem {
   i64 device, B, T, H, Hk, M, N;
   int in;
   Gate g;
-  i64 every;                          // borders at which the gradient of g starts anew: every 2^every blocks
+  i64 every;                          // of borders
   const void* lengths;
   at::TensorOptions bytes;            // float32 on the device: workspaces
 };
@@ -271,7 +279,7 @@ void check(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, c
 Problem problem(const Tensor& q, const Tensor& v, const Tensor& g, const optional<Tensor>& lengths) {
   const Gate of_g = gate(g);
   return {q.device().index(), q.size(0), q.size(1), v.size(2), q.size(2), v.size(3), q.size(3), type_of(q.scalar_type()), of_g,
-          of_g.st == 0 ? 0 : 3,       // (a decay that all tokens share: see la_gate)
+          every_of(q.size(0), q.size(1), v.size(2), v.size(3), q.size(3), of_g.st == 0),
           ptr(lengths), q.options().dtype(at::kFloat)};
 }
 
@@ -736,6 +744,7 @@ TORCH_LIBRARY_IMPL(flex_rnn, Autograd, m) {
 extern "C" {
 void frnn_ops_set_loader(Loader loader) { g_loader = loader; }
 void frnn_ops_segments(i64 groups, i64 blocks, i64* out) { std::tie(out[0], out[1]) = segments(groups, blocks); }
+i64 frnn_ops_every(i64 B, i64 T, i64 H, i64 M, i64 N, i64 shared) { return every_of(B, T, H, M, N, shared != 0); }
 void frnn_ops_norm_shape(i64 rows, i64 heads, i64 C, i64 size, i64* out) {      // wide, threads, pieces, lanes, teams
   const Shape s = shape_of(C, size);
   out[0] = s.wide, out[1] = s.threads, out[2] = s.pieces, out[3] = s.lanes, out[4] = teams_of(rows, heads, s.lanes);

@@ -210,6 +210,12 @@ def segments(groups: int, blocks: int) -> Tuple[int, int]:
     return out[0], out[1]
 
 
+def blocks_between_borders(B: int, T: int, H: int, M: int, N: int, shared: bool) -> int:
+    f = load().frnn_ops_every
+    f.restype = ctypes.c_int64
+    return 1 << f(*(ctypes.c_int64(x) for x in (B, T, H, M, N, shared)))
+
+
 def norm_shape(rows: int, heads: int, C: int, size: int) -> Dict[str, int]:
     out = (ctypes.c_int64 * 5)()
     load().frnn_ops_norm_shape(ctypes.c_int64(rows), ctypes.c_int64(heads), ctypes.c_int64(C), ctypes.c_int64(size), out)

@@ -906,3 +906,23 @@ def test_gradient_of_a_decay_that_all_tokens_share():
         got = _gradients(_gpu(inputs), None, 1.0, dy.cuda(), ds.cuda())[5]
         off.append(float((got.cpu().double() - grads[3]).abs() / (math.sqrt(256 * n) * 2.0 ** -24 * each)))
     assert sum(x * x for x in off) / len(off) < 1.0, off
+
+
+@pytest.mark.parametrize('H,blocks', [(5, 2), (9, 4)])
+def test_borders_further_apart_for_shared_decays_of_long_sequences(H, blocks):
+    """Where states at every block would not fit: a shared decay's gradient against the sum of the gradients of the same decays per
+    token.  Each q.dq and k.dk, rounded to 32 bits (0.41 2^-24 in the mean square), counts up to 256 times there (148 in the
+    mean square) and 128 times here (74): 91 2^-24 times the root of the number of tokens times the products; four times that."""
+    from flex_rnn_amd import handwritten
+    print(f'case borders apart {H}', flush=True)
+    T, M, N = 2 ** 18, 256, 256
+    assert handwritten.blocks_between_borders(1, T, H, M, N, True) == blocks
+    gen = th.Generator(device='cuda').manual_seed(0)
+    randn = lambda *s: th.randn(*s, generator=gen, device='cuda')  # noqa: E731
+    q, k, v, dy = randn(1, T, H, N).to(BF16), (randn(1, T, H, N) / 16).to(BF16), randn(1, T, H, M).to(BF16), randn(1, T, H, M).to(BF16)
+    g = -0.02 - 0.3 * th.rand(H, generator=gen, device='cuda')
+    back = th.ops.flex_rnn.linear_attention_backward
+    dq, dk, _, shared, _ = back(q, k, v, g, None, None, dy, None, 1.0, True, False)
+    each = ((q.float() * dq.float()).sum(-1).square() + (k.float() * dk.float()).sum(-1).square()).mean(1).sqrt()[0]
+    apart = back(q, k, v, g.expand(1, T, H).contiguous(), None, None, dy, None, 1.0, True, False)[3].double().sum((0, 1))
+    assert bool(((shared.double() - apart).abs() <= 4 * 91 * 2.0 ** -24 * math.sqrt(T) * each.double()).all())

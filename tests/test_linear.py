@@ -354,3 +354,18 @@ def test_gpu_gradient_cases_reach_every_build_that_serves_the_gradient_of_g():
             reached.add((names[dtype], next(w for w in (64, 128, 256) if M <= w), fast, int(bool(fast and H > Hk and dtype != th.float32))))
     built = {(d['IN'], d['W'], d['FAST'], d['WIDE']) for d in (dict(b[2]) for b in handwritten.builds()) if d.get('DOTS')}
     assert reached == built
+
+
+def test_borders_of_shared_decays_fit_in_memory():
+    """Between borders lie 8 blocks for decays per token; one for a shared decay, more where what is written down at them would
+    take over 8 GiB."""
+    every = handwritten.blocks_between_borders
+    assert every(8, 1024, 32, 128, 128, False) == 8 and every(1, 2 ** 24, 64, 256, 256, False) == 8
+    assert every(8, 1024, 32, 128, 128, True) == 1 and every(1, 0, 1, 1, 1, True) == 1
+    last = 1
+    for T in (2 ** 15, 2 ** 17, 2 ** 18, 2 ** 19, 2 ** 21, 2 ** 31 - 65):
+        n = every(1, T, 32, 128, 128, True)
+        size = 32 * -(-T // (32 * n)) * 128 * 128 * 4
+        assert last <= n <= 8 and (size <= 2 ** 33 or n == 8) and (n == 1 or 2 * size > 2 ** 33)
+        last = n
+    assert last == 8
