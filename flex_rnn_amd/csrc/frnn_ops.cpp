@@ -188,7 +188,9 @@ States states(const optional<Tensor>& s, bool rows_m) {
 // walk over k and v for the state at their starts, about half as long as the first, and a launch, about three blocks long:
 // from 12 blocks on, segments of four and more win (T777, 24 workgroups: 53 us in two, 32 us in six).  Two workgroups per unit
 // are worth up to 16 segments (T8192 H16 128x128: 97 us, 108 with one per unit); more, whose states each segment adds up, only
-// reach for one (T16384 H4: 68 us in 32 segments, 84 in 64; T65536 H2: 91 in 64, 137 in 32).
+// reach for one (T16384 H4: 68 us in 32 segments, 84 in 64; T65536 H2: 91 in 64, 137 in 32).  All of these are bfloat16 or small
+// heads, of which two workgroups fit a unit, and at most 64 walks: builds of which one fits (float16 over 128 columns, float32 over 64)
+// and 65 to 511 walks go by the same rule unmeasured.
 std::pair<i64, i64> segments(i64 groups, i64 blocks) {
   groups = std::max<i64>(groups, 1);
   const i64 n = std::min(std::max(std::min<i64>(up(WORKGROUPS, groups), 16), std::min(up(UNITS, groups), MAX_SEGMENTS)), blocks / 4);
@@ -396,7 +398,7 @@ Tensor attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const T
 }
 
 // ------------------------------------------------------------------ layer norm
-constexpr i64 THREADS = 256 * 2 * 256;      // in flight: two workgroups of 256 per compute unit (measured from one half to sixteen: 5.0 TB/s at two, 3.9 at eight)
+constexpr i64 THREADS = 256 * 2 * 256;      // in flight: two workgroups of 256 per compute unit (measured on the forward pass over rows of 128, from one half to sixteen: 5.0 TB/s at two, 3.9 at eight; the backward pass and rows of a workgroup go by it, too)
 
 struct NormArgs {
   const void *x, *dy;

@@ -537,12 +537,14 @@ DEV i64 border_at(int c, int nreal, int nall, int every) {
 // columns of y, the block's own share, and updates its state.  The operands of blocks to come are on their way into
 // registers meanwhile.
 //
-// What bounds it: a block's instructions.  With 8 x 1024 tokens x 32 heads of 128x128 in bfloat16, two workgroups per unit, a walk
-// takes 100 us (its four tensors alone: 53 us at the rate of a large copy); the vector pipes are busy 33 % of the time, the matrix
-// cores 19 %, LDS 41 % (a third of that bank conflicts of the reads down columns), and waves wait for loads and barriers 37 % of
-// theirs: four phases of one wave, of which two waves per SIMD hide each other only in part.  Blocks of 64 tokens took longer
-// (P and its products grow with the block, and the tiles leave room for one workgroup), as did every other row stride in LDS.
-// With DOTS: 150 us, the state as three parts (24 of 64 matrix products) and the sums in 64 bits.
+// What bounds it: latency.  With 8 x 1024 tokens x 32 heads of 128x128 in bfloat16, two workgroups per unit, a walk takes 105 us
+// (its four tensors alone: 53 us at the rate of a large copy), and no pipe is near its limit: the vector pipes are busy 42 % of the
+// time, the matrix cores 21 %, LDS 40 % (a third of that bank conflicts of the reads down columns), and waves wait for loads and
+// barriers a third of theirs.  A block is four phases of one wave that follow each other, and two waves per SIMD hide each other
+// only in part.  Blocks of 64 tokens took longer (P and its products grow with the block, and the tiles leave room for one
+// workgroup), as did every other row stride in LDS; swapping pieces of rows instead has not been tried.
+// With DOTS: dk 148 us (it also writes the states at borders, 84 MB), dq 158 us (it reads them), the state as three parts (24 of 58
+// matrix products) and the sums in 64 bits.
 //
 // With DOTS the walk also leaves, per token, what the gradient of g is made of (see la_gate): forwards (dq) the products
 // q_i.dq_i with the block's own share taken from unrounded numbers, less the share of each j; backwards (dk) the products
@@ -1074,12 +1076,12 @@ extern "C" __global__ void __launch_bounds__(256, OCC) la_block(BlockArgs args) 
 //     <X, S> + q_t.dq_t - k_t.dk_t.
 // Summed backwards in 64 bits from the nearest border, never over a whole sequence, where what is left of a fast decay would drown
 // in the rounding of what came before.  Borders stand every eight blocks; at every block where all tokens share a decay, whose gradient
-// counts a token's error once for each token in front of it in the span (3 x 4877 tokens, one head, float32, terms that cancel to 1/300:
-// 3e-5 off with eight blocks, 6e-6 with two, 1e-6 with one; 8 x 1024 tokens x 32 heads of 128x128 take 489, 531 and 620 us).  The tokens' products come in 64 bits,
-// too: their rounding to 32 was the largest error of all.  The block's own share of q.dq and k.dk is the same numbers once by rows
-// and once by columns, so it cancels where it should.
-// One workgroup per (batch, head, 32 blocks), a token per thread, a block per half wave.  Bound by waiting for its few loads: 8 us
-// for 8 x 1024 tokens x 32 heads (10 MB).
+// counts a token's error once for each token in front of it in the span (3 x 4877 tokens, one head, float32, terms that cancel to
+// 1/300: 3e-5 off with eight blocks, 6e-6 with two, 1e-6 with one; a training step of 8 x 1024 tokens x 32 heads of 128x128 takes
+// 489, 531 and 620 us).  The tokens' products come in 64 bits, too: their rounding to 32 was the largest error of all.  The block's
+// own share of q.dq and k.dk is the same numbers once by rows and once by columns, so it cancels where it should.
+// One workgroup per (batch, head, 32 blocks), a token per thread, a block per half wave.  Bound by waiting for its few loads: 10 us
+// for 8 x 1024 tokens x 32 heads (25 MB).
 struct GateArgs {
   const double* dots_q;     // [tiles][B*H][T]
   const double* dots_k;
