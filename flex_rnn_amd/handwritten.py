@@ -9,6 +9,7 @@ library's file name holds their hash (and PyTorch's version, whose C++ interface
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import glob
 import hashlib
@@ -161,7 +162,8 @@ def build_library(verbose: bool = False) -> str:
     os.replace(tmp, OPS_PATH)
     for old in glob.glob(os.path.join(_HERE, 'libfrnn_ops*.so')):
         if old != OPS_PATH:
-            os.remove(old)
+            with contextlib.suppress(FileNotFoundError):         # (another process builds, too)
+                os.remove(old)
     return OPS_PATH
 
 
